@@ -429,6 +429,24 @@ int v1t_inputs_multi(const float* const* images, const float* const* behaviors, 
  * (s_memtime / s_memrealtime) and the cycles per MFMA and SIMD. Allocates and frees its own few KB; synchronises `stream`. */
 int v1t_mfma_peak_probe(int iters, int waves_per_simd, double* tflops, double* ghz, double* cycles_per_mfma, void* stream);
 
+/* Rotary positions with several axes (no reference counterpart: its cores add a learned or a sine table, vit.py:101-106, cct.py:17-27). One pass
+ * over up to two operands (q and k) of (B, T, heads, D) elements with unit stride in D: token t of sequence b has position[a] on each of n_axes
+ * (1..4) axes; axis a turns sections[a] pairs of a head's features, in order; pair number i of an axis of s pairs turns by
+ * position * base^(-i / s) (shared = 0) or, with j counting the P = sum(sections) pairs of all axes, by position * base^(-j / P) (shared = 1).
+ * halves = 0: pair j is features (2j, 2j + 1); 1: (j, P + j). Features >= 2P are copied. inverse: by the negated angles (the backward pass).
+ * y may be x (same pointer and strides: in place); any other overlap of y with x, of two tokens' rows of y, or of y with positions is the
+ * caller's error. dtype 0 = bf16, 1 = fp16, 2 = fp32; position_type 0 = int32, 1 = int64 (exact below 2^53), 2 = fp32; strides in elements,
+ * any sign; pos_stride_b 0 = one set of positions for all sequences. P <= 256. */
+typedef struct v1t_rotary_operand {
+    const void* x;
+    void* y;
+    long long x_stride_b, x_stride_t, x_stride_h, y_stride_b, y_stride_t, y_stride_h;
+    int heads, pad_;
+} v1t_rotary_operand;
+int v1t_rotary(const v1t_rotary_operand* operands, int n_operands, int dtype, int B, int T, int D, const int* sections, int n_axes, double base, int shared,
+               int halves, int inverse, const void* positions, int position_type, long long pos_stride_b, long long pos_stride_t, long long pos_stride_a,
+               void* stream);
+
 /* LayerNorm (vit.py:220,145) forward: z bf16 (rows, DP) = LN(x (+ inject[b])) ; backward: see
  * csrc/elementwise.h LnBwdArgs (gout = gin + dLN; optional token-sum, next-branch cast + bias colsum) */
 int v1t_layernorm_forward(const float* x, const float* inject, float* xout, const float* gamma,

@@ -51,6 +51,11 @@ class AdamRange(C.Structure):
     _fields_ = [("p", c_void_p), ("g", c_void_p), ("m", c_void_p), ("v", c_void_p), ("n", c_ll), ("lr", c_float), ("l1", c_float), ("step", c_int), ("pad_", c_int)]
 
 
+class RotaryOperand(C.Structure):
+    """`v1t_rotary_operand`: one tensor of `v1t_rotary`, its strides in elements."""
+    _fields_ = [("x", c_void_p), ("y", c_void_p), ("xb", c_ll), ("xt", c_ll), ("xh", c_ll), ("yb", c_ll), ("yt", c_ll), ("yh", c_ll), ("heads", c_int), ("pad_", c_int)]
+
+
 # name -> (restype, argtypes); every symbol declared in include/v1t_amd.h
 SIGNATURES: t.Dict[str, t.Tuple[t.Any, t.List[t.Any]]] = {
     "v1t_abi_version": (c_int, []),
@@ -130,6 +135,8 @@ SIGNATURES: t.Dict[str, t.Tuple[t.Any, t.List[t.Any]]] = {
     "v1t_attention_probs": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]),
     "v1t_rollout_vecmat": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "v1t_rollout_matmul": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
+    "v1t_rotary": (c_int, [C.POINTER(RotaryOperand), c_int, c_int, c_int, c_int, c_int, C.POINTER(c_int), c_int, C.c_double, c_int, c_int, c_int, c_void_p, c_int,
+                           c_ll, c_ll, c_ll, c_void_p]),
     "v1t_profile_enable": (c_int, [c_int, c_int]),
     "v1t_profile_read": (c_int, [C.POINTER(c_int), C.POINTER(C.c_double)]),
     "v1t_layernorm_forward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_void_p]),
@@ -185,6 +192,20 @@ def stream() -> int:
 def require_cuda(x: torch.Tensor, what: str) -> None:
     if not x.is_cuda:
         raise RuntimeError(f"v1t_amd {what}: tensor is on {x.device}; the HIP path needs a GPU tensor (no CPU fallback).")
+
+
+def leaf_in_capture(x: torch.Tensor, what: str) -> None:
+    """Called by an operator's differentiable forward for each tensor it saves a gradient path to. The node that receives a leaf's gradient belongs to
+    the stream of the first pass that used the leaf, for as long as any graph of that pass lives; a backward pass captured meanwhile on another
+    stream would wait on that stream inside the capture, which ends the process when the capture ends. So an eager pass marks the node with its
+    stream, and a captured pass that finds another stream's mark is refused."""
+    if not (x.is_leaf and x.requires_grad):
+        return
+    here = torch.cuda.current_stream(x.device).cuda_stream
+    made_on = torch.autograd.graph.get_gradient_edge(x).node.metadata.setdefault("v1t_stream", here)
+    if made_on != here and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"v1t_amd {what}: a graph of an earlier pass over the same leaf tensor is still alive on another stream; its backward cannot be "
+                           "captured beside it. Drop that pass's outputs (del) before the capture.")
 
 
 def grad_sink(p):

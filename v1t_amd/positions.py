@@ -1,0 +1,175 @@
+"""Rotary positions with several axes - a patch's row and column, a frame's time - on the queries and keys of an attention.
+
+The reference's cores add a table of positions to the tokens (a learned one, core/vit.py:101-106; sines, core/cct.py:17-27): its length is
+the training grid's. A rotation of q and k by the position makes their product depend on the distance of two tokens alone, for any grid
+and any clip length. `ViTCore` / `CCTCore` run it in every block (`args.rotary`); `rotary` is the same operator for a core of one's own."""
+from __future__ import annotations
+
+import ctypes as C
+import typing as t
+
+import torch
+
+from . import lib as L
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_LAYOUTS = {"pairs": 0, "halves": 1}
+MAX_PAIRS = 256
+
+
+class _Turn(t.NamedTuple):
+    sections: t.Tuple[int, ...]
+    base: float
+    shared: int
+    halves: int
+    inverse: int
+
+
+def _check(q: torch.Tensor, k: t.Optional[torch.Tensor], positions: torch.Tensor, sections, base: float, layout: str) -> t.Tuple[int, ...]:
+    sections = tuple(int(s) for s in sections)
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or sum(sections) < 1:
+        raise ValueError(f"rotary: sections are 1 to 4 non-negative numbers of pairs, got {sections}")
+    if sum(sections) > MAX_PAIRS:
+        raise ValueError(f"rotary: {sum(sections)} pairs a head, at most {MAX_PAIRS} are supported")
+    if layout not in _LAYOUTS:
+        raise ValueError(f"rotary: layout is 'pairs' or 'halves', got {layout!r}")
+    if not 0.0 < float(base) < float("inf"):
+        raise ValueError(f"rotary: base must be positive and finite, got {base}")
+    for x in (q, k):
+        if x is None:
+            continue
+        if x.dim() not in (3, 4):
+            raise ValueError(f"rotary: q and k are (tokens, heads, features) or (batch, tokens, heads, features), got {tuple(x.shape)}")
+        if x.dtype not in _DTYPES or x.dtype != q.dtype:
+            raise TypeError(f"rotary: q and k share one of {list(_DTYPES)}, got {[y.dtype for y in (q, k) if y is not None]}")
+        if 2 * sum(sections) > x.shape[-1]:
+            raise ValueError(f"rotary: {sum(sections)} pairs need {2 * sum(sections)} features a head, got {x.shape[-1]}")
+        if x.device != q.device or x.shape[:-2] != q.shape[:-2] or x.shape[-1] != q.shape[-1]:
+            raise ValueError(f"rotary: q and k share device, batch, tokens and features, got {tuple(q.shape)} on {q.device} and {tuple(x.shape)} on {x.device}")
+        if x.shape[-2] < 1:
+            raise ValueError("rotary: no heads")
+    if positions.dtype not in _POSITION_TYPES:
+        raise TypeError(f"rotary: positions are one of {list(_POSITION_TYPES)}, got {positions.dtype}")
+    if positions.requires_grad:
+        raise ValueError("rotary: no gradient with respect to positions")
+    ok = (q.shape[-3], len(sections))
+    if positions.device != q.device or tuple(positions.shape) not in ((ok, (q.shape[0],) + ok) if q.dim() == 4 else (ok,)):
+        raise ValueError(f"rotary: positions are (tokens, axes) = {ok} - or (batch, tokens, axes) - on {q.device}, got {tuple(positions.shape)} on {positions.device}")
+    return sections
+
+
+def _launch(turn: _Turn, positions: torch.Tensor, pairs_of: t.Sequence[t.Tuple[torch.Tensor, torch.Tensor]]) -> None:
+    """One launch over [(x, y), ...]; x and y have unit stride in their last dimension."""
+    x0 = pairs_of[0][0]
+    if x0.numel() == 0:
+        return
+    if x0.device.index != torch.cuda.current_device():
+        with torch.cuda.device(x0.device):
+            return _launch(turn, positions, pairs_of)
+    four = x0.dim() == 4
+    ops = (L.RotaryOperand * len(pairs_of))()
+    for o, (x, y) in zip(ops, pairs_of):
+        sx, sy = x.stride(), y.stride()
+        o.x, o.y, o.heads = x.data_ptr(), y.data_ptr(), x.shape[-2]
+        o.xb, o.xt, o.xh = (sx[0], sx[1], sx[2]) if four else (0, sx[0], sx[1])
+        o.yb, o.yt, o.yh = (sy[0], sy[1], sy[2]) if four else (0, sy[0], sy[1])
+    sp = positions.stride()
+    n = len(turn.sections)
+    L.check(L.load().v1t_rotary(ops, len(pairs_of), _DTYPES[x0.dtype], x0.shape[0] if four else 1, x0.shape[-3], x0.shape[-1], (C.c_int * n)(*turn.sections), n,
+                                turn.base, turn.shared, turn.halves, turn.inverse, positions.data_ptr(), _POSITION_TYPES[positions.dtype],
+                                sp[0] if positions.dim() == 3 else 0, sp[-2], sp[-1], L.stream()), "rotary")
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, turn: _Turn, positions: torch.Tensor, q: torch.Tensor, k: t.Optional[torch.Tensor]):
+        ctx.set_materialize_grads(False)
+        ctx.turn = turn
+        for x in (q, k):
+            if x is not None:
+                L.leaf_in_capture(x, "rotary")
+        ctx.save_for_backward(positions)
+        xs = [_rows(x) for x in (q, k) if x is not None]
+        ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+        _launch(turn, positions, list(zip(xs, ys)))
+        return ys[0] if k is None else tuple(ys)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        """A rotation is orthogonal: the gradient turns back. Differentiable itself (a second derivative turns forward again)."""
+        (positions,) = ctx.saved_tensors
+        back = ctx.turn._replace(inverse=1 - ctx.turn.inverse)
+        out: t.List[t.Optional[torch.Tensor]] = [None, None]
+        which = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[2 + i]]
+        if len(which) == 2:
+            out = list(_RotaryFn.apply(back, positions, *grads))
+        elif which:
+            out[which[0]] = _RotaryFn.apply(back, positions, grads[which[0]], None)
+        return (None, None, *out)
+
+
+def rotary(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int], k: t.Optional[torch.Tensor] = None, base: float = 10000.0,
+           layout: str = "pairs", shared: bool = False, inverse: bool = False):
+    """q (and k) turned by their tokens' positions: new contiguous tensors; differentiable in q and k.
+
+    q: (batch, tokens, heads, features) or (tokens, heads, features), bf16 / fp16 / fp32, any strides; k: the same with its own number of heads.
+    positions: (tokens, axes) for all sequences, or (batch, tokens, axes); int32, int64 or fp32, negative ones too. A token at 0 on every axis is
+    left as it is (a class token).
+    sections: pairs of features that each axis turns, in order; pair i of an axis with s pairs turns by position * base^(-i / s), or - `shared` - the
+    P pairs of all axes share one ladder, pair j turns by position * base^(-j / P). layout: pair j is features (2j, 2j + 1), "pairs", or (j, P + j),
+    "halves". Features behind the 2P turned ones are copied.
+    Angles are reduced in 64 bits (exact positions up to 2^53); products are fp32, rounded once to the tensor's type."""
+    sections = _check(q, k, positions, sections, base, layout)
+    L.require_cuda(q, "rotary")
+    turn = _Turn(sections, float(base), int(bool(shared)), _LAYOUTS[layout], int(bool(inverse)))
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _RotaryFn.apply(turn, positions, q, k)
+    xs = [_rows(x) for x in (q, k) if x is not None]
+    ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+    _launch(turn, positions, list(zip(xs, ys)))
+    return ys[0] if k is None else tuple(ys)
+
+
+def _apart(q: torch.Tensor, k: torch.Tensor) -> bool:
+    """Whether no element of q is one of k: whole ranges apart, or - views of one packed projection - apart within every token's row."""
+    if q.numel() == 0 or k.numel() == 0 or q.untyped_storage().data_ptr() != k.untyped_storage().data_ptr():
+        return True
+
+    def extent(x, dims):
+        return 1 + sum((n - 1) * s for n, s in zip(x.shape[dims:], x.stride()[dims:]))
+
+    a, b = q.storage_offset(), k.storage_offset()
+    (lo, x), (hi, y) = ((a, q), (b, k)) if a <= b else ((b, k), (a, q))
+    if lo + extent(x, 0) <= hi:
+        return True
+    outer = [(n, s) for n, s in zip(x.shape[:-2], x.stride()[:-2]) if n > 1]
+    same = outer == [(n, s) for n, s in zip(y.shape[:-2], y.stride()[:-2]) if n > 1]
+    return same and lo + extent(x, -2) <= hi and hi - lo + extent(y, -2) <= min((s for _, s in outer), default=1 << 62)
+
+
+def rotary_(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int], k: t.Optional[torch.Tensor] = None, base: float = 10000.0,
+            layout: str = "pairs", shared: bool = False, inverse: bool = False):
+    """`rotary` in place, outside autograd (a new token's q and k, a projection's buffer): the same values, features behind the turned ones untouched."""
+    sections = _check(q, k, positions, sections, base, layout)
+    xs = [x for x in (q, k) if x is not None]
+    for x in xs:
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError("rotary_: a tensor that requires grad cannot be turned in place; use rotary")
+        if x.stride(-1) != 1 and x.shape[-1] > 1:
+            raise ValueError(f"rotary_: unit stride in the last dimension is needed, got strides {x.stride()}")
+        dims = sorted((s, n) for s, n in zip(x.stride(), x.shape) if n > 1)
+        if any(s < prev_s * prev_n for (prev_s, prev_n), (s, _) in zip(dims, dims[1:])) or any(s == 0 for s, _ in dims):
+            raise ValueError(f"rotary_: elements of an expanded or overlapping view cannot be turned in place, got shape {tuple(x.shape)}, strides {x.stride()}")
+    if k is not None and not _apart(q, k):
+        raise ValueError("rotary_: q and k share elements")
+    L.require_cuda(q, "rotary_")
+    _launch(_Turn(sections, float(base), int(bool(shared)), _LAYOUTS[layout], int(bool(inverse))), positions, [(x, x) for x in xs])
+    for x in xs:
+        if not x.is_inference():
+            torch.autograd.graph.increment_version(x)
+    return xs[0] if k is None else tuple(xs)
