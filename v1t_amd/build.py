@@ -18,7 +18,9 @@ LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libv1t_amd.so")
 SOURCES = ["api.hip", "gemm.hip", "attention.hip", "elementwise.hip", "readout.hip", "gridprep.hip", "metrics.hip", "data.hip", "probe.hip", "tails.hip", "rotary.hip"]
 HEADERS = ["common.h", "gemm.h", "attention.h", "elementwise.h", "readout.h", "gridprep.h", os.path.join("..", "..", "include", "v1t_amd.h")]
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result"]
+# -packed-fp32-ops: no packed fp32 VALU instructions (v_pk_add / mul / fma_f32), which the compiler makes of ordinary float code; some of their forms
+# have given wrong results on this hardware now and then
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result", "-Wno-unknown-warning-option", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 EXTRA = os.environ.get("V1T_HIPCC_EXTRA", "").split()  # dev: extra compiler flags (ablations)
 # attention: no SLP vectorisation - packed f32 VALU (v_pk_mul_f32 / v_pk_fma_f32) beside MFMAs issue slower than the two scalar
 # instructions they replace (MI355X_MICROARCH.md; A/B in one process: forward -3.8 %, backward -1 %)
