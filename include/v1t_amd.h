@@ -447,6 +447,32 @@ int v1t_rotary(const v1t_rotary_operand* operands, int n_operands, int dtype, in
                int halves, int inverse, const void* positions, int position_type, long long pos_stride_b, long long pos_stride_t, long long pos_stride_a,
                void* stream);
 
+/* Orthogonalised updates (no reference counterpart: train.py:216-223 steps every parameter with AdamW). For each of n matrices U (rows x cols), on its
+ * own: X = U / (|U|_F + eps) with the shorter side first; `steps` times (<= 32) A = X X^T, X <- a X + (b A + c A A) X with the step's
+ * (a, b, c) = coefficients[3k .. 3k + 2] (host memory); the result in U's shape. fp32 arithmetic throughout whatever the dtype (0 = bf16, 1 = fp16, 2 = fp32 of
+ * `in` and `out`), rounded once. Coefficients that let a plane of the iteration grow to 128 or more (their bound over all singular values in
+ * [0, 1]) are refused. `in` has element strides of any sign, `out` is row-major without gaps and overlaps no `in` of the call but its own, where that is
+ * laid out alike. m = min(rows, cols) <= 32768, rows * cols <= 2^31. Deterministic. The workspace is 16-byte aligned. */
+typedef struct v1t_matrix {
+    const void* in;
+    void* out;
+    long long row_stride, col_stride;
+    int rows, cols;
+} v1t_matrix;
+long long v1t_orthogonalize_ws_bytes(const int* rows, const int* cols, int n); /* also v1t_muon_step's; negative = error code */
+int v1t_orthogonalize(const v1t_matrix* units, int n, int dtype, int steps, const float* coefficients, float eps, void* workspace, long long ws_bytes, void* stream);
+/* The momentum step over n fp32 matrices, row-major without gaps: g' = g + l1 sign(p); m <- momentum m + g'; U = nesterov ? g' + momentum m : m;
+ * p <- decay p - lr O(U), O as above (lr holds the factor for the matrix's shape, decay = 1 - learning rate * weight decay). zero_grad: g is cleared. No two of
+ * the call's tensors overlap. */
+typedef struct v1t_muon_range {
+    float *p, *g, *m;
+    int rows, cols;
+    float lr, decay, l1;
+    int pad_;
+} v1t_muon_range;
+int v1t_muon_step(const v1t_muon_range* units, int n, float momentum, int nesterov, int steps, const float* coefficients, float eps, int zero_grad, void* workspace,
+                  long long ws_bytes, void* stream);
+
 /* LayerNorm (vit.py:220,145) forward: z bf16 (rows, DP) = LN(x (+ inject[b])) ; backward: see
  * csrc/elementwise.h LnBwdArgs (gout = gin + dLN; optional token-sum, next-branch cast + bias colsum) */
 int v1t_layernorm_forward(const float* x, const float* inject, float* xout, const float* gamma,

@@ -56,6 +56,16 @@ class RotaryOperand(C.Structure):
     _fields_ = [("x", c_void_p), ("y", c_void_p), ("xb", c_ll), ("xt", c_ll), ("xh", c_ll), ("yb", c_ll), ("yt", c_ll), ("yh", c_ll), ("heads", c_int), ("pad_", c_int)]
 
 
+class Matrix(C.Structure):
+    """`v1t_matrix`: one update of `v1t_orthogonalize`."""
+    _fields_ = [("in_", c_void_p), ("out", c_void_p), ("row_stride", c_ll), ("col_stride", c_ll), ("rows", c_int), ("cols", c_int)]
+
+
+class MuonRange(C.Structure):
+    """`v1t_muon_range`: one matrix of `v1t_muon_step`."""
+    _fields_ = [("p", c_void_p), ("g", c_void_p), ("m", c_void_p), ("rows", c_int), ("cols", c_int), ("lr", c_float), ("decay", c_float), ("l1", c_float), ("pad_", c_int)]
+
+
 # name -> (restype, argtypes); every symbol declared in include/v1t_amd.h
 SIGNATURES: t.Dict[str, t.Tuple[t.Any, t.List[t.Any]]] = {
     "v1t_abi_version": (c_int, []),
@@ -137,6 +147,9 @@ SIGNATURES: t.Dict[str, t.Tuple[t.Any, t.List[t.Any]]] = {
     "v1t_rollout_matmul": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "v1t_rotary": (c_int, [C.POINTER(RotaryOperand), c_int, c_int, c_int, c_int, c_int, C.POINTER(c_int), c_int, C.c_double, c_int, c_int, c_int, c_void_p, c_int,
                            c_ll, c_ll, c_ll, c_void_p]),
+    "v1t_orthogonalize_ws_bytes": (c_ll, [C.POINTER(c_int), C.POINTER(c_int), c_int]),
+    "v1t_orthogonalize": (c_int, [C.POINTER(Matrix), c_int, c_int, c_int, C.POINTER(c_float), c_float, c_void_p, c_ll, c_void_p]),
+    "v1t_muon_step": (c_int, [C.POINTER(MuonRange), c_int, c_float, c_int, c_int, C.POINTER(c_float), c_float, c_int, c_void_p, c_ll, c_void_p]),
     "v1t_profile_enable": (c_int, [c_int, c_int]),
     "v1t_profile_read": (c_int, [C.POINTER(c_int), C.POINTER(C.c_double)]),
     "v1t_layernorm_forward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_void_p]),

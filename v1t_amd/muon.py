@@ -1,0 +1,143 @@
+"""Orthogonalised updates: `orthogonalize`, the momentum step `muon_step` around it, and `FusedMuon`, the optimizer of a model whose matrices
+take that step and whose other parameters keep `FusedAdamW`'s (the reference steps all of them with AdamW, train.py:216-223).
+
+A matrix's update is replaced by (nearly) the closest matrix with all singular values one: every direction that the gradient points to moves equally
+far, whatever its scale. The products are Newton-Schulz steps, all matrices of a model in one launch each (csrc/orthogonal.hip)."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+import typing as t
+
+import torch
+
+from . import lib as L
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # drive singular values to about 1 (0.7 to 1.2) within five steps from 0.003 on
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+MAX_STEPS = 32
+
+
+def _coefficients(coefficients, steps: int) -> t.Any:
+    if not 0 <= int(steps) <= MAX_STEPS:
+        raise ValueError(f"orthogonalize: 0 to {MAX_STEPS} steps, got {steps}")
+    c = list(coefficients)
+    if len(c) == 3 and all(isinstance(x, (int, float)) for x in c):
+        c = [c] * steps
+    if len(c) != steps or any(len(x) != 3 for x in c):
+        raise ValueError(f"orthogonalize: coefficients are (a, b, c) or one such triple for each of the {steps} steps")
+    return (C.c_float * max(1, 3 * steps))(*[float(v) for x in c for v in x])
+
+
+def _workspace(shapes: t.Sequence[t.Tuple[int, int]], device) -> torch.Tensor:
+    n = len(shapes)
+    nbytes = int(L.load().v1t_orthogonalize_ws_bytes((C.c_int * n)(*[r for r, _ in shapes]), (C.c_int * n)(*[c for _, c in shapes]), n))
+    L.check(min(nbytes, 0), "orthogonalize")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _refused(code: int, what: str) -> None:
+    if code == -1:
+        raise ValueError(f"{what}: coefficients under which the iteration's numbers grow to 128 or more (or are not finite), or a negative eps")
+    L.check(code, what)
+
+
+def orthogonalize(updates, *, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7):
+    """Each update's Newton-Schulz iterate: X = U / (|U|_F + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T (of the shorter side).
+
+    updates: a matrix, a stack (count, rows, cols), or a list of matrices of any shapes; bf16 / fp16 / fp32, any strides, one device. Returns new contiguous
+    tensors, laid out alike. coefficients: (a, b, c) or one triple per step. Arithmetic is fp32 whatever the type; the result is rounded once. A matrix of
+    zeros stays zero; NaN or infinity spoils its own matrix only. Not differentiable."""
+    one = isinstance(updates, torch.Tensor)
+    if one and updates.dim() not in (2, 3):
+        raise ValueError(f"orthogonalize: a matrix, a stack of matrices or a list of matrices, got shape {tuple(updates.shape)}")
+    us = ([updates] if updates.dim() == 2 else list(updates)) if one else list(updates)
+    co = _coefficients(coefficients, steps)
+    if not 0.0 <= float(eps) < math.inf:
+        raise ValueError(f"orthogonalize: eps must be non-negative and finite, got {eps}")
+    for u in us:
+        if not isinstance(u, torch.Tensor) or u.dim() != 2:
+            raise ValueError("orthogonalize: every update is a matrix")
+        if u.dtype not in _DTYPES or u.dtype != us[0].dtype:
+            raise TypeError(f"orthogonalize: updates share one of {list(_DTYPES)}, got {sorted({str(x.dtype) for x in us})}")
+        if u.device != us[0].device:
+            raise ValueError("orthogonalize: updates on several devices")
+        if torch.is_grad_enabled() and u.requires_grad:
+            raise RuntimeError("orthogonalize: not differentiable; call it under torch.no_grad() or on detached tensors")
+    if not us:
+        return updates.clone() if one else []
+    L.require_cuda(us[0], "orthogonalize")
+    if one and updates.dim() == 3:
+        out = torch.empty(updates.shape, dtype=updates.dtype, device=updates.device)
+        outs: t.List[torch.Tensor] = list(out)
+    else:
+        outs = [torch.empty(u.shape, dtype=u.dtype, device=u.device) for u in us]
+        out = outs[0] if one else outs
+    _orthogonalize([(u, o) for u, o in zip(us, outs) if u.numel()], int(steps), co, float(eps))
+    return out
+
+
+def _orthogonalize(pairs, steps: int, co, eps: float) -> None:
+    if not pairs:
+        return
+    u0 = pairs[0][0]
+    if u0.device.index != torch.cuda.current_device():
+        with torch.cuda.device(u0.device):
+            return _orthogonalize(pairs, steps, co, eps)
+    units = (L.Matrix * len(pairs))()
+    for m, (u, o) in zip(units, pairs):
+        m.in_, m.out = u.data_ptr(), o.data_ptr()
+        m.row_stride, m.col_stride = u.stride()
+        m.rows, m.cols = u.shape
+    ws = _workspace([tuple(u.shape) for u, _ in pairs], u0.device)
+    _refused(L.load().v1t_orthogonalize(units, len(pairs), _DTYPES[u0.dtype], steps, co, eps, ws.data_ptr(), ws.numel(), L.stream()), "orthogonalize")
+
+
+def muon_step(params: t.Sequence[torch.Tensor], grads: t.Sequence[torch.Tensor], moments: t.Sequence[torch.Tensor], *, lr, momentum: float = 0.95,
+              nesterov: bool = True, weight_decay: float = 0.0, l1: float = 0.0, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7,
+              zero_grad: bool = False) -> None:
+    """One step over matrices, in place: g' = g + l1 sign(p); m <- momentum m + g'; U = g' + momentum m (or m, without Nesterov's look ahead);
+    p <- (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) orthogonalize(U).
+
+    fp32 tensors without gaps of the same shape per matrix; a parameter of more dimensions (a convolution's) is a matrix of its first dimension
+    by all others. lr: a number, or one per matrix. zero_grad: the gradients are cleared. No two tensors of the call may share memory."""
+    params, grads, moments = list(params), list(grads), list(moments)
+    if not len(params) == len(grads) == len(moments):
+        raise ValueError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(moments)} momenta")
+    lrs = list(lr) if isinstance(lr, (list, tuple)) else [lr] * len(params)
+    if len(lrs) != len(params):
+        raise ValueError(f"muon_step: {len(lrs)} learning rates for {len(params)} parameters")
+    co = _coefficients(coefficients, steps)
+    if not 0.0 <= float(eps) < math.inf or not all(math.isfinite(float(x)) for x in (momentum, weight_decay, l1, *lrs)):
+        raise ValueError("muon_step: eps is non-negative, every coefficient is finite")
+    for p, g, m in zip(params, grads, moments):
+        if p.dim() < 2:
+            raise ValueError(f"muon_step: a parameter of shape {tuple(p.shape)} is no matrix")
+        for x in (p, g, m):
+            if x.dtype != torch.float32:
+                raise TypeError(f"muon_step: fp32 tensors are needed, got {x.dtype}")
+            if x.shape != p.shape or not x.is_contiguous() or x.device != params[0].device:
+                raise ValueError(f"muon_step: parameter, gradient and momentum are contiguous tensors of one shape on one device, got {[tuple(y.shape) for y in (p, g, m)]}")
+    spans = sorted((x.data_ptr(), x.data_ptr() + 4 * x.numel()) for x in params + grads + moments if x.numel())
+    if any(b < e for (_, e), (b, _) in zip(spans, spans[1:])):
+        raise ValueError("muon_step: tensors of the call share memory")
+    triples = [x for x in zip(params, grads, moments, lrs) if x[0].numel()]
+    if not triples:
+        return
+    L.require_cuda(params[0], "muon_step")
+    rs = []
+    for p, g, m, a in triples:
+        rows, cols = p.shape[0], p.numel() // p.shape[0]
+        rs.append(L.MuonRange(p.data_ptr(), g.data_ptr(), m.data_ptr(), rows, cols, float(a) * math.sqrt(max(1.0, rows / cols)), 1.0 - float(a) * weight_decay, l1, 0))
+    with torch.cuda.device(params[0].device):
+        muon_ranges(rs, momentum, nesterov, int(steps), co, float(eps), zero_grad, params[0].device)
+    for x in params + moments + (grads if zero_grad else []):
+        if not x.is_inference():
+            torch.autograd.graph.increment_version(x)
+
+
+def muon_ranges(rs: t.Sequence[L.MuonRange], momentum: float, nesterov: bool, steps: int, co, eps: float, zero_grad: bool, device) -> None:
+    """`v1t_muon_step` over a table of matrices, on the current stream."""
+    ws = _workspace([(r.rows, r.cols) for r in rs], device)
+    _refused(L.load().v1t_muon_step((L.MuonRange * len(rs))(*rs), len(rs), momentum, int(bool(nesterov)), steps, co, eps, int(bool(zero_grad)), ws.data_ptr(),
+                                    ws.numel(), L.stream()), "muon_step")
