@@ -58,6 +58,10 @@ typedef struct v1t_vit v1t_vit;       /* opaque plan: dims, arena/shadow/workspa
 
 int v1t_vit_create(const v1t_vit_config* cfg, v1t_vit** out);
 void v1t_vit_destroy(v1t_vit* h);
+/* Rotary positions in every block of this plan (no reference counterpart): q and k behind the projection - and their gradients - are turned as by v1t_rotary
+ * (pairs, a ladder of rates per axis) by `positions`, (tokens, n_axes) int32 on the device of the plan's launches, which the caller keeps alive as long as
+ * the plan uses them. positions = NULL: none (the state after v1t_vit_create). Set before the forward whose backward is to use them. */
+int v1t_vit_set_rotary(v1t_vit* h, const int* positions, const int* sections, int n_axes, double base);
 
 /* Parameter arena: ONE flat fp32 buffer; tensors keep the reference's natural shapes and state-dict
  * names so checkpoints stay compatible. Entries [0, param_count) are

@@ -67,6 +67,8 @@ class Config:
     num_neurons: t.Dict[str, int] = field(default_factory=lambda: {"A": 256})
     core: str = "vit"      # "vit" (core/vit.py) or "cct" (core/cct.py: conv tokenizer, no class token, head dim emb_dim / heads^2)
     pos_emb: str = "sine"  # cct only (train.py:603-605): "sine" | "none"
+    rotary: bool = False   # beyond the reference: q and k turned by the patch's row and column (`turn`)
+    rotary_base: float = 100.0
 
     @property
     def grid_hw(self) -> t.Tuple[int, int]:
@@ -205,6 +207,21 @@ def behavior_mlp(cfg: Config, sd: SD, k: int, v: Tensor, mouse_id: str, pfx: str
     return torch.tanh(linear(h, sd[p + "3.weight"], sd.get(p + "3.bias")))
 
 
+def turn(cfg: Config, x: Tensor) -> Tensor:
+    """Rotary positions of q or k, (batch, heads, tokens, head dim): the first half of the turned pairs (2j, 2j + 1) by the patch's row, the second by its
+    column, pair i of an axis with s = head dim // 4 pairs by position * base^(-i / s); a class token is at (0, 0)."""
+    gh, gw = cfg.grid_hw
+    lead, s = x.shape[2] - gh * gw, x.shape[3] // 4
+    rate = cfg.rotary_base ** -(torch.arange(s, dtype=torch.float64) / s)
+    row = torch.cat([torch.zeros(lead, dtype=torch.float64), torch.arange(gh, dtype=torch.float64).repeat_interleave(gw)])
+    col = torch.cat([torch.zeros(lead, dtype=torch.float64), torch.arange(gw, dtype=torch.float64).repeat(gh)])
+    angle = torch.cat([row[:, None] * rate, col[:, None] * rate], dim=1)
+    cos, sin = angle.cos().to(x.dtype), angle.sin().to(x.dtype)
+    even, odd = x[..., 0:4 * s:2], x[..., 1:4 * s:2]
+    pairs = torch.stack([even * cos - odd * sin, even * sin + odd * cos], dim=-1).flatten(-2)
+    return torch.cat([pairs, x[..., 4 * s:]], dim=-1)
+
+
 def attention(
     cfg: Config,
     sd: SD,
@@ -226,6 +243,8 @@ def attention(
     q = q.reshape(b, n, h, d).permute(0, 2, 1, 3)
     kk = kk.reshape(b, n, h, d).permute(0, 2, 1, 3)
     v = v.reshape(b, n, h, d).permute(0, 2, 1, 3)
+    if cfg.rotary:
+        q, kk = turn(cfg, q), turn(cfg, kk)
     scale = sd[p + "scale"]
     dots = q @ kk.transpose(-1, -2)
     if cfg.use_lsa:
@@ -334,6 +353,8 @@ def cct_attention(cfg: Config, sd: SD, k: int, x: Tensor, masks: t.Optional[t.Di
     q = q.reshape(b, n, h, d).permute(0, 2, 1, 3) * sd[p + "scale"]
     kk = kk.reshape(b, n, h, d).permute(0, 2, 1, 3)
     v = v.reshape(b, n, h, d).permute(0, 2, 1, 3)
+    if cfg.rotary:
+        q, kk = turn(cfg, q), turn(cfg, kk)
     attn = softmax_lastdim(q @ kk.transpose(-1, -2))
     attn = apply_mask(attn, masks.get(f"attn{k}"), masks.get("attn_p", cfg.t_dropout))
     o = (attn @ v).permute(0, 2, 1, 3).reshape(b, n, h * d)

@@ -99,3 +99,51 @@ def test_coefficients_that_grow_are_refused_by_name():
     units = (L.Matrix * 1)(L.Matrix(4096, 4096, 6, 1, 4, 6))
     for ok in ((3.4445, -4.775, 2.0315), (1.5, -0.5, 0.0), (1.0, 0.0, 0.0)):
         assert lib.v1t_orthogonalize(units, 1, 2, 5, (C.c_float * 15)(*(ok * 5)), 1e-7, None, 0, None) == -4  # past the check: no workspace
+
+
+def small(**over):
+    from v1t_amd.synthetic import sensorium_config
+
+    args, ds = sensorium_config({"A": 10}, **{**dict(input_shape=(1, 36, 64), resize_image=0, num_blocks=1, emb_dim=64, mlp_dim=128), **over})
+    return v1t_amd.Model(args, ds), args, ds
+
+
+def test_fused_muon_refusals():
+    from v1t_amd.trainer import Trainer
+
+    model, args, ds = small()
+    with pytest.raises(ValueError, match="positive"):
+        v1t_amd.FusedMuon.for_model(model, lr=1e-3, core_lr=0.0)
+    with pytest.raises(ValueError, match="finite"):
+        v1t_amd.FusedMuon.for_model(model, lr=1e-3, muon_lr=math.nan)
+    with pytest.raises(ValueError, match="steps"):
+        v1t_amd.FusedMuon.for_model(model, lr=1e-3, steps=99)
+    args.optimizer = "lamb"
+    with pytest.raises(NotImplementedError, match="lamb"):
+        Trainer(args, model, ds)
+    muon = v1t_amd.FusedMuon.for_model(model, lr=1e-3)
+    adam = v1t_amd.FusedAdamW.for_model(model, lr=1e-3)
+    for a, b in ((muon, adam), (adam, muon)):
+        with pytest.raises(ValueError, match="other optimizer"):
+            a.load_state_dict(b.state_dict())
+    # every attention and MLP matrix of the core, q, k and v apart; no table, no BehaviorMLP
+    assert [(r, c) for _, r, c in muon.matrices()] == [(256, 64)] * 3 + [(64, 256), (128, 64), (64, 128)]
+
+
+def test_rotary_core_refusals():
+    with pytest.raises(ValueError, match="head dim 3"):
+        small(rotary=True, emb_dim=3, num_heads=1)
+    with pytest.raises(NotImplementedError, match="use_lsa"):
+        small(rotary=True, use_lsa=True)
+    with pytest.raises(ValueError, match="rotary_base"):
+        small(rotary=True, rotary_base=-1.0)
+    model, _, _ = small(rotary=True)
+    at = model.core.rotary_positions()
+    assert at.shape == (1654, 2) and at[0].tolist() == [0, 0] and at[1].tolist() == [0, 0] and at[58].tolist() == [1, 0] and at[-1].tolist() == [28, 56]
+    lib = L.load()
+    sections = ints(16, 16)
+    for positions, sec, axes, base in ((4096, None, 2, 100.0), (4096, sections, 0, 100.0), (4096, sections, 5, 100.0), (4096, sections, 2, 0.0), (4096, sections, 2, math.nan),
+                                       (4096, ints(17, 16), 2, 100.0), (4096, ints(-1, 3), 2, 100.0), (4096, ints(0, 0), 2, 100.0)):
+        assert lib.v1t_vit_set_rotary(model.core._plan, positions, sec, axes, base) == -1
+    assert lib.v1t_vit_set_rotary(None, 4096, sections, 2, 100.0) == -1
+    assert lib.v1t_vit_set_rotary(model.core._plan, None, None, 0, 0.0) == 0

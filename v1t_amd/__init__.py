@@ -6,10 +6,10 @@ from .readout import Gaussian2DReadout, Readout, Readouts, register as register_
 from .model import ELU1, CoreShifter, CoreShifters, ImageCropper, Model  # noqa: F401
 from .muon import muon_step, orthogonalize  # noqa: F401
 from .positions import rotary, rotary_  # noqa: F401
-from .trainer import FusedAdamW  # noqa: F401  (opt-in optimizer for the reference's own loop: FusedAdamW.for_model)
+from .trainer import FusedAdamW, FusedMuon  # noqa: F401  (opt-in optimizers for the reference's own loop: FusedAdamW.for_model)
 
 __all__ = ["Core", "ViTCore", "CCTCore", "get_core", "register_core", "Gaussian2DReadout", "Readout", "Readouts", "register_readout",
-           "ELU1", "CoreShifter", "CoreShifters", "ImageCropper", "Model", "FusedAdamW", "muon_step", "orthogonalize", "rotary", "rotary_", "install_into_reference"]
+           "ELU1", "CoreShifter", "CoreShifters", "ImageCropper", "Model", "FusedAdamW", "FusedMuon", "muon_step", "orthogonalize", "rotary", "rotary_", "install_into_reference"]
 
 
 def install_into_reference() -> bool:

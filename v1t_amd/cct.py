@@ -112,6 +112,11 @@ class CCTCore(ViTCore):
             tr.blocks.append(block)
         self.transformer = tr
 
+    def _patch_grid(self, args):
+        """tokens behind the convolution and the max pool (cct.py:46-56)"""
+        _, h, w = self.input_shape
+        return tuple(((n + 2 * self.CONV_PADDING - args.patch_size) // args.patch_stride + 1 + 2 - 3) // 2 + 1 for n in (h, w))
+
     @staticmethod
     def find_shape(num_patches: int):
         """reference cct.py:293-299"""

@@ -23,6 +23,7 @@ from torch import nn
 
 from . import lib as L
 from .flat import FlatArena, Slot
+from .positions import MAX_PAIRS
 
 _CORES: t.Dict[str, t.Any] = dict()
 
@@ -291,7 +292,11 @@ class ViTCore(Core):
     patch_size, patch_stride, emb_dim, p_dropout, num_blocks, num_heads, mlp_dim, t_dropout, use_lsa,
     drop_path, disable_bias, output_shapes (mouse ids for behavior_mode 4). `grad_checkpointing` is
     accepted and ignored: the fused attention never materialises (B,H,T,T), so there is nothing to
-    recompute (vit.py:277-284)."""
+    recompute (vit.py:277-284).
+
+    Beyond the reference: `args.rotary` (default False) turns q and k of every block by their patch's row and column (`positions.rotary`; a class
+    token stays as it is), beside whatever table the tokens carry, at the rates `args.rotary_base`^(-i / s) of the s = head dim // 4 pairs per axis
+    (default base 100: the slowest pair turns by half a radian over a grid of 29 x 57)."""
 
     def __init__(self, args, input_shape: t.Tuple[int, int, int], name: str = "ViTCore"):
         super().__init__(args, input_shape=input_shape, name=name)
@@ -341,6 +346,7 @@ class ViTCore(Core):
         self._block_events = None  # set by the data-parallel trainer (dist.MouseSharding.reduce_core_overlapped)
         self._path_scale_override = None  # tests: (num_blocks, 2, B) factors to replay instead of drawing them
         self.num_blocks = int(args.num_blocks)
+        self._init_rotary(args, c)
         self.attach_recorder_taps()  # no-op unless v1t_amd.install_into_reference() has named the reference's Attention class
         if not hasattr(self, "drop_path_rates"):  # ViT: one DropPath module for every block (vit.py:333)
             self.drop_path_rates = torch.full((self.num_blocks,), self.drop_path_rate, dtype=torch.float32)
@@ -352,6 +358,38 @@ class ViTCore(Core):
 
             warnings.warn(f"v1t_amd: attention-probability dropout runs at {self.attention_dropout_rate:.5f} (t_dropout = {float(args.t_dropout):.5f} "
                           f"quantised to 1/65536); the proj / MLP dropouts use the exact rate", stacklevel=2)
+
+    # ------------------------------------------------------------------ rotary positions (args.rotary)
+    def _patch_grid(self, args) -> t.Tuple[int, int]:
+        _, h, w = self.input_shape
+        return (h - args.patch_size) // args.patch_stride + 1, (w - args.patch_size) // args.patch_stride + 1
+
+    def _init_rotary(self, args, c: int) -> None:
+        self.rotary = bool(getattr(args, "rotary", False))
+        self._rotary_at: t.Optional[torch.Tensor] = None
+        if not self.rotary:
+            return
+        if self._cfg.use_lsa:
+            # the gradient of LSA's per-head scale, sum(dS o S), cancels to a hundredth of its terms: the second bf16 rounding of q and k takes it from
+            # 1.2e-2 of its size to 1.3e-2, past what the core's gradients are held to
+            raise NotImplementedError("rotary positions with use_lsa are not supported: the second rounding of q and k spoils the gradient of LSA's scale")
+        head = args.emb_dim if self.cls_tokens else args.emb_dim // args.num_heads // args.num_heads  # vit.py:218; cct.py:110-127
+        if head < 4:
+            raise ValueError(f"rotary positions turn at least one pair of features per axis: head dim {head} < 4")
+        self.rotary_sections = (head // 4, head // 4)
+        self.rotary_base = float(getattr(args, "rotary_base", 100.0))
+        if not 0.0 < self.rotary_base < math.inf:
+            raise ValueError(f"rotary_base must be positive and finite, got {self.rotary_base}")
+        if sum(self.rotary_sections) > MAX_PAIRS:
+            raise ValueError(f"rotary positions of head dim {head}: at most {2 * MAX_PAIRS + 3} are supported")
+        self._rotary_grid = self._patch_grid(args)
+        assert self._rotary_grid[0] * self._rotary_grid[1] == self.num_tokens - self.cls_tokens
+
+    def rotary_positions(self, device=None) -> torch.Tensor:
+        """(tokens, 2) int32: every patch's row and column; (0, 0) for the class token."""
+        gh, gw = self._rotary_grid
+        at = torch.stack(torch.meshgrid(torch.arange(gh), torch.arange(gw), indexing="ij"), -1).reshape(-1, 2)
+        return torch.cat([at.new_zeros(self.cls_tokens, 2), at]).to(device=device, dtype=torch.int32)
 
     def __del__(self):
         try:
@@ -455,6 +493,9 @@ class ViTCore(Core):
         a.ensure()
         if self._anchor.device != a.data.device:
             self._anchor = torch.zeros((), device=a.data.device, requires_grad=True)
+        if self.rotary and (self._rotary_at is None or self._rotary_at.device != a.data.device):
+            self._rotary_at = self.rotary_positions(a.data.device)
+            L.check(L.load().v1t_vit_set_rotary(self._plan, self._rotary_at.data_ptr(), (C.c_int * 2)(*self.rotary_sections), 2, self.rotary_base), "vit_set_rotary")
         key = (a.generation, a.version())
         if self._shadow is None or self._shadow.device != a.data.device:
             self._shadow = torch.empty(L.load().v1t_vit_shadow_bytes(self._plan), dtype=torch.uint8, device=a.data.device)

@@ -71,6 +71,22 @@ struct v1t_vit {
     // the dX GEMMs of the same gradients (created by the first such backward)
     mutable hipStream_t dw_stream = nullptr;
     mutable hipEvent_t dw_ready[4] = {}, dw_done[4] = {};
+    // rotary positions of q and k (v1t_vit_set_rotary): the caller's (T, rot_axes) int32 table, nullptr = none
+    const int* rot_at = nullptr;
+    int rot_axes = 0, rot_sections[4] = {};
+    double rot_base = 0.0;
+    // q and k - 2 H neighbouring heads of a row of the packed projection - turned in place (forward), their gradients turned back (inverse). A pass of its own
+    // over two thirds of the buffer: the values are rounded to bf16 a second time, half a step as in the projection's epilogue
+    int rotate(bf16_t* qkv, int B, int inverse, hipStream_t s) const {
+        if (!rot_at) return V1T_OK;
+        v1t_rotary_operand o{};
+        o.x = o.y = qkv;
+        o.x_stride_b = o.y_stride_b = (long long)T * 3 * HDP;
+        o.x_stride_t = o.y_stride_t = 3 * HDP;
+        o.x_stride_h = o.y_stride_h = HEP;
+        o.heads = 2 * H;
+        return v1t_rotary(&o, 1, 0, B, T, HE, rot_sections, rot_axes, rot_base, 0, 0, inverse, rot_at, 0, 0, rot_axes, 1, s);
+    }
 
     long long add(const std::string& name, std::initializer_list<long long> shape, bool is_param, long long& cursor) {
         TensorInfo t;
@@ -562,6 +578,26 @@ int v1t_vit_create(const v1t_vit_config* cfg, v1t_vit** out) {
     return V1T_OK;
 }
 
+int v1t_vit_set_rotary(v1t_vit* h, const int* positions, const int* sections, int n_axes, double base) {
+    if (!h) return V1T_ERR_ARG;
+    if (!positions) {
+        h->rot_at = nullptr;
+        return V1T_OK;
+    }
+    if (!sections || n_axes < 1 || n_axes > 4 || !(base > 0.0) || !std::isfinite(base)) return V1T_ERR_ARG;
+    long long pairs = 0;
+    for (int a = 0; a < n_axes; ++a) {
+        if (sections[a] < 0) return V1T_ERR_ARG;
+        pairs += sections[a];
+    }
+    if (pairs < 1 || 2 * pairs > h->HE) return V1T_ERR_ARG;
+    if (pairs > 256) return V1T_ERR_UNSUPPORTED;
+    h->rot_at = positions;
+    h->rot_axes = n_axes;
+    for (int a = 0; a < 4; ++a) h->rot_sections[a] = a < n_axes ? sections[a] : 0;
+    h->rot_base = base;
+    return V1T_OK;
+}
 void v1t_vit_destroy(v1t_vit* h) {
     if (!h) return;
     if (h->d_pack) (void)hipFree(h->d_pack);
@@ -754,6 +790,7 @@ int v1t_vit_forward(const v1t_vit* h, const float* arena, const void* shadow, co
         if (g_nosplit & 1) g.A_lo = g.B_lo = nullptr;
         fwd_operands(g);
         CHECK(ln_then_gemm(l1, g, EPI_BF16, s));
+        CHECK(h->rotate(qkv, B, 0, s));
 
         AttnArgs at{};
         at.qkv = qkv; at.ldqkv = 3 * HDP; at.o = x16o ? nullptr : o; at.ldo = HDP; at.o_lo = (bf16_t*)(wb + w.o_lo); at.lo_f16 = g_fwd_f16; at.lse2 = (float*)(wb + w.lse2);
@@ -1034,6 +1071,7 @@ int v1t_vit_backward_input(const v1t_vit* h, const float* arena, const void* sha
         if (!rowdot) CHECK(launch_attn_delta(at, h->HEP, delta, s));
         else if (k == h->NB - 1) CHECK(launch_attn_rc_pad(at, s));  // the pad rows are constants and only this call writes them: once per backward
         CHECK(launch_attn_bwd(at, h->HEP, s));
+        CHECK(h->rotate(dqkv, B, 1, s));
         // dWqkv += dqkv^T z1
         t = GemmTNArgs{};
         t.Y = dqkv; t.ldy = 3 * HDP; t.X = z1; t.ldx = DP; t.M = R; t.NY = 3 * HDP; t.NX = DP; t.dW = grads + b.qkv; t.ldw = D;

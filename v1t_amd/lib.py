@@ -80,6 +80,7 @@ SIGNATURES: t.Dict[str, t.Tuple[t.Any, t.List[t.Any]]] = {
     "v1t_error_string": (C.c_char_p, [c_int]),
     "v1t_vit_create": (c_int, [C.POINTER(VitConfig), C.POINTER(c_void_p)]),
     "v1t_vit_destroy": (None, [c_void_p]),
+    "v1t_vit_set_rotary": (c_int, [c_void_p, c_void_p, C.POINTER(c_int), c_int, C.c_double]),
     "v1t_vit_arena_floats": (c_ll, [c_void_p]),
     "v1t_vit_param_floats": (c_ll, [c_void_p]),
     "v1t_vit_num_tensors": (c_int, [c_void_p]),

@@ -23,6 +23,7 @@ import warnings
 import torch
 
 from . import lib as L
+from . import muon
 from .dist import MouseSharding
 from .losses import elu1_poisson_loss
 from .model import Model, mouse_arena, mouse_step_ranges
@@ -149,6 +150,8 @@ class FusedAdamW:
         saved_groups = sd["param_groups"]
         if len(saved_groups) != len(self.param_groups):
             raise ValueError("loaded state dict has a different number of parameter groups")
+        if any(bool(g.get("muon")) for g in saved_groups) != any(bool(g.get("muon")) for g in self.param_groups):
+            raise ValueError("loaded state dict is of the other optimizer: FusedMuon keeps a momentum where FusedAdamW keeps a gradient's mean and mean square")
         if all("name" in g for g in saved_groups):
             by_name = {g["name"]: g for g in saved_groups}
             if len(by_name) != len(saved_groups) or set(by_name) != {g["name"] for g in self.param_groups}:
@@ -215,6 +218,94 @@ class FusedAdamW:
         if rs:
             arr = (L.AdamRange * len(rs))(*rs)
             L.check(L.load().v1t_adamw_multi(arr, len(rs), self.betas[0], self.betas[1], self.eps, self.weight_decay, int(zero_grad), L.stream()), "adamw_multi")
+
+
+class FusedMuon(FusedAdamW):
+    """`FusedAdamW` whose core matrices - the attention projections and the MLP matrices of every block - take the orthogonalised momentum step
+    instead (`muon.muon_step`, one `v1t_muon_step` over the arena's slices; q, k and v of a fused projection are three matrices). Everything else of the
+    core (tables, patch embedding, norms, biases, BehaviorMLPs) and of the mice keeps AdamW.
+
+    `muon_lr` is the matrices' learning rate where the core's group has `core_lr`; a scheduler that scales the group's "lr" scales both. A matrix's momentum lives
+    in its slice of the arena's `exp_avg`, its slice of `exp_avg_sq` stays zero: checkpoints keep torch.optim's format, and the "muon" entry of the core's
+    group tells them from AdamW's (`load_state_dict` refuses the other kind). Ranks of a data-parallel step that hold the same gradients compute the same update."""
+
+    def __init__(self, lr: float, betas=(0.9, 0.9999), eps: float = 1e-8, weight_decay: float = 0.0, muon_lr: float = 0.02, momentum: float = 0.95,
+                 nesterov: bool = True, steps: int = 5):
+        super().__init__(lr, betas=betas, eps=eps, weight_decay=weight_decay)
+        if not all(math.isfinite(x) for x in (muon_lr, momentum)):
+            raise ValueError(f"FusedMuon: muon_lr {muon_lr} and momentum {momentum} must be finite")
+        self.muon_lr, self.momentum, self.nesterov, self.steps = float(muon_lr), float(momentum), bool(nesterov), int(steps)
+        self._coefficients = muon._coefficients(muon.COEFFICIENTS, self.steps)
+
+    @classmethod
+    def for_model(cls, model: Model, lr: float, core_lr: t.Optional[float] = None, betas=(0.9, 0.9999), eps: float = 1e-8, weight_decay: float = 0.0,
+                  **muon_options) -> "FusedMuon":
+        opt = cls(lr, betas=betas, eps=eps, weight_decay=weight_decay, **muon_options)
+        opt.bind(model, lr if core_lr is None else core_lr)
+        return opt
+
+    def bind(self, model: Model, core_lr: float) -> None:
+        if not core_lr > 0.0:
+            raise ValueError(f"FusedMuon: the matrices' learning rate follows the core's, which must be positive, got {core_lr}")
+        super().bind(model, core_lr)
+        self._per_core_lr = self.muon_lr / float(core_lr)
+        for g in self.param_groups:
+            if g["name"] == "core":
+                g["muon"] = {"lr": self.muon_lr, "momentum": self.momentum, "nesterov": self.nesterov, "steps": self.steps}
+        self._matrices: t.Optional[t.List[t.Tuple[int, int, int]]] = None
+
+    def matrices(self) -> t.List[t.Tuple[int, int, int]]:
+        """(offset, rows, cols) in the core's arena of every matrix that takes the momentum step, in order."""
+        if self._matrices is None:
+            core = self.model.core
+            names = {id(p): k for k, p in core.named_parameters()}
+            found = []
+            for s in core._arena.slots:
+                key = names.get(id(s.tensor), "")
+                if not s.is_param or s.tensor.dim() != 2 or ".blocks." not in key or not (".mha." in key or ".mlp." in key):
+                    continue
+                rows, cols = s.tensor.shape
+                parts = 3 if key.endswith("qkv.weight") else 1
+                found += [(s.offset + i * (rows // parts) * cols, rows // parts, cols) for i in range(parts)]
+            self._matrices = sorted(found)
+        return self._matrices
+
+    def step_arena(self, arena, ranges: t.Sequence[t.Tuple[int, int, float, float]], zero_grad: bool = True) -> None:
+        if arena is not self.model.core._arena:
+            return super().step_arena(arena, ranges, zero_grad)
+        arena.step += 1
+        m, v = arena.moments()
+        p_, g_, m_, v_ = (x.data_ptr() for x in (arena.data, arena.grad, m, v))
+        rest, mats = [], []
+        for start, n, l1, lr in ranges:
+            at, end = start, start + n
+            for off, rows, cols in self.matrices():
+                size = rows * cols
+                if off + size <= start or off >= end:
+                    continue
+                if off < start or off + size > end:
+                    raise RuntimeError("FusedMuon: a range of the core's arena ends inside a matrix")
+                if off > at:
+                    rest.append((at, off - at, l1, lr))
+                a = lr * self._per_core_lr
+                mats.append(L.MuonRange(p_ + 4 * off, g_ + 4 * off, m_ + 4 * off, rows, cols, a * math.sqrt(max(1.0, rows / cols)), 1.0 - a * self.weight_decay, l1, 0))
+                at = off + size
+            if end > at:
+                rest.append((at, end - at, l1, lr))
+        if rest:
+            rs = (L.AdamRange * len(rest))(*[L.AdamRange(p_ + 4 * o, g_ + 4 * o, m_ + 4 * o, v_ + 4 * o, n, lr, l1, arena.step, 0) for o, n, l1, lr in rest])
+            L.check(L.load().v1t_adamw_multi(rs, len(rest), self.betas[0], self.betas[1], self.eps, self.weight_decay, int(zero_grad), L.stream()), "adamw_multi")
+        if mats:
+            muon.muon_ranges(mats, self.momentum, self.nesterov, self.steps, self._coefficients, 1e-7, zero_grad, arena.data.device)
+
+    def step_arenas(self, items, zero_grad: bool = True) -> None:
+        core = self.model.core._arena
+        for item in items:
+            if item[0] is core:
+                self.step_arena(*item, zero_grad)
+        mice = [item for item in items if item[0] is not core]
+        if mice:
+            super().step_arenas(mice, zero_grad)
 
 
 class _NativeStep:
@@ -492,7 +583,12 @@ class Trainer:
         self.sharding = sharding or MouseSharding(self.mouse_ids, rank=0, world=1)
         self.lr = args.lr
         self.core_lr = args.lr if getattr(args, "core_lr", None) is None else args.core_lr
-        self.opt = FusedAdamW(args.lr, betas=(args.adam_beta1, args.adam_beta2), eps=args.adam_eps)
+        kind = getattr(args, "optimizer", "adamw")
+        if kind not in ("adamw", "muon"):
+            raise NotImplementedError(f"--optimizer {kind} not implemented.")
+        adam = dict(betas=(args.adam_beta1, args.adam_beta2), eps=args.adam_eps)
+        self.opt = FusedAdamW(args.lr, **adam) if kind == "adamw" else FusedMuon(args.lr, **adam, muon_lr=getattr(args, "muon_lr", 0.02),
+                                                                                  momentum=getattr(args, "muon_momentum", 0.95))
         self.opt.bind(model, self.core_lr)
         self.batch_size = args.batch_size
         self._core_l1: t.Optional[float] = None
