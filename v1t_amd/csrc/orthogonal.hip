@@ -161,38 +161,154 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(const NsUnit* units, int n
 }
 
 // ---- the products -------------------------------------------------------------------------
-// C[i][j] = sum_k P[i][k] Q[j][k]: a workgroup of 4 waves computes a B x B tile, wave (wi, wj) a quarter of it, in K steps of 32. The tile's rows of P and Q go
-// to LDS by LDS-DMA, double buffered. i is on the accumulators' lanes and j in their registers, four in a row: a lane stores 8 B of a plane's row.
+// C[i][j] = sum_k P[i][k] Q[j][k]: a workgroup of 4 waves computes a 64 TW x 64 TW tile, wave (wi, wj) a quarter of it, in K steps of 32. The tile's rows of P
+// and Q go to LDS by LDS-DMA into a ring of NST stages. In the accumulators i is on the lanes and j in the registers, four in a row.
 enum NsKind { NS_GRAM = 0, NS_POLY = 1, NS_APPLY = 2, NS_LAST = 3 };
 struct NsStep {
     float alpha, beta;   // C <- alpha (P Q^T) + beta D, on the scaled planes
     int from;            // which of the two X planes is read
     float inv;           // 2^-e
 };
+typedef f16_t f16x4 __attribute__((ext_vector_type(4)));
 
-template <int B, int KIND, typename T>
-__global__ __launch_bounds__(256, 2) void ns_gemm_kernel(const NsUnit* units, int n, char* ws, NsStep st) {
-    constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY, TR = !SYM;  // TR: Q is stored [k][j]
-    constexpr int TW = B / 64;                  // 32 x 32 blocks per wave and side
-    constexpr int PL = B * NS_BK;               // elements of an LDS plane
-    constexpr int PIECES = PL * 2 / 1024 / 4;   // LDS-DMA instructions per wave and plane
-    static_assert(PIECES >= 1, "tile");
-    __shared__ __attribute__((aligned(16))) f16_t lds[2][4][PL];
-    const NsUnit& u = ns_find(units, n, blockIdx.x, SYM ? &NsUnit::sym0 : &NsUnit::full0);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave >> 1, wj = wave & 1;
-    int bi, bj;
+template <int TW>
+struct NsTile {
+    static constexpr int B = 64 * TW, PL = B * NS_BK, SIDE = 32 * TW;
+    static constexpr int PIECES = PL * 2 / 1024 / 4;      // LDS-DMA instructions per wave and plane: one per 64 rows
+    static constexpr int NST = TW == 1 ? 4 : TW == 2 ? 2 : 3;
+    static constexpr int LDS = NST * 4 * PL;              // elements; the epilogue's fp32 tile fits
+    static_assert(4 * SIDE * SIDE * 4 <= LDS * 2, "epilogue");
+};
+
+// where a tile lies and what it reads and writes
+struct NsWhere {
+    int bi, bj, i0, j0;
+    const f16_t *D, *Dl;
+    f16_t *C, *Cl;
+    int ldd, cols;
+};
+template <int TW, int KIND>
+DEVFN NsWhere ns_where(const NsUnit& u, char* ws, const NsStep& st, int block) {
+    constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY;
+    constexpr int B = NsTile<TW>::B;
+    NsWhere w;
     if constexpr (SYM) {  // tile number -> (bi <= bj) of the upper triangle, columns of tiles one after another
-        const int t = blockIdx.x - u.sym0;
-        bj = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
-        while ((bj + 1) * (bj + 2) / 2 <= t) ++bj;
-        while (bj * (bj + 1) / 2 > t) --bj;
-        bi = t - bj * (bj + 1) / 2;
+        const int t = block - u.sym0;
+        w.bj = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+        while ((w.bj + 1) * (w.bj + 2) / 2 <= t) ++w.bj;
+        while (w.bj * (w.bj + 1) / 2 > t) --w.bj;
+        w.bi = t - w.bj * (w.bj + 1) / 2;
     } else {
-        const int t = blockIdx.x - u.full0, ni = (u.mp + B - 1) / B;
-        bi = t % ni;
-        bj = t / ni;
+        const int t = block - u.full0, ni = (u.mp + B - 1) / B;
+        w.bi = t % ni;
+        w.bj = t / ni;
     }
-    const int i0 = bi * B, j0 = bj * B;
+    w.i0 = w.bi * B;
+    w.j0 = w.bj * B;
+    const size_t xlo = (size_t)u.mp * u.np, alo = (size_t)u.mp * u.mp;
+    w.D = KIND == NS_POLY ? (const f16_t*)(ws + u.a) : (const f16_t*)(ws + u.x[st.from]);
+    w.Dl = w.D + (KIND == NS_POLY ? alo : xlo);
+    w.ldd = KIND == NS_POLY ? u.mp : u.np;
+    w.C = (f16_t*)(ws + (KIND == NS_GRAM ? u.a : KIND == NS_POLY ? u.s : u.x[st.from ^ 1]));
+    w.Cl = w.C + (SYM ? alo : xlo);
+    w.cols = SYM ? u.mp : u.np;
+    return w;
+}
+
+// Accumulators -> alpha acc + beta D -> planes (both triangles of a symmetric product), or the result. Each wave turns its part over in its own LDS, so that
+// planes are read and written 16 B a lane along their rows - also the mirrored tile's - and the result along its own rows, whichever way the matrix lies.
+// LDS image [SIDE][SIDE] fp32, 16-B chunks of a row swizzled by the row: writes by lanes of one column and reads along rows both spread over the banks.
+template <int TW, int KIND, typename T>
+DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x16 (&acc)[TW][TW], float* img, int wi, int wj, int lane) {
+    constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY;
+    constexpr int SIDE = 32 * TW;
+    auto chunk = [&](int i, int c) { return i * SIDE + 4 * (TW == 2 ? c ^ (i & 15) : c ^ (i >> 1 & 7)); };
+    const int r = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int ti = 0; ti < TW; ++ti)
+#pragma unroll
+        for (int tj = 0; tj < TW; ++tj)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x16& a = acc[ti][tj];
+                *(f32x4*)(img + chunk(32 * ti + r, 8 * tj + 2 * q + h)) =
+                    f32x4{st.alpha * a[4 * q], st.alpha * a[4 * q + 1], st.alpha * a[4 * q + 2], st.alpha * a[4 * q + 3]};
+            }
+    __builtin_amdgcn_wave_barrier();
+    const int iw = w.i0 + SIDE * wi, jw = w.j0 + SIDE * wj;
+    const bool mirror = SYM && w.bi != w.bj;  // the lower triangle
+    for (int k = lane; k < SIDE * SIDE / 8; k += 64) {
+        const int il = k / (SIDE / 8), jl = 8 * (k % (SIDE / 8)), i = iw + il, j = jw + jl;
+        if (i >= u.mp || j >= w.cols) continue;  // both are multiples of 32: groups of 8 are whole
+        f32x4 v0 = *(const f32x4*)(img + chunk(il, jl / 4)), v1 = *(const f32x4*)(img + chunk(il, jl / 4 + 1));
+        if constexpr (KIND != NS_GRAM) {
+            const f16x8 dh = *(const f16x8*)(w.D + (size_t)i * w.ldd + j), dl = *(const f16x8*)(w.Dl + (size_t)i * w.ldd + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v0[e] += st.beta * ((float)dh[e] + (float)dl[e]);
+                v1[e] += st.beta * ((float)dh[4 + e] + (float)dl[4 + e]);
+            }
+        }
+        if constexpr (KIND != NS_LAST) {
+            f16x8 ch, cl;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                f16_t a, b;
+                ns_split(e < 4 ? v0[e] : v1[e - 4], a, b);
+                ch[e] = a;
+                cl[e] = b;
+            }
+            *(f16x8*)(w.C + (size_t)i * w.cols + j) = ch;
+            *(f16x8*)(w.Cl + (size_t)i * w.cols + j) = cl;
+        }
+        if (KIND == NS_LAST || (KIND == NS_POLY && mirror)) {
+            *(f32x4*)(img + chunk(il, jl / 4)) = v0;
+            *(f32x4*)(img + chunk(il, jl / 4 + 1)) = v1;
+        }
+    }
+    __builtin_amdgcn_wave_barrier();
+    auto at = [&](int il, int jl) { return img[chunk(il, jl / 4) + (jl & 3)]; };
+    if constexpr (SYM) {
+        if (!mirror) return;
+        for (int k = lane; k < SIDE * SIDE / 8; k += 64) {
+            const int jl = k / (SIDE / 8), il = 8 * (k % (SIDE / 8)), i = iw + il, j = jw + jl;
+            if (i >= u.mp || j >= w.cols) continue;
+            f16x8 ch, cl;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                f16_t a, b;
+                ns_split(at(il + e, jl), a, b);
+                ch[e] = a;
+                cl[e] = b;
+            }
+            *(f16x8*)(w.C + (size_t)j * w.cols + i) = ch;
+            *(f16x8*)(w.Cl + (size_t)j * w.cols + i) = cl;
+        }
+    } else if constexpr (KIND == NS_LAST) {
+        auto put = [&](int row, int col, float o) {
+            if (row >= u.rows || col >= u.cols) return;
+            const long long x = (long long)row * u.cols + col;
+            if (u.out) ((T*)u.out)[x] = (T)o;
+            else u.w[x] = u.decay * u.w[x] - u.lr * o;
+        };
+        for (int k = lane; k < SIDE * SIDE; k += 64) {
+            const int a = k / SIDE, b = k % SIDE;  // b runs along the result's rows
+            if (u.trans) put(jw + a, iw + b, at(b, a) * st.inv);
+            else put(iw + a, jw + b, at(a, b) * st.inv);
+        }
+    }
+}
+
+template <int TW, int KIND, typename T>
+__global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(const NsUnit* units, int n, char* ws, NsStep st) {
+    constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY, TR = !SYM;  // TR: Q is stored [k][j]
+    using Tile = NsTile<TW>;
+    constexpr int B = Tile::B, PL = Tile::PL, PIECES = Tile::PIECES, NST = Tile::NST;
+    __shared__ __attribute__((aligned(16))) f16_t lds[Tile::LDS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave >> 1, wj = wave & 1;
+    const int block = xcd_remap(blockIdx.x, gridDim.x);
+    const NsUnit& u = ns_find(units, n, block, SYM ? &NsUnit::sym0 : &NsUnit::full0);
+    const NsWhere w = ns_where<TW, KIND>(u, ws, st, block);
     const int K = KIND == NS_GRAM ? u.np : u.mp, nk = K / NS_BK;
     const f16_t* X = (const f16_t*)(ws + u.x[st.from]);
     const f16_t* A = (const f16_t*)(ws + u.a);
@@ -204,28 +320,36 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(const NsUnit* units, in
 
     // A 1-KB piece fills 64 16-B chunks of a plane in order; which 16 B of the tile's row a chunk holds is swizzled, so that the fragment reads below spread over
     // all banks. Rows [.][32]: four chunks a row, chunk c at c ^ (row / 4 % 4). Q as [k][j], B / 8 chunks a row: c ^ 4 (k % 4) - B = 64, where two rows fill
-    // the 64 banks: c ^ 4 (k / 2 % 2).
-    size_t po[PIECES], qo[PIECES];
+    // the 64 banks: c ^ 4 (k / 2 % 2). A lane's byte offset from the tile's first row is loop-invariant; piece p of a wave goes by the instruction's offset, which
+    // moves the LDS and the global address alike: the lane offset carries 1024 p less, the base 2048 less.
+    unsigned po[PIECES], qo[PIECES];
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
         const int c = 64 * (wave * PIECES + p) + lane;
-        po[p] = (size_t)min(i0 + c / 4, u.mp - 1) * ldp + 8 * ((c & 3) ^ (c >> 4 & 3));
+        po[p] = (unsigned)min(c / 4, u.mp - 1 - w.i0) * (unsigned)(2 * ldp) + 16 * ((c & 3) ^ (c >> 4 & 3)) + 2048 - 1024 * p;
         if constexpr (TR) {
             const int k = c / (B / 8), cc = (c % (B / 8)) ^ (B == 64 ? (k >> 1 & 1) << 2 : (k & 3) << 2);
-            qo[p] = (size_t)k * ldq + min(j0 + 8 * cc, u.np - 8);
+            qo[p] = (unsigned)k * (unsigned)(2 * ldq) + 2 * min(8 * cc, u.np - 8 - w.j0) + 2048 - 1024 * p;
         } else {
-            qo[p] = (size_t)min(j0 + c / 4, u.mp - 1) * ldq + 8 * ((c & 3) ^ (c >> 4 & 3));
+            qo[p] = (unsigned)min(c / 4, u.mp - 1 - w.j0) * (unsigned)(2 * ldq) + 16 * ((c & 3) ^ (c >> 4 & 3)) + 2048 - 1024 * p;
         }
     }
+    const char* pb = (const char*)(P + (size_t)w.i0 * ldp) - 2048;
+    const char* qb = (const char*)(TR ? Q + w.j0 : Q + (size_t)w.j0 * ldq) - 2048;
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)lds);
+    auto uniform = [](const char* p) {
+        const unsigned long long b = (unsigned long long)(uintptr_t)p;
+        const unsigned hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(b >> 32)), lo = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)b);
+        return (const char*)(uintptr_t)(((unsigned long long)hi << 32) | lo);
+    };
     auto issue = [&](int t, int buf) {
-        const size_t pk = (size_t)t * NS_BK, qk = TR ? (size_t)t * NS_BK * ldq : (size_t)t * NS_BK;
+        const size_t pk = (size_t)t * (2 * NS_BK), qk = TR ? (size_t)t * (2 * NS_BK) * ldq : (size_t)t * (2 * NS_BK);
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p) {
-            const int at = 512 * (wave * PIECES + p);
-            lds_dma16(P + po[p] + pk, &lds[buf][0][at]);
-            lds_dma16(P + po[p] + pk + plo, &lds[buf][1][at]);
-            lds_dma16(Q + qo[p] + qk, &lds[buf][2][at]);
-            lds_dma16(Q + qo[p] + qk + qlo, &lds[buf][3][at]);
+        for (int plane = 0; plane < 4; ++plane) {
+            const char* base = uniform(plane == 0 ? pb + pk : plane == 1 ? pb + pk + 2 * plo : plane == 2 ? qb + qk : qb + qk + 2 * qlo);
+            const unsigned m0 = lds0 + 2u * (unsigned)((buf * 4 + plane) * PL) + 1024u * (unsigned)(wave * PIECES);
+            const unsigned* o = plane < 2 ? po : qo;
+            TileDma<32, 32>::template group<PIECES>(base, m0, o[0], o[PIECES > 1 ? 1 : 0], o[PIECES > 2 ? 2 : 0], 0);
         }
     };
 
@@ -250,98 +374,45 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(const NsUnit* units, in
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     auto compute = [&](int buf) {
+        const f16_t* img = lds + buf * 4 * PL;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             bf16x8 ph[TW], pl[TW], qh[TW], ql[TW];
 #pragma unroll
             for (int i = 0; i < TW; ++i) {
-                ph[i] = row_frag(lds[buf][0], 32 * (TW * wi + i), s);
-                pl[i] = row_frag(lds[buf][1], 32 * (TW * wi + i), s);
+                ph[i] = row_frag(img, 32 * (TW * wi + i), s);
+                pl[i] = row_frag(img + PL, 32 * (TW * wi + i), s);
                 if constexpr (TR) {
-                    qh[i] = col_frag(lds[buf][2], 32 * (TW * wj + i), s);
-                    ql[i] = col_frag(lds[buf][3], 32 * (TW * wj + i), s);
+                    qh[i] = col_frag(img + 2 * PL, 32 * (TW * wj + i), s);
+                    ql[i] = col_frag(img + 3 * PL, 32 * (TW * wj + i), s);
                 } else {
-                    qh[i] = row_frag(lds[buf][2], 32 * (TW * wj + i), s);
-                    ql[i] = row_frag(lds[buf][3], 32 * (TW * wj + i), s);
+                    qh[i] = row_frag(img + 2 * PL, 32 * (TW * wj + i), s);
+                    ql[i] = row_frag(img + 3 * PL, 32 * (TW * wj + i), s);
                 }
             }
 #pragma unroll
-            for (int i = 0; i < TW; ++i)
+            for (int x = 0; x < 3; ++x)
 #pragma unroll
-                for (int j = 0; j < TW; ++j) {
-                    acc[i][j] = mfma32h(ql[j], ph[i], acc[i][j]);
-                    acc[i][j] = mfma32h(qh[j], pl[i], acc[i][j]);
-                    acc[i][j] = mfma32h(qh[j], ph[i], acc[i][j]);
-                }
+                for (int i = 0; i < TW; ++i)
+#pragma unroll
+                    for (int j = 0; j < TW; ++j) acc[i][j] = mfma32h(x == 0 ? ql[j] : qh[j], x == 1 ? pl[i] : ph[i], acc[i][j]);
         }
     };
-    issue(0, 0);
-    dma_wait_and_barrier();
+    // every wave issues 4 PIECES operations per stage: "all but the newest NST - 2 stages have landed" is one counted wait
+#pragma unroll
+    for (int t = 0; t < NST - 1; ++t)
+        if (t < nk) issue(t, t);
+    int buf = 0;
     for (int t = 0; t < nk; ++t) {
-        if (t + 1 < nk) issue(t + 1, (t + 1) & 1);
-        compute(t & 1);
-        dma_wait_and_barrier();
+        if (t + NST - 1 <= nk) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * PIECES * (NST - 2)) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();  // stage t is there for all; the stage before it has been read by all
+        if (t + NST - 1 < nk) issue(t + NST - 1, buf == 0 ? NST - 1 : buf - 1);
+        compute(buf);
+        buf = buf + 1 == NST ? 0 : buf + 1;
     }
-
-    // ---- epilogue
-    const f16_t* D = KIND == NS_POLY ? A : X;
-    const size_t dlo = KIND == NS_POLY ? alo : xlo;
-    const int ldd = KIND == NS_POLY ? u.mp : u.np, cols = SYM ? u.mp : u.np;
-    f16_t* C = (f16_t*)(ws + (KIND == NS_GRAM ? u.a : KIND == NS_POLY ? u.s : u.x[st.from ^ 1]));
-    const size_t clo = SYM ? alo : xlo;
-    const int ldc = cols;
-#pragma unroll
-    for (int ti = 0; ti < TW; ++ti) {
-        const int i = i0 + 32 * (TW * wi + ti) + r;
-        if (i >= u.mp) continue;
-#pragma unroll
-        for (int tj = 0; tj < TW; ++tj)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int j = j0 + 32 * (TW * wj + tj) + 8 * q + 4 * h;
-                if (j >= cols) continue;  // cols is a multiple of 32: groups of 4 are whole
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = st.alpha * acc[ti][tj][4 * q + e];
-                typedef f16_t f16x4 __attribute__((ext_vector_type(4)));
-                if constexpr (KIND != NS_GRAM) {
-                    const f16x4 dh = *(const f16x4*)(D + (size_t)i * ldd + j), dl = *(const f16x4*)(D + dlo + (size_t)i * ldd + j);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] += st.beta * ((float)dh[e] + (float)dl[e]);
-                }
-                if constexpr (KIND == NS_LAST) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int row = u.trans ? j + e : i, col = u.trans ? i : j + e;
-                        if (row >= u.rows || col >= u.cols) continue;
-                        const long long at = (long long)row * u.cols + col;
-                        const float o = v[e] * st.inv;
-                        if (u.out) ((T*)u.out)[at] = (T)o;
-                        else u.w[at] = u.decay * u.w[at] - u.lr * o;
-                    }
-                } else {
-                    f16x4 ch, cl;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        f16_t a, b;
-                        ns_split(v[e], a, b);
-                        ch[e] = a;
-                        cl[e] = b;
-                    }
-                    *(f16x4*)(C + (size_t)i * ldc + j) = ch;
-                    *(f16x4*)(C + clo + (size_t)i * ldc + j) = cl;
-                    if constexpr (SYM) {
-                        if (bi != bj) {  // the lower triangle
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                C[(size_t)(j + e) * ldc + i] = ch[e];
-                                C[clo + (size_t)(j + e) * ldc + i] = cl[e];
-                            }
-                        }
-                    }
-                }
-            }
-    }
+    __syncthreads();
+    ns_epilogue<TW, KIND, T>(u, w, st, acc, (float*)lds + wave * (32 * TW) * (32 * TW), wi, wj, lane);
 }
 
 // no steps: the normalised update itself
@@ -436,25 +507,25 @@ bool ns_exponent(const float* coefficients, int steps, int* exponent) {
     return true;
 }
 
-template <int B, int KIND, typename T>
+template <int TW, int KIND, typename T>
 int ns_gemm(const NsLayout& l, const NsUnit* table, int n, char* ws, const NsStep& st, hipStream_t s) {
     const int grid = KIND == NS_GRAM || KIND == NS_POLY ? l.nsym : l.nfull;
-    hipLaunchKernelGGL((ns_gemm_kernel<B, KIND, T>), dim3(grid), dim3(256), 0, s, table, n, ws, st);
+    hipLaunchKernelGGL((ns_gemm_kernel<TW, KIND, T>), dim3(grid), dim3(256), 0, s, table, n, ws, st);
     return hipGetLastError() == hipSuccess ? V1T_OK : V1T_ERR_LAUNCH;
 }
 
 #define NS_TRY(x) do { const int rc_ = (x); if (rc_ != V1T_OK) return rc_; } while (0)
 
-template <int B, typename T>
+template <int TW, typename T>
 int ns_steps(const NsLayout& l, const NsUnit* table, int n, char* ws, int steps, const float* co, int exponent, hipStream_t s) {
     const float inv = std::ldexp(1.f, -exponent);
     for (int k = 0; k < steps; ++k) {
         const float a = co[3 * k], b = co[3 * k + 1], c = co[3 * k + 2];
-        NS_TRY((ns_gemm<B, NS_GRAM, float>(l, table, n, ws, NsStep{inv, 0.f, k & 1, inv}, s)));
-        NS_TRY((ns_gemm<B, NS_POLY, float>(l, table, n, ws, NsStep{c * inv, b, k & 1, inv}, s)));
+        NS_TRY((ns_gemm<TW, NS_GRAM, float>(l, table, n, ws, NsStep{inv, 0.f, k & 1, inv}, s)));
+        NS_TRY((ns_gemm<TW, NS_POLY, float>(l, table, n, ws, NsStep{c * inv, b, k & 1, inv}, s)));
         const NsStep last{inv, a, k & 1, inv};
-        if (k + 1 < steps) NS_TRY((ns_gemm<B, NS_APPLY, float>(l, table, n, ws, last, s)));
-        else NS_TRY((ns_gemm<B, NS_LAST, T>(l, table, n, ws, last, s)));
+        if (k + 1 < steps) NS_TRY((ns_gemm<TW, NS_APPLY, float>(l, table, n, ws, last, s)));
+        else NS_TRY((ns_gemm<TW, NS_LAST, T>(l, table, n, ws, last, s)));
     }
     return V1T_OK;
 }
@@ -470,7 +541,7 @@ int ns_run(const NsLayout& l, int n, char* ws, const NsMomentum& mo, float eps, 
         hipLaunchKernelGGL((ns_copy_kernel<T>), dim3(l.nprep), dim3(256), 0, s, table, n, ws, std::ldexp(1.f, -exponent));
         return hipGetLastError() == hipSuccess ? V1T_OK : V1T_ERR_LAUNCH;
     }
-    return l.tile == 128 ? ns_steps<128, T>(l, table, n, ws, steps, co, exponent, s) : ns_steps<64, T>(l, table, n, ws, steps, co, exponent, s);
+    return l.tile == 128 ? ns_steps<2, T>(l, table, n, ws, steps, co, exponent, s) : ns_steps<1, T>(l, table, n, ws, steps, co, exponent, s);
 }
 
 // lays out the units, checks the workspace, writes the table
