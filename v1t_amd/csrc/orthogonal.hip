@@ -17,6 +17,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <utility>
 
 #include "../../include/v1t_amd.h"
 #include "common.h"
@@ -24,7 +25,7 @@
 namespace {
 
 constexpr int NS_BK = 32;            // K step of the products; planes are padded to it with zeros both ways
-constexpr int NS_PART = 16384;       // elements per partial sum of squares
+constexpr int NS_PART = 4096;        // least number of elements per partial sum of squares; at most 1024 partial sums a unit
 constexpr int NS_TILE_PREP = 64;     // the first planes are written in 64 x 64 tiles
 constexpr int NS_CHUNK = 16;         // units per table launch (kernel arguments)
 constexpr int NS_MAX_STEPS = 32;
@@ -36,7 +37,7 @@ struct NsUnit {
     long long rs, cs;                // element strides of `in`; out, mom and w are row-major without gaps
     long long x[2], a, s;            // byte offsets of the planes in the workspace (hi, and lo behind it)
     int rows, cols, m, n, mp, np, trans;
-    int part0, nparts, prep0, sym0, full0;  // first workgroup of this unit in the launches of each kind
+    int part, part0, nparts, prep0, sym0, full0;  // first workgroup of this unit in the launches of each kind
     float lr, decay, l1;             // w <- decay w - lr O;  gradient + l1 sign(w)
 };
 
@@ -80,33 +81,62 @@ DEVFN double ns_block_sum(double v) {
     return s[0];
 }
 
-template <typename T>
-DEVFN float ns_gradient(const NsUnit& u, int r, int c, long long i) {
-    const float g = (float)((const T*)u.in)[(long long)r * u.rs + (long long)c * u.cs];
-    return u.l1 == 0.f ? g : g + u.l1 * ns_sign(u.w[i]);
-}
-// the update's element (r, c). MOM: the gradient with its L1 term in front of the momentum (already updated), Nesterov's look ahead
-template <typename T, bool MOM>
-DEVFN float ns_update(const NsUnit& u, const NsMomentum& mo, int r, int c) {
-    if constexpr (!MOM) return (float)((const T*)u.in)[(long long)r * u.rs + (long long)c * u.cs];
-    const long long i = (long long)r * u.cols + c;
-    const float m = u.mom[i];
-    return mo.nesterov ? ns_gradient<T>(u, r, c, i) + mo.mu * m : m;
-}
+// N elements of the update: gradient with its L1 term, momentum (MOM), then U. The loads of a batch stand together: each of a tensor that is written, too, would
+// wait for the store before it
+template <typename T, bool MOM, int N>
+struct NsBatch {
+    float g[N], m[N];
+    DEVFN void load(const NsUnit& u, const long long (&src)[N], const long long (&at)[N], const bool (&on)[N]) {
+        float w[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) g[e] = on[e] ? (float)((const T*)u.in)[src[e]] : 0.f;
+        if constexpr (MOM) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) m[e] = on[e] ? u.mom[at[e]] : 0.f;
+            if (u.l1 != 0.f) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) w[e] = on[e] ? u.w[at[e]] : 0.f;
+#pragma unroll
+                for (int e = 0; e < N; ++e) g[e] += u.l1 * ns_sign(w[e]);
+            }
+        }
+    }
+    DEVFN float update(const NsMomentum& mo, int e) const { return !MOM ? g[e] : mo.nesterov ? g[e] + mo.mu * m[e] : m[e]; }
+};
 
 // partial sums of squares, in 64 bits (their range is that of the inputs squared); MOM: momentum <- mu momentum + gradient on the way
 template <typename T, bool MOM>
 __global__ __launch_bounds__(256) void ns_norm_kernel(const NsUnit* units, int n, NsMomentum mo, double* parts) {
+    constexpr int N = 8;
     const NsUnit& u = ns_find(units, n, blockIdx.x, &NsUnit::part0);
-    const long long all = (long long)u.rows * u.cols, i0 = (long long)(blockIdx.x - u.part0) * NS_PART;
-    const int len = (int)min((long long)NS_PART, all - i0);
+    const long long all = (long long)u.rows * u.cols, i0 = (long long)(blockIdx.x - u.part0) * u.part;
+    const int len = (int)min((long long)u.part, all - i0);
+    const bool flat = u.cs == 1 && u.rs == u.cols;
     double sum = 0.0;
-    for (int k = threadIdx.x; k < len; k += 256) {
-        const long long i = i0 + k;
-        const int r = (int)(i / u.cols), c = (int)(i - (long long)r * u.cols);
-        if constexpr (MOM) u.mom[i] = mo.mu * u.mom[i] + ns_gradient<T>(u, r, c, i);
-        const double v = (double)ns_update<T, MOM>(u, mo, r, c);
-        sum += v * v;
+    for (int k0 = 0; k0 < len; k0 += 256 * N) {
+        long long src[N], at[N];
+        bool on[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int k = k0 + 256 * e + (int)threadIdx.x;
+            on[e] = k < len;
+            at[e] = src[e] = i0 + k;
+            if (!flat) {
+                const long long r = at[e] / u.cols;
+                src[e] = r * u.rs + (at[e] - r * u.cols) * u.cs;
+            }
+        }
+        NsBatch<T, MOM, N> b;
+        b.load(u, src, at, on);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            if constexpr (MOM) {
+                b.m[e] = mo.mu * b.m[e] + b.g[e];
+                if (on[e]) u.mom[at[e]] = b.m[e];
+            }
+            const double v = (double)b.update(mo, e);
+            sum += v * v;
+        }
     }
     sum = ns_block_sum(sum);
     if (threadIdx.x == 0) parts[blockIdx.x] = sum;
@@ -130,16 +160,28 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(const NsUnit* units, int n
     const int tj = (u.np + NS_TILE_PREP - 1) / NS_TILE_PREP, t = blockIdx.x - u.prep0;
     const int i0 = t / tj * NS_TILE_PREP, j0 = t % tj * NS_TILE_PREP;  // in X
     const int r0 = u.trans ? j0 : i0, c0 = u.trans ? i0 : j0;            // in the update
-    for (int k = threadIdx.x; k < NS_TILE_PREP * NS_TILE_PREP; k += 256) {
-        const int r = k / NS_TILE_PREP, c = k % NS_TILE_PREP;
-        float v = 0.f;
-        if (r0 + r < u.rows && c0 + c < u.cols) {
-            v = (float)((double)ns_update<T, MOM>(u, mo, r0 + r, c0 + c) * mul);
-            if constexpr (MOM) {
-                if (zero) ((T*)u.in)[(long long)(r0 + r) * u.rs + (long long)(c0 + c) * u.cs] = (T)0.f;
-            }
+    constexpr int N = 8;
+#pragma unroll
+    for (int k0 = 0; k0 < NS_TILE_PREP * NS_TILE_PREP; k0 += 256 * N) {
+        long long src[N], at[N];
+        bool on[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int k = k0 + 256 * e + (int)threadIdx.x, r = r0 + k / NS_TILE_PREP, c = c0 + k % NS_TILE_PREP;
+            on[e] = r < u.rows && c < u.cols;
+            src[e] = (long long)r * u.rs + (long long)c * u.cs;
+            at[e] = (long long)r * u.cols + c;
         }
-        s[r][c] = v;
+        NsBatch<T, MOM, N> b;
+        b.load(u, src, at, on);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int k = k0 + 256 * e + (int)threadIdx.x;
+            if constexpr (MOM) {
+                if (zero && on[e]) ((T*)u.in)[src[e]] = (T)0.f;
+            }
+            s[k / NS_TILE_PREP][k % NS_TILE_PREP] = on[e] ? (float)((double)b.update(mo, e) * mul) : 0.f;
+        }
     }
     __syncthreads();
     f16_t* hi = (f16_t*)(ws + u.x[0]);
@@ -285,16 +327,30 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
             *(f16x8*)(w.Cl + (size_t)j * w.cols + i) = cl;
         }
     } else if constexpr (KIND == NS_LAST) {
-        auto put = [&](int row, int col, float o) {
-            if (row >= u.rows || col >= u.cols) return;
-            const long long x = (long long)row * u.cols + col;
-            if (u.out) ((T*)u.out)[x] = (T)o;
-            else u.w[x] = u.decay * u.w[x] - u.lr * o;
-        };
-        for (int k = lane; k < SIDE * SIDE; k += 64) {
-            const int a = k / SIDE, b = k % SIDE;  // b runs along the result's rows
-            if (u.trans) put(jw + a, iw + b, at(b, a) * st.inv);
-            else put(iw + a, jw + b, at(a, b) * st.inv);
+        constexpr int N = 8;
+        for (int k0 = lane; k0 < SIDE * SIDE; k0 += 64 * N) {  // a batch's loads of the weights stand together
+            long long x[N];
+            float o[N], wt[N];
+            bool on[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int a = (k0 + 64 * e) / SIDE, b = (k0 + 64 * e) % SIDE;  // b runs along the result's rows
+                const int row = (u.trans ? jw : iw) + a, col = (u.trans ? iw : jw) + b;
+                on[e] = row < u.rows && col < u.cols;
+                x[e] = (long long)row * u.cols + col;
+                o[e] = (u.trans ? at(b, a) : at(a, b)) * st.inv;
+            }
+            if (u.out) {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (on[e]) ((T*)u.out)[x[e]] = (T)o[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) wt[e] = on[e] ? u.w[x[e]] : 0.f;
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (on[e]) u.w[x[e]] = u.decay * wt[e] - u.lr * o[e];
+            }
         }
     }
 }
@@ -439,6 +495,11 @@ struct NsLayout {
     int nparts = 0, nprep = 0, nsym = 0, nfull = 0, tile = 128;
     long long sym128 = 0, full128 = 0;
 };
+// elements per partial sum, and how many sums
+std::pair<int, int> ns_parts(long long elements) {
+    const long long part = std::max<long long>(NS_PART, (elements + 1023) / 1024);
+    return {(int)part, (int)((elements + part - 1) / part)};
+}
 long long ns_align(long long x) { return (x + 255) / 256 * 256; }
 
 // Places every unit's planes. `shape(i, rows, cols)`; `put` (or null) receives the filled units in order.
@@ -455,7 +516,7 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
         const long long a = (m + 127) / 128, b = (nn + 127) / 128;
         sym += a * (a + 1) / 2;
         full += a * b;
-        nparts += (m * nn + NS_PART - 1) / NS_PART;
+        nparts += ns_parts(m * nn).second;
     }
     l.sym128 = sym; l.full128 = full;
     l.tile = sym >= 256 ? 128 : 64;
@@ -474,7 +535,7 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
         at = u.s + ab;
         const long long ti = (u.mp + l.tile - 1) / l.tile, tj = (u.np + l.tile - 1) / l.tile;
         const long long pi = (u.mp + NS_TILE_PREP - 1) / NS_TILE_PREP, pj = (u.np + NS_TILE_PREP - 1) / NS_TILE_PREP;
-        u.part0 = (int)part; u.nparts = (int)(((long long)u.rows * u.cols + NS_PART - 1) / NS_PART);
+        u.part = ns_parts((long long)u.rows * u.cols).first; u.part0 = (int)part; u.nparts = ns_parts((long long)u.rows * u.cols).second;
         u.prep0 = (int)prep; u.sym0 = (int)s0; u.full0 = (int)f0;
         part += u.nparts; prep += pi * pj; s0 += ti * (ti + 1) / 2; f0 += ti * tj;
         if (std::max(std::max(part, prep), std::max(s0, f0)) > 0x7fffffffll) return V1T_ERR_UNSUPPORTED;
