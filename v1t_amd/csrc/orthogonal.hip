@@ -18,6 +18,7 @@
 #include <cmath>
 #include <cstring>
 #include <utility>
+#include <vector>
 
 #include "../../include/v1t_amd.h"
 #include "common.h"
@@ -28,7 +29,7 @@ constexpr int NS_BK = 32;            // K step of the products; planes are padde
 constexpr int NS_PART = 4096;        // least number of elements per partial sum of squares; at most 1024 partial sums a unit
 constexpr int NS_TILE_PREP = 64;     // the first planes are written in 64 x 64 tiles
 constexpr int NS_CHUNK = 16;         // units per table launch (kernel arguments)
-constexpr int NS_MAX_STEPS = 32;
+constexpr int NS_MAX_STEPS = 32, NS_MAX_UNITS = 1 << 16;
 
 struct NsUnit {
     const void* in;   // the update, or the gradient
@@ -37,7 +38,9 @@ struct NsUnit {
     long long rs, cs;                // element strides of `in`; out, mom and w are row-major without gaps
     long long x[2], a, s;            // byte offsets of the planes in the workspace (hi, and lo behind it)
     int rows, cols, m, n, mp, np, trans;
-    int part, part0, nparts, prep0, sym0, full0;  // first workgroup of this unit in the launches of each kind
+    int part, part0, nparts, prep0;  // elements per partial sum; first workgroup of this unit in the launches of each kind
+    int first[3];                    // first tile in the products' launches: gram, poly, apply / last
+    int group0[3], group[3];         // first tile and tiles of the run of units of this size
     float lr, decay, l1;             // w <- decay w - lr O;  gradient + l1 sign(w)
 };
 
@@ -51,15 +54,23 @@ __global__ void ns_table_kernel(NsChunk c, int n, NsUnit* to) {
     for (int i = threadIdx.x; i < n * (int)(sizeof(NsUnit) / 4); i += blockDim.x) ((uint32_t*)to)[i] = src[i];
 }
 
-// the unit whose range of workgroups `block` falls into: the last one that begins at or before it
-DEVFN const NsUnit& ns_find(const NsUnit* u, int n, int block, int NsUnit::*first) {
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (u[mid].*first <= block) lo = mid;
-        else hi = mid - 1;
+// the unit whose range of workgroups `block` falls into: the last one that begins at or before it. 64 units' beginnings are read at once - a search would wait
+// for one read after another. W: the launch - 0 .. 2 the products', 3 the partial sums', 4 the first planes'
+template <int W>
+DEVFN int ns_find(const NsUnit* u, int n, int block) {
+    const int lane = threadIdx.x & 63;
+    int found = -1;
+    for (int i = 0; i < n; i += 64) {
+        bool before = false;
+        if (i + lane < n) {
+            const NsUnit& x = u[i + lane];
+            before = (W < 3 ? x.first[W < 3 ? W : 0] : W == 3 ? x.part0 : x.prep0) <= block;
+        }
+        const int k = __popcll(__ballot(before));
+        found += k;
+        if (k < 64) break;
     }
-    return u[lo];
+    return __builtin_amdgcn_readfirstlane(found);
 }
 
 struct NsMomentum {
@@ -108,7 +119,7 @@ struct NsBatch {
 template <typename T, bool MOM>
 __global__ __launch_bounds__(256) void ns_norm_kernel(const NsUnit* units, int n, NsMomentum mo, double* parts) {
     constexpr int N = 8;
-    const NsUnit& u = ns_find(units, n, blockIdx.x, &NsUnit::part0);
+    const NsUnit& u = units[ns_find<3>(units, n, blockIdx.x)];
     const long long all = (long long)u.rows * u.cols, i0 = (long long)(blockIdx.x - u.part0) * u.part;
     const int len = (int)min((long long)u.part, all - i0);
     const bool flat = u.cs == 1 && u.rs == u.cols;
@@ -151,7 +162,7 @@ DEVFN void ns_split(float v, f16_t& hi, f16_t& lo) {
 // cleared behind its last reader
 template <typename T, bool MOM>
 __global__ __launch_bounds__(256) void ns_prep_kernel(const NsUnit* units, int n, NsMomentum mo, const double* parts, char* ws, float eps, float scale, int zero) {
-    const NsUnit& u = ns_find(units, n, blockIdx.x, &NsUnit::prep0);
+    const NsUnit& u = units[ns_find<4>(units, n, blockIdx.x)];
     __shared__ float s[NS_TILE_PREP][NS_TILE_PREP + 1];
     double sum = 0.0;
     for (int i = threadIdx.x; i < u.nparts; i += 256) sum += parts[u.part0 + i];
@@ -210,7 +221,20 @@ struct NsStep {
     float alpha, beta;   // C <- alpha (P Q^T) + beta D, on the scaled planes
     int from;            // which of the two X planes is read
     float inv;           // 2^-e
+    int whole, split;    // tiles [0, whole) are computed by a workgroup each, the others in `split` pieces of their K steps
+    float* slab;         // the pieces' sums
 };
+
+constexpr int ns_launch(int kind) { return kind == NS_GRAM ? 0 : kind == NS_POLY ? 1 : 2; }
+
+// The tile of a run that its workgroup number `local` computes: workgroups b, b + 8, .. share an XCD and its L2, and get neighbouring tiles. A run is all units of
+// one size: over a whole launch one XCD would get the units with the longest K, over one unit an XCD would read a part of every unit
+DEVFN int ns_deal(int local, int first, int count) {
+    const int d = first & 7, v = local + d, x = v & 7, end = count + d;
+    const int base = (end >> 3) * x + min(end & 7, x) - min(d, x);  // tiles of the XCDs before this one
+    const int lead = x >= d ? x : x + 8;
+    return base + ((v - lead) >> 3);
+}
 typedef f16_t f16x4 __attribute__((ext_vector_type(4)));
 
 template <int TW>
@@ -230,18 +254,17 @@ struct NsWhere {
     int ldd, cols;
 };
 template <int TW, int KIND>
-DEVFN NsWhere ns_where(const NsUnit& u, char* ws, const NsStep& st, int block) {
+DEVFN NsWhere ns_where(const NsUnit& u, char* ws, const NsStep& st, int t) {  // t: the unit's tile
     constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY;
     constexpr int B = NsTile<TW>::B;
     NsWhere w;
     if constexpr (SYM) {  // tile number -> (bi <= bj) of the upper triangle, columns of tiles one after another
-        const int t = block - u.sym0;
         w.bj = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
         while ((w.bj + 1) * (w.bj + 2) / 2 <= t) ++w.bj;
         while (w.bj * (w.bj + 1) / 2 > t) --w.bj;
         w.bi = t - w.bj * (w.bj + 1) / 2;
     } else {
-        const int t = block - u.full0, ni = (u.mp + B - 1) / B;
+        const int ni = (u.mp + B - 1) / B;
         w.bi = t % ni;
         w.bj = t / ni;
     }
@@ -362,10 +385,20 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(const NsU
     constexpr int B = Tile::B, PL = Tile::PL, PIECES = Tile::PIECES, NST = Tile::NST;
     __shared__ __attribute__((aligned(16))) f16_t lds[Tile::LDS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave >> 1, wj = wave & 1;
-    const int block = xcd_remap(blockIdx.x, gridDim.x);
-    const NsUnit& u = ns_find(units, n, block, SYM ? &NsUnit::sym0 : &NsUnit::full0);
-    const NsWhere w = ns_where<TW, KIND>(u, ws, st, block);
-    const int K = KIND == NS_GRAM ? u.np : u.mp, nk = K / NS_BK;
+    constexpr int W = ns_launch(KIND);
+    const int b = blockIdx.x, over = b - st.whole;
+    const bool piece = SYM && over >= 0;  // workgroup-uniform
+    int number = b;
+    if (piece) {
+        number = st.whole + over / st.split;
+    } else {
+        const NsUnit& g = units[ns_find<W>(units, n, b)];
+        number = g.group0[W] + ns_deal(b - g.group0[W], g.group0[W], SYM ? min(g.group[W], st.whole - g.group0[W]) : g.group[W]);
+    }
+    const NsUnit& u = units[ns_find<W>(units, n, number)];
+    const NsWhere w = ns_where<TW, KIND>(u, ws, st, number - u.first[W]);
+    const int steps = (KIND == NS_GRAM ? u.np : u.mp) / NS_BK, each = piece ? (steps + st.split - 1) / st.split : steps;
+    const int t0 = piece ? over % st.split * each : 0, nk = max(0, min(each, steps - t0));  // this workgroup's K steps
     const f16_t* X = (const f16_t*)(ws + u.x[st.from]);
     const f16_t* A = (const f16_t*)(ws + u.a);
     const f16_t* P = KIND == NS_GRAM ? X : KIND == NS_POLY ? A : (const f16_t*)(ws + u.s);
@@ -399,7 +432,7 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(const NsU
         return (const char*)(uintptr_t)(((unsigned long long)hi << 32) | lo);
     };
     auto issue = [&](int t, int buf) {
-        const size_t pk = (size_t)t * (2 * NS_BK), qk = TR ? (size_t)t * (2 * NS_BK) * ldq : (size_t)t * (2 * NS_BK);
+        const size_t pk = (size_t)(t0 + t) * (2 * NS_BK), qk = TR ? (size_t)(t0 + t) * (2 * NS_BK) * ldq : (size_t)(t0 + t) * (2 * NS_BK);
 #pragma unroll
         for (int plane = 0; plane < 4; ++plane) {
             const char* base = uniform(plane == 0 ? pb + pk : plane == 1 ? pb + pk + 2 * plo : plane == 2 ? qb + qk : qb + qk + 2 * qlo);
@@ -467,14 +500,55 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(const NsU
         compute(buf);
         buf = buf + 1 == NST ? 0 : buf + 1;
     }
+    if (piece) {  // its sums in the accumulators' order; ns_join_kernel adds the pieces up
+        float* to = st.slab + ((size_t)over * 4 + wave) * (TW * TW * 1024) + 4 * lane;
+#pragma unroll
+        for (int i = 0; i < TW; ++i)
+#pragma unroll
+            for (int j = 0; j < TW; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) *(f32x4*)(to + ((i * TW + j) * 4 + q) * 256) = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        return;
+    }
     __syncthreads();
     ns_epilogue<TW, KIND, T>(u, w, st, acc, (float*)lds + wave * (32 * TW) * (32 * TW), wi, wj, lane);
+}
+
+// The pieces of the split tiles, added up in their order, and the epilogue: one wave per quarter of a tile
+template <int TW, int KIND>
+__global__ __launch_bounds__(64) void ns_join_kernel(const NsUnit* units, int n, char* ws, NsStep st) {
+    constexpr int W = ns_launch(KIND);
+    __shared__ __attribute__((aligned(16))) float lds[32 * TW * 32 * TW];
+    const int lane = threadIdx.x, wave = blockIdx.x & 3, tile = blockIdx.x >> 2;
+    const NsUnit& u = units[ns_find<W>(units, n, st.whole + tile)];
+    const NsWhere w = ns_where<TW, KIND>(u, ws, st, st.whole + tile - u.first[W]);
+    f32x16 acc[TW][TW];
+#pragma unroll
+    for (int i = 0; i < TW; ++i)
+#pragma unroll
+        for (int j = 0; j < TW; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    for (int p = 0; p < st.split; ++p) {
+        const float* from = st.slab + (((size_t)tile * st.split + p) * 4 + wave) * (TW * TW * 1024) + 4 * lane;
+#pragma unroll
+        for (int i = 0; i < TW; ++i)
+#pragma unroll
+            for (int j = 0; j < TW; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 v = *(const f32x4*)(from + ((i * TW + j) * 4 + q) * 256);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += v[e];
+                }
+    }
+    ns_epilogue<TW, KIND, float>(u, w, st, acc, lds, wave >> 1, wave & 1, lane);
 }
 
 // no steps: the normalised update itself
 template <typename T>
 __global__ __launch_bounds__(256) void ns_copy_kernel(const NsUnit* units, int n, const char* ws, float inv) {
-    const NsUnit& u = ns_find(units, n, blockIdx.x, &NsUnit::prep0);
+    const NsUnit& u = units[ns_find<4>(units, n, blockIdx.x)];
     const int tj = (u.np + NS_TILE_PREP - 1) / NS_TILE_PREP, t = blockIdx.x - u.prep0;
     const int i0 = t / tj * NS_TILE_PREP, j0 = t % tj * NS_TILE_PREP;
     const f16_t* hi = (const f16_t*)(ws + u.x[0]);
@@ -490,10 +564,17 @@ __global__ __launch_bounds__(256) void ns_copy_kernel(const NsUnit* units, int n
 }
 
 // ---- host ---------------------------------------------------------------------------------
+// A product's launch: tiles of 64 tw, the first `whole` computed whole, the others in `split` pieces
+struct NsPlan {
+    int tw = 1, tiles = 0, whole = 0, split = 1;
+    int grid() const { return whole + (tiles - whole) * split; }
+    int joined() const { return tiles - whole; }
+    long long slab() const { return split > 1 ? (long long)(tiles - whole) * split * 16384ll * tw * tw : 0; }
+};
 struct NsLayout {
-    long long table = 0, parts = 0, bytes = 0;
-    int nparts = 0, nprep = 0, nsym = 0, nfull = 0, tile = 128;
-    long long sym128 = 0, full128 = 0;
+    long long table = 0, parts = 0, slab = 0, bytes = 0;
+    int nparts = 0, nprep = 0;
+    NsPlan gram, poly, full;
 };
 // elements per partial sum, and how many sums
 std::pair<int, int> ns_parts(long long elements) {
@@ -502,46 +583,105 @@ std::pair<int, int> ns_parts(long long elements) {
 }
 long long ns_align(long long x) { return (x + 255) / 256 * 256; }
 
-// Places every unit's planes. `shape(i, rows, cols)`; `put` (or null) receives the filled units in order.
+// Tile and split of a product with t64 / t128 tiles of each size whose K steps sum to k64 / k128, at the least estimated time. A CU holds two workgroups of
+// either tile. Measured, us per K step: the larger tile 1.6 with two on a CU and 0.9 alone, the smaller 0.85 and 0.25 (so the larger does twice
+// the work in a time, where there is enough of it), their epilogues 5 and 1.5; the launch that joins pieces 6, and their sums at 3 TB/s. Only the tiles of the last, part-filled round
+// are split, in pieces of at least 4 steps.
+NsPlan ns_plan(long long t64, long long k64, long long t128, long long k128, bool may_split) {
+    constexpr int SLOTS = 512, CUS = 256;
+    NsPlan best;
+    double least = 1e30;
+    for (int tw = 1; tw <= 2; ++tw) {
+        const long long tiles = tw == 1 ? t64 : t128;
+        const double steps = (double)(tw == 1 ? k64 : k128) / (double)tiles;
+        const double full = tw == 1 ? 0.85 : 1.6, alone = tw == 1 ? 0.25 : 0.9;
+        for (int split = 1; split <= (may_split ? 16 : 1); ++split) {
+            const long long whole = split == 1 ? tiles : tiles / SLOTS * SLOTS, rest = tiles - whole, pieces = rest * split;
+            if (split > 1 && (rest == 0 || pieces > SLOTS || steps < 4 * split)) continue;
+            const double tail = tw == 1 ? 1.5 : 5.0;
+            auto round = [&](double k, long long w) { return w == 0 ? 0.0 : tail + k * (w <= CUS ? alone : full); };
+            double t = (double)(whole / SLOTS) * round(steps, SLOTS) + round(steps, whole % SLOTS);
+            if (split > 1) t += round(steps / split, pieces) + 6.0 + (double)pieces * tw * tw * 16384.0 * 2.0 / 3e6;
+            if (t < least) {
+                least = t;
+                best.tw = tw; best.tiles = (int)tiles; best.whole = (int)whole; best.split = split;
+            }
+        }
+    }
+    return best;
+}
+
+// Places every unit's planes. `shape(i, rows, cols)`; `put` receives the filled units in the order of the table.
 template <typename Shape, typename Put>
 int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
-    long long nparts = 0;
-    long long sym = 0, full = 0;
+    if (n > NS_MAX_UNITS) return V1T_ERR_UNSUPPORTED;
+    long long nparts = 0, prep = 0;
+    long long gt[2] = {}, gk[2] = {}, pk[2] = {}, ft[2] = {}, fk[2] = {};  // tiles and K steps: 64, 128
+    std::vector<int> order(n);
+    std::vector<std::pair<int, int>> size(n);
     for (int i = 0; i < n; ++i) {
         int rows, cols;
         shape(i, rows, cols);
         if (rows < 1 || cols < 1) return V1T_ERR_ARG;
         const long long m = std::min(rows, cols), nn = std::max(rows, cols);
         if (m > 32768 || nn > (1 << 22) || m * nn > (1ll << 31)) return V1T_ERR_UNSUPPORTED;
-        const long long a = (m + 127) / 128, b = (nn + 127) / 128;
-        sym += a * (a + 1) / 2;
-        full += a * b;
+        size[i] = {(int)nn, (int)m};
+        order[i] = i;
+        for (int k = 0; k < 2; ++k) {
+            const long long B = 64 << k, mp = round_up((int)m, NS_BK), np = round_up((int)nn, NS_BK), a = (mp + B - 1) / B, b = (np + B - 1) / B;
+            gt[k] += a * (a + 1) / 2; gk[k] += a * (a + 1) / 2 * (np / NS_BK); pk[k] += a * (a + 1) / 2 * (mp / NS_BK);
+            ft[k] += a * b; fk[k] += a * b * (mp / NS_BK);
+        }
         nparts += ns_parts(m * nn).second;
+        prep += (m / NS_TILE_PREP + 1) * (nn / NS_TILE_PREP + 1);
     }
-    l.sym128 = sym; l.full128 = full;
-    l.tile = sym >= 256 ? 128 : 64;
+    if (std::max(std::max(gt[0], ft[0]), std::max(nparts, prep)) > 0x3fffffffll) return V1T_ERR_UNSUPPORTED;
+    if (n == 0) return V1T_OK;
+    // the tiles with the longest K first: what is left for the last round is short
+    std::sort(order.begin(), order.end(), [&](int a, int b) { return size[a] != size[b] ? size[a] > size[b] : a < b; });
+    l.gram = ns_plan(gt[0], gk[0], gt[1], gk[1], true);
+    l.poly = ns_plan(gt[0], pk[0], gt[1], pk[1], true);
+    l.full = ns_plan(ft[0], fk[0], ft[1], fk[1], false);
     l.table = 0;
     l.parts = ns_align((long long)n * (long long)sizeof(NsUnit));
-    long long at = ns_align(l.parts + 8 * nparts);
-    long long part = 0, prep = 0, s0 = 0, f0 = 0;
-    for (int i = 0; i < n; ++i) {
+    l.slab = ns_align(l.parts + 8 * nparts);
+    long long at = ns_align(l.slab + std::max(l.gram.slab(), l.poly.slab()));
+    int part = 0, first = 0, next[3] = {}, group0[3] = {}, group[3] = {};
+    for (int k = 0; k < n; ++k) {
         NsUnit u{};
-        shape(i, u.rows, u.cols);
+        shape(order[k], u.rows, u.cols);
         u.trans = u.rows > u.cols;
         u.m = std::min(u.rows, u.cols); u.n = std::max(u.rows, u.cols);
         u.mp = round_up(u.m, NS_BK); u.np = round_up(u.n, NS_BK);
         const long long xb = ns_align(4ll * u.mp * u.np), ab = ns_align(4ll * u.mp * u.mp);
         u.x[0] = at; u.x[1] = at + xb; u.a = at + 2 * xb; u.s = u.a + ab;
         at = u.s + ab;
-        const long long ti = (u.mp + l.tile - 1) / l.tile, tj = (u.np + l.tile - 1) / l.tile;
-        const long long pi = (u.mp + NS_TILE_PREP - 1) / NS_TILE_PREP, pj = (u.np + NS_TILE_PREP - 1) / NS_TILE_PREP;
-        u.part = ns_parts((long long)u.rows * u.cols).first; u.part0 = (int)part; u.nparts = ns_parts((long long)u.rows * u.cols).second;
-        u.prep0 = (int)prep; u.sym0 = (int)s0; u.full0 = (int)f0;
-        part += u.nparts; prep += pi * pj; s0 += ti * (ti + 1) / 2; f0 += ti * tj;
-        if (std::max(std::max(part, prep), std::max(s0, f0)) > 0x7fffffffll) return V1T_ERR_UNSUPPORTED;
-        put(i, u);
+        const auto ps = ns_parts((long long)u.rows * u.cols);
+        u.part = ps.first; u.nparts = ps.second; u.part0 = part; u.prep0 = first;
+        part += u.nparts;
+        first += ((u.mp + NS_TILE_PREP - 1) / NS_TILE_PREP) * ((u.np + NS_TILE_PREP - 1) / NS_TILE_PREP);
+        auto tiles = [&](int kind) {
+            const NsPlan& p = kind == 0 ? l.gram : kind == 1 ? l.poly : l.full;
+            const int a = (u.mp + 64 * p.tw - 1) / (64 * p.tw), b = (u.np + 64 * p.tw - 1) / (64 * p.tw);
+            return kind < 2 ? a * (a + 1) / 2 : a * b;
+        };
+        if (k == 0 || size[order[k]] != size[order[k - 1]]) {
+            int same = 1;
+            while (k + same < n && size[order[k + same]] == size[order[k]]) ++same;
+            for (int kind = 0; kind < 3; ++kind) {
+                group0[kind] = next[kind];
+                group[kind] = same * tiles(kind);
+            }
+        }
+        for (int kind = 0; kind < 3; ++kind) {
+            u.first[kind] = next[kind];
+            u.group0[kind] = group0[kind];
+            u.group[kind] = group[kind];
+            next[kind] += tiles(kind);
+        }
+        put(k, order[k], u);
     }
-    l.nparts = (int)part; l.nprep = (int)prep; l.nsym = (int)s0; l.nfull = (int)f0;
+    l.nparts = part; l.nprep = first;
     l.bytes = at;
     return V1T_OK;
 }
@@ -568,25 +708,32 @@ bool ns_exponent(const float* coefficients, int steps, int* exponent) {
     return true;
 }
 
-template <int TW, int KIND, typename T>
-int ns_gemm(const NsLayout& l, const NsUnit* table, int n, char* ws, const NsStep& st, hipStream_t s) {
-    const int grid = KIND == NS_GRAM || KIND == NS_POLY ? l.nsym : l.nfull;
-    hipLaunchKernelGGL((ns_gemm_kernel<TW, KIND, T>), dim3(grid), dim3(256), 0, s, table, n, ws, st);
+template <int KIND, typename T>
+int ns_gemm(const NsLayout& l, const NsUnit* table, int n, char* ws, NsStep st, hipStream_t s) {
+    const NsPlan& p = KIND == NS_GRAM ? l.gram : KIND == NS_POLY ? l.poly : l.full;
+    st.whole = p.whole; st.split = p.split; st.slab = (float*)(ws + l.slab);
+    if (p.tw == 2) hipLaunchKernelGGL((ns_gemm_kernel<2, KIND, T>), dim3(p.grid()), dim3(256), 0, s, table, n, ws, st);
+    else hipLaunchKernelGGL((ns_gemm_kernel<1, KIND, T>), dim3(p.grid()), dim3(256), 0, s, table, n, ws, st);
+    if constexpr (KIND == NS_GRAM || KIND == NS_POLY)
+        if (p.joined()) {
+            if (p.tw == 2) hipLaunchKernelGGL((ns_join_kernel<2, KIND>), dim3(4 * p.joined()), dim3(64), 0, s, table, n, ws, st);
+            else hipLaunchKernelGGL((ns_join_kernel<1, KIND>), dim3(4 * p.joined()), dim3(64), 0, s, table, n, ws, st);
+        }
     return hipGetLastError() == hipSuccess ? V1T_OK : V1T_ERR_LAUNCH;
 }
 
 #define NS_TRY(x) do { const int rc_ = (x); if (rc_ != V1T_OK) return rc_; } while (0)
 
-template <int TW, typename T>
+template <typename T>
 int ns_steps(const NsLayout& l, const NsUnit* table, int n, char* ws, int steps, const float* co, int exponent, hipStream_t s) {
     const float inv = std::ldexp(1.f, -exponent);
     for (int k = 0; k < steps; ++k) {
         const float a = co[3 * k], b = co[3 * k + 1], c = co[3 * k + 2];
-        NS_TRY((ns_gemm<TW, NS_GRAM, float>(l, table, n, ws, NsStep{inv, 0.f, k & 1, inv}, s)));
-        NS_TRY((ns_gemm<TW, NS_POLY, float>(l, table, n, ws, NsStep{c * inv, b, k & 1, inv}, s)));
+        NS_TRY((ns_gemm<NS_GRAM, float>(l, table, n, ws, NsStep{inv, 0.f, k & 1, inv}, s)));
+        NS_TRY((ns_gemm<NS_POLY, float>(l, table, n, ws, NsStep{c * inv, b, k & 1, inv}, s)));
         const NsStep last{inv, a, k & 1, inv};
-        if (k + 1 < steps) NS_TRY((ns_gemm<TW, NS_APPLY, float>(l, table, n, ws, last, s)));
-        else NS_TRY((ns_gemm<TW, NS_LAST, T>(l, table, n, ws, last, s)));
+        if (k + 1 < steps) NS_TRY((ns_gemm<NS_APPLY, float>(l, table, n, ws, last, s)));
+        else NS_TRY((ns_gemm<NS_LAST, T>(l, table, n, ws, last, s)));
     }
     return V1T_OK;
 }
@@ -602,21 +749,21 @@ int ns_run(const NsLayout& l, int n, char* ws, const NsMomentum& mo, float eps, 
         hipLaunchKernelGGL((ns_copy_kernel<T>), dim3(l.nprep), dim3(256), 0, s, table, n, ws, std::ldexp(1.f, -exponent));
         return hipGetLastError() == hipSuccess ? V1T_OK : V1T_ERR_LAUNCH;
     }
-    return l.tile == 128 ? ns_steps<2, T>(l, table, n, ws, steps, co, exponent, s) : ns_steps<1, T>(l, table, n, ws, steps, co, exponent, s);
+    return ns_steps<T>(l, table, n, ws, steps, co, exponent, s);
 }
 
 // lays out the units, checks the workspace, writes the table
 template <typename Shape, typename Fill>
-int ns_begin(int n, Shape shape, Fill fill, void* workspace, long long ws_bytes, NsLayout& l, hipStream_t s) {
-    NS_TRY(ns_layout(n, shape, [](int, NsUnit&) {}, l));
+int ns_begin(int n, Shape shape, Fill fill, void* workspace, long long ws_bytes, NsLayout& l, hipStream_t s) try {
+    NS_TRY(ns_layout(n, shape, [](int, int, NsUnit&) {}, l));
     if (!workspace || ws_bytes < l.bytes) return V1T_ERR_WORKSPACE;
     if ((uintptr_t)workspace & 15) return V1T_ERR_ARG;
     NsChunk c;
     NsUnit* table = (NsUnit*)((char*)workspace + l.table);
     int rc = V1T_OK;
     NsLayout again;
-    ns_layout(n, shape, [&](int i, NsUnit& u) {
-        fill(i, u);
+    ns_layout(n, shape, [&](int i, int from, NsUnit& u) {
+        fill(from, u);
         c.u[i % NS_CHUNK] = u;
         if (i % NS_CHUNK == NS_CHUNK - 1 || i == n - 1) {
             const int k = i % NS_CHUNK + 1;
@@ -625,15 +772,21 @@ int ns_begin(int n, Shape shape, Fill fill, void* workspace, long long ws_bytes,
         }
     }, again);
     return rc;
+} catch (...) {
+    return V1T_ERR_WORKSPACE;
 }
 
 }  // namespace
 
 extern "C" long long v1t_orthogonalize_ws_bytes(const int* rows, const int* cols, int n) {
     if (n < 0 || (n > 0 && (!rows || !cols))) return V1T_ERR_ARG;
-    NsLayout l;
-    const int rc = ns_layout(n, [&](int i, int& r, int& c) { r = rows[i]; c = cols[i]; }, [](int, NsUnit&) {}, l);
-    return rc == V1T_OK ? l.bytes : rc;
+    try {  // (the layout's own tables: nothing leaves a C entry but a code)
+        NsLayout l;
+        const int rc = ns_layout(n, [&](int i, int& r, int& c) { r = rows[i]; c = cols[i]; }, [](int, int, NsUnit&) {}, l);
+        return rc == V1T_OK ? l.bytes : rc;
+    } catch (...) {
+        return V1T_ERR_WORKSPACE;
+    }
 }
 
 extern "C" int v1t_orthogonalize(const v1t_matrix* units, int n, int dtype, int steps, const float* coefficients, float eps, void* workspace, long long ws_bytes,
