@@ -2,7 +2,10 @@
 //
 //     X <- U / (|U|_F + eps), laid with its shorter side m first (m x n)
 //     A = X X^T,  S = b A + c A A,  X <- a X + S X          a few times, with (a, b, c) of each step
-// The polynomial a s + b s^3 + c s^5 acts on every singular value s of X and drives it towards 1.
+// The polynomial a s + b s^3 + c s^5 acts on every singular value s of X and drives it towards 1. Where X is long, two steps go over it at once, on m x m matrices
+// alone: with S of the first, T = a A + S A, A' = a T + S T is the next step's X X^T, S' its polynomial, and X <- Q X with
+// Q = (a' + S') (a + S) = a a' + (a' S + a S' + S' S). Every m x m product is symmetric: half its tiles are computed.
+// The first pair applies a a' X + (...) X, which keeps small singular values exact; later ones, whose Q is near 1, all of Q: a a' = 12 would cancel.
 //
 // Precision: fp32, on fp16 matrix instructions. A number v of X, A or S (spectral norm known to the host to stay below 2^15 / 2^e for the given
 // coefficients) is kept as two fp16 planes of v 2^e: hi = fp16(v 2^e) and lo = fp16(v 2^e - hi), 22 bits of it, and a product of two such numbers is
@@ -36,7 +39,7 @@ struct NsUnit {
     void* out;        // the result, or nullptr: w is updated
     float *mom, *w;
     long long rs, cs;                // element strides of `in`; out, mom and w are row-major without gaps
-    long long x[2], a, s;            // byte offsets of the planes in the workspace (hi, and lo behind it)
+    long long x[2], sq[4];           // byte offsets of the planes in the workspace (hi, and lo behind it): X twice, the m x m matrices
     int rows, cols, m, n, mp, np, trans;
     int part, part0, nparts, prep0;  // elements per partial sum; first workgroup of this unit in the launches of each kind
     int first[3];                    // first tile in the products' launches: gram, poly, apply / last
@@ -216,16 +219,17 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(const NsUnit* units, int n
 // ---- the products -------------------------------------------------------------------------
 // C[i][j] = sum_k P[i][k] Q[j][k]: a workgroup of 4 waves computes a 64 TW x 64 TW tile, wave (wi, wj) a quarter of it, in K steps of 32. The tile's rows of P
 // and Q go to LDS by LDS-DMA into a ring of NST stages. In the accumulators i is on the lanes and j in the registers, four in a row.
-enum NsKind { NS_GRAM = 0, NS_POLY = 1, NS_APPLY = 2, NS_LAST = 3 };
+enum NsKind { NS_GRAM = 0, NS_SQUARE = 1, NS_APPLY = 2, NS_LAST = 3 };  // A = X X^T; sq[out] = sq[p] sq[q] + ..; X = sq[p] X + ..; the same, the result
 struct NsStep {
-    float alpha, beta;   // C <- alpha (P Q^T) + beta D, on the scaled planes
+    float alpha, beta, beta2, diagonal;  // C <- alpha (P Q^T) + beta D + beta2 D2 + diagonal 1, on the scaled planes
+    int p, q, d, d2, out;                // which m x m matrices
     int from;            // which of the two X planes is read
     float inv;           // 2^-e
     int whole, split;    // tiles [0, whole) are computed by a workgroup each, the others in `split` pieces of their K steps
     float* slab;         // the pieces' sums
 };
 
-constexpr int ns_launch(int kind) { return kind == NS_GRAM ? 0 : kind == NS_POLY ? 1 : 2; }
+constexpr int ns_launch(int kind) { return kind == NS_GRAM ? 0 : kind == NS_SQUARE ? 1 : 2; }
 
 // The tile of a run that its workgroup number `local` computes: workgroups b, b + 8, .. share an XCD and its L2, and get neighbouring tiles. A run is all units of
 // one size: over a whole launch one XCD would get the units with the longest K, over one unit an XCD would read a part of every unit
@@ -249,13 +253,13 @@ struct NsTile {
 // where a tile lies and what it reads and writes
 struct NsWhere {
     int bi, bj, i0, j0;
-    const f16_t *D, *Dl;
+    const f16_t *D, *Dl, *D2, *D2l;
     f16_t *C, *Cl;
     int ldd, cols;
 };
 template <int TW, int KIND>
 DEVFN NsWhere ns_where(const NsUnit& u, char* ws, const NsStep& st, int t) {  // t: the unit's tile
-    constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY;
+    constexpr bool SYM = KIND == NS_GRAM || KIND == NS_SQUARE;
     constexpr int B = NsTile<TW>::B;
     NsWhere w;
     if constexpr (SYM) {  // tile number -> (bi <= bj) of the upper triangle, columns of tiles one after another
@@ -271,10 +275,12 @@ DEVFN NsWhere ns_where(const NsUnit& u, char* ws, const NsStep& st, int t) {  //
     w.i0 = w.bi * B;
     w.j0 = w.bj * B;
     const size_t xlo = (size_t)u.mp * u.np, alo = (size_t)u.mp * u.mp;
-    w.D = KIND == NS_POLY ? (const f16_t*)(ws + u.a) : (const f16_t*)(ws + u.x[st.from]);
-    w.Dl = w.D + (KIND == NS_POLY ? alo : xlo);
-    w.ldd = KIND == NS_POLY ? u.mp : u.np;
-    w.C = (f16_t*)(ws + (KIND == NS_GRAM ? u.a : KIND == NS_POLY ? u.s : u.x[st.from ^ 1]));
+    w.D = KIND == NS_SQUARE ? (const f16_t*)(ws + u.sq[st.d]) : (const f16_t*)(ws + u.x[st.from]);
+    w.Dl = w.D + (KIND == NS_SQUARE ? alo : xlo);
+    w.D2 = (const f16_t*)(ws + u.sq[st.d2]);
+    w.D2l = w.D2 + alo;
+    w.ldd = KIND == NS_SQUARE ? u.mp : u.np;
+    w.C = (f16_t*)(ws + (KIND == NS_GRAM ? u.sq[0] : KIND == NS_SQUARE ? u.sq[st.out] : u.x[st.from ^ 1]));
     w.Cl = w.C + (SYM ? alo : xlo);
     w.cols = SYM ? u.mp : u.np;
     return w;
@@ -285,7 +291,7 @@ DEVFN NsWhere ns_where(const NsUnit& u, char* ws, const NsStep& st, int t) {  //
 // LDS image [SIDE][SIDE] fp32, 16-B chunks of a row swizzled by the row: writes by lanes of one column and reads along rows both spread over the banks.
 template <int TW, int KIND, typename T>
 DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x16 (&acc)[TW][TW], float* img, int wi, int wj, int lane) {
-    constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY;
+    constexpr bool SYM = KIND == NS_GRAM || KIND == NS_SQUARE;
     constexpr int SIDE = 32 * TW;
     auto chunk = [&](int i, int c) { return i * SIDE + 4 * (TW == 2 ? c ^ (i & 15) : c ^ (i >> 1 & 7)); };
     const int r = lane & 31, h = lane >> 5;
@@ -314,6 +320,21 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
                 v1[e] += st.beta * ((float)dh[4 + e] + (float)dl[4 + e]);
             }
         }
+        if constexpr (KIND == NS_SQUARE) {
+            if (st.beta2 != 0.f) {
+                const f16x8 dh = *(const f16x8*)(w.D2 + (size_t)i * w.ldd + j), dl = *(const f16x8*)(w.D2l + (size_t)i * w.ldd + j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v0[e] += st.beta2 * ((float)dh[e] + (float)dl[e]);
+                    v1[e] += st.beta2 * ((float)dh[4 + e] + (float)dl[4 + e]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (i == j + e && i < u.m) v0[e] += st.diagonal;
+                if (i == j + 4 + e && i < u.m) v1[e] += st.diagonal;
+            }
+        }
         if constexpr (KIND != NS_LAST) {
             f16x8 ch, cl;
 #pragma unroll
@@ -326,7 +347,7 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
             *(f16x8*)(w.C + (size_t)i * w.cols + j) = ch;
             *(f16x8*)(w.Cl + (size_t)i * w.cols + j) = cl;
         }
-        if (KIND == NS_LAST || (KIND == NS_POLY && mirror)) {
+        if (KIND == NS_LAST || (KIND == NS_SQUARE && mirror)) {
             *(f32x4*)(img + chunk(il, jl / 4)) = v0;
             *(f32x4*)(img + chunk(il, jl / 4 + 1)) = v1;
         }
@@ -380,7 +401,7 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
 
 template <int TW, int KIND, typename T>
 __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(const NsUnit* units, int n, char* ws, NsStep st) {
-    constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY, TR = !SYM;  // TR: Q is stored [k][j]
+    constexpr bool SYM = KIND == NS_GRAM || KIND == NS_SQUARE, TR = !SYM;  // TR: Q is stored [k][j]
     using Tile = NsTile<TW>;
     constexpr int B = Tile::B, PL = Tile::PL, PIECES = Tile::PIECES, NST = Tile::NST;
     __shared__ __attribute__((aligned(16))) f16_t lds[Tile::LDS];
@@ -400,12 +421,11 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(const NsU
     const int steps = (KIND == NS_GRAM ? u.np : u.mp) / NS_BK, each = piece ? (steps + st.split - 1) / st.split : steps;
     const int t0 = piece ? over % st.split * each : 0, nk = max(0, min(each, steps - t0));  // this workgroup's K steps
     const f16_t* X = (const f16_t*)(ws + u.x[st.from]);
-    const f16_t* A = (const f16_t*)(ws + u.a);
-    const f16_t* P = KIND == NS_GRAM ? X : KIND == NS_POLY ? A : (const f16_t*)(ws + u.s);
-    const f16_t* Q = KIND == NS_POLY ? A : X;
+    const f16_t* P = KIND == NS_GRAM ? X : (const f16_t*)(ws + u.sq[st.p]);
+    const f16_t* Q = KIND == NS_SQUARE ? (const f16_t*)(ws + u.sq[st.q]) : X;
     const size_t xlo = (size_t)u.mp * u.np, alo = (size_t)u.mp * u.mp;
-    const int ldp = KIND == NS_GRAM ? u.np : u.mp, ldq = KIND == NS_POLY ? u.mp : u.np;
-    const size_t plo = KIND == NS_GRAM ? xlo : alo, qlo = KIND == NS_POLY ? alo : xlo;
+    const int ldp = KIND == NS_GRAM ? u.np : u.mp, ldq = KIND == NS_SQUARE ? u.mp : u.np;
+    const size_t plo = KIND == NS_GRAM ? xlo : alo, qlo = KIND == NS_SQUARE ? alo : xlo;
 
     // A 1-KB piece fills 64 16-B chunks of a plane in order; which 16 B of the tile's row a chunk holds is swizzled, so that the fragment reads below spread over
     // all banks. Rows [.][32]: four chunks a row, chunk c at c ^ (row / 4 % 4). Q as [k][j], B / 8 chunks a row: c ^ 4 (k % 4) - B = 64, where two rows fill
@@ -567,6 +587,7 @@ __global__ __launch_bounds__(256) void ns_copy_kernel(const NsUnit* units, int n
 // A product's launch: tiles of 64 tw, the first `whole` computed whole, the others in `split` pieces
 struct NsPlan {
     int tw = 1, tiles = 0, whole = 0, split = 1;
+    double us = 0.0;
     int grid() const { return whole + (tiles - whole) * split; }
     int joined() const { return tiles - whole; }
     long long slab() const { return split > 1 ? (long long)(tiles - whole) * split * 16384ll * tw * tw : 0; }
@@ -574,6 +595,7 @@ struct NsPlan {
 struct NsLayout {
     long long table = 0, parts = 0, slab = 0, bytes = 0;
     int nparts = 0, nprep = 0;
+    bool pairs = false;  // two steps at once
     NsPlan gram, poly, full;
 };
 // elements per partial sum, and how many sums
@@ -604,7 +626,7 @@ NsPlan ns_plan(long long t64, long long k64, long long t128, long long k128, boo
             if (split > 1) t += round(steps / split, pieces) + 6.0 + (double)pieces * tw * tw * 16384.0 * 2.0 / 3e6;
             if (t < least) {
                 least = t;
-                best.tw = tw; best.tiles = (int)tiles; best.whole = (int)whole; best.split = split;
+                best.us = t; best.tw = tw; best.tiles = (int)tiles; best.whole = (int)whole; best.split = split;
             }
         }
     }
@@ -642,6 +664,8 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
     l.gram = ns_plan(gt[0], gk[0], gt[1], gk[1], true);
     l.poly = ns_plan(gt[0], pk[0], gt[1], pk[1], true);
     l.full = ns_plan(ft[0], fk[0], ft[1], fk[1], false);
+    // two steps: gram, poly, full each twice, or gram, five m x m products, full; 3 us a launch
+    l.pairs = l.gram.us + 5 * l.poly.us + l.full.us + 21.0 < 0.9 * (2 * (l.gram.us + l.poly.us + l.full.us) + 18.0);
     l.table = 0;
     l.parts = ns_align((long long)n * (long long)sizeof(NsUnit));
     l.slab = ns_align(l.parts + 8 * nparts);
@@ -654,8 +678,9 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
         u.m = std::min(u.rows, u.cols); u.n = std::max(u.rows, u.cols);
         u.mp = round_up(u.m, NS_BK); u.np = round_up(u.n, NS_BK);
         const long long xb = ns_align(4ll * u.mp * u.np), ab = ns_align(4ll * u.mp * u.mp);
-        u.x[0] = at; u.x[1] = at + xb; u.a = at + 2 * xb; u.s = u.a + ab;
-        at = u.s + ab;
+        u.x[0] = at; u.x[1] = at + xb;
+        at += 2 * xb;
+        for (int q = 0; q < (l.pairs ? 4 : 2); ++q, at += ab) u.sq[q] = at;
         const auto ps = ns_parts((long long)u.rows * u.cols);
         u.part = ps.first; u.nparts = ps.second; u.part0 = part; u.prep0 = first;
         part += u.nparts;
@@ -687,19 +712,29 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
 }
 
 // The exponent of the planes' common scale: 2^15 over the largest number of any plane. A step maps a singular value s in [0, top] to a s + b s^3 + c s^5;
-// X, A = X X^T and S are bounded by their spectral norms. The maxima are sampled, 0.1 % is added for what lies between the samples and for rounding.
-bool ns_exponent(const float* coefficients, int steps, int* exponent) {
+// X, A = X X^T, S and, where steps are taken in pairs, T, the next A, S' and Q are bounded by their spectral norms. The maxima are sampled, 0.1 % of a
+// singular value and 1 % of the rest are added for what lies between the samples and for rounding.
+bool ns_exponent(const float* coefficients, int steps, bool pairs, int* exponent) {
     double top = 1.001, most = top;
     for (int k = 0; k < steps; ++k) {
-        const double a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
-        if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
+        const float* f = coefficients + 3 * k;
+        for (int e = 0; e < 3; ++e)
+            if (!std::isfinite(f[e])) return false;
+        const bool pair = pairs && k + 1 < steps;
         double next = 0.0;
-        most = std::max(most, top * top);
         for (int i = 0; i <= 4096; ++i) {
-            const double s = top * i / 4096.0, t = s * s;
-            next = std::max(next, std::fabs(s * (a + t * (b + t * c))));
-            most = std::max(most, std::fabs(t * (b + t * c)));
+            const double s = top * i / 4096.0, t = s * s, poly = t * (f[1] + t * f[2]);
+            double end = s * (f[0] + poly);
+            most = std::max({most, t, std::fabs(poly)});
+            if (pair) {
+                const double a1 = f[3], t1 = end * end, poly1 = t1 * (f[4] + t1 * f[5]);
+                most = std::max({most, std::fabs(t * (f[0] + poly)), t1, std::fabs(poly1), std::fabs((a1 + poly1) * (f[0] + poly)),
+                                 std::fabs((a1 + poly1) * (f[0] + poly) - a1 * f[0])});
+                end *= a1 + poly1;
+            }
+            next = std::max(next, std::fabs(end));
         }
+        if (pair) ++k;
         top = 1.001 * next;
         most = std::max(most, top);
         if (!(most < 128.0)) return false;
@@ -710,11 +745,11 @@ bool ns_exponent(const float* coefficients, int steps, int* exponent) {
 
 template <int KIND, typename T>
 int ns_gemm(const NsLayout& l, const NsUnit* table, int n, char* ws, NsStep st, hipStream_t s) {
-    const NsPlan& p = KIND == NS_GRAM ? l.gram : KIND == NS_POLY ? l.poly : l.full;
+    const NsPlan& p = KIND == NS_GRAM ? l.gram : KIND == NS_SQUARE ? l.poly : l.full;
     st.whole = p.whole; st.split = p.split; st.slab = (float*)(ws + l.slab);
     if (p.tw == 2) hipLaunchKernelGGL((ns_gemm_kernel<2, KIND, T>), dim3(p.grid()), dim3(256), 0, s, table, n, ws, st);
     else hipLaunchKernelGGL((ns_gemm_kernel<1, KIND, T>), dim3(p.grid()), dim3(256), 0, s, table, n, ws, st);
-    if constexpr (KIND == NS_GRAM || KIND == NS_POLY)
+    if constexpr (KIND == NS_GRAM || KIND == NS_SQUARE)
         if (p.joined()) {
             if (p.tw == 2) hipLaunchKernelGGL((ns_join_kernel<2, KIND>), dim3(4 * p.joined()), dim3(64), 0, s, table, n, ws, st);
             else hipLaunchKernelGGL((ns_join_kernel<1, KIND>), dim3(4 * p.joined()), dim3(64), 0, s, table, n, ws, st);
@@ -724,22 +759,45 @@ int ns_gemm(const NsLayout& l, const NsUnit* table, int n, char* ws, NsStep st, 
 
 #define NS_TRY(x) do { const int rc_ = (x); if (rc_ != V1T_OK) return rc_; } while (0)
 
+NsStep ns_square(int out, int p, int q, float alpha, int d, float beta, int d2 = 0, float beta2 = 0.f, float diagonal = 0.f) {
+    NsStep st{};
+    st.alpha = alpha; st.p = p; st.q = q; st.d = d; st.beta = beta; st.d2 = d2; st.beta2 = beta2; st.diagonal = diagonal; st.out = out;
+    return st;
+}
+
 template <typename T>
-int ns_steps(const NsLayout& l, const NsUnit* table, int n, char* ws, int steps, const float* co, int exponent, hipStream_t s) {
+int ns_steps(const NsLayout& l, const NsUnit* table, int n, char* ws, int steps, const float* co, bool pairs, int exponent, hipStream_t s) {
+    enum { A = 0, S = 1, U = 2, S1 = 3 };  // the m x m matrices; U holds T, then Q
     const float inv = std::ldexp(1.f, -exponent);
+    int from = 0;
     for (int k = 0; k < steps; ++k) {
         const float a = co[3 * k], b = co[3 * k + 1], c = co[3 * k + 2];
-        NS_TRY((ns_gemm<NS_GRAM, float>(l, table, n, ws, NsStep{inv, 0.f, k & 1, inv}, s)));
-        NS_TRY((ns_gemm<NS_POLY, float>(l, table, n, ws, NsStep{c * inv, b, k & 1, inv}, s)));
-        const NsStep last{inv, a, k & 1, inv};
-        if (k + 1 < steps) NS_TRY((ns_gemm<NS_APPLY, float>(l, table, n, ws, last, s)));
-        else NS_TRY((ns_gemm<NS_LAST, T>(l, table, n, ws, last, s)));
+        NsStep st{};
+        st.alpha = inv; st.from = from; st.inv = inv;
+        NS_TRY((ns_gemm<NS_GRAM, float>(l, table, n, ws, st, s)));
+        NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, n, ws, ns_square(S, A, A, c * inv, A, b), s)));
+        st.p = S; st.beta = a;
+        if (pairs && k + 1 < steps) {
+            const float a1 = co[3 * k + 3], b1 = co[3 * k + 4], c1 = co[3 * k + 5];
+            NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, n, ws, ns_square(U, S, A, inv, A, a), s)));
+            NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, n, ws, ns_square(A, S, U, inv, U, a), s)));
+            NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, n, ws, ns_square(S1, A, A, c1 * inv, A, b1), s)));
+            NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, n, ws, ns_square(U, S1, S, inv, S, a1, S1, a, k == 0 ? 0.f : std::ldexp(a * a1, exponent)), s)));
+            st.p = U; st.beta = k == 0 ? a * a1 : 0.f;
+            ++k;
+        }
+        if (k + 1 < steps) NS_TRY((ns_gemm<NS_APPLY, float>(l, table, n, ws, st, s)));
+        else NS_TRY((ns_gemm<NS_LAST, T>(l, table, n, ws, st, s)));
+        from ^= 1;
     }
     return V1T_OK;
 }
 
 template <typename T, bool MOM>
-int ns_run(const NsLayout& l, int n, char* ws, const NsMomentum& mo, float eps, int zero, int steps, const float* co, int exponent, hipStream_t s) {
+int ns_run(const NsLayout& l, int n, char* ws, const NsMomentum& mo, float eps, int zero, int steps, const float* co, hipStream_t s) {
+    int exponent = 0;
+    const bool pairs = l.pairs && ns_exponent(co, steps, true, &exponent);  // coefficients whose pairs would leave the planes' range go step by step
+    if (!pairs && !ns_exponent(co, steps, false, &exponent)) return V1T_ERR_ARG;
     const NsUnit* table = (const NsUnit*)(ws + l.table);
     double* parts = (double*)(ws + l.parts);
     hipLaunchKernelGGL((ns_norm_kernel<T, MOM>), dim3(l.nparts), dim3(256), 0, s, table, n, mo, parts);
@@ -749,7 +807,7 @@ int ns_run(const NsLayout& l, int n, char* ws, const NsMomentum& mo, float eps, 
         hipLaunchKernelGGL((ns_copy_kernel<T>), dim3(l.nprep), dim3(256), 0, s, table, n, ws, std::ldexp(1.f, -exponent));
         return hipGetLastError() == hipSuccess ? V1T_OK : V1T_ERR_LAUNCH;
     }
-    return ns_steps<T>(l, table, n, ws, steps, co, exponent, s);
+    return ns_steps<T>(l, table, n, ws, steps, co, pairs, exponent, s);
 }
 
 // lays out the units, checks the workspace, writes the table
@@ -793,7 +851,7 @@ extern "C" int v1t_orthogonalize(const v1t_matrix* units, int n, int dtype, int 
                                  void* stream) {
     if (n < 0 || (n > 0 && !units) || dtype < 0 || dtype > 2 || steps < 0 || steps > NS_MAX_STEPS || (steps > 0 && !coefficients) || !(eps >= 0.f)) return V1T_ERR_ARG;
     int exponent = 0;
-    if (!ns_exponent(coefficients, steps, &exponent)) return V1T_ERR_ARG;
+    if (!ns_exponent(coefficients, steps, false, &exponent)) return V1T_ERR_ARG;
     for (int i = 0; i < n; ++i)
         if (!units[i].in || !units[i].out) return V1T_ERR_ARG;
     if (n == 0) return V1T_OK;
@@ -804,16 +862,16 @@ extern "C" int v1t_orthogonalize(const v1t_matrix* units, int n, int dtype, int 
                     workspace, ws_bytes, l, s));
     const NsMomentum mo{0.f, 0};
     char* ws = (char*)workspace;
-    if (dtype == 0) return ns_run<bf16_t, false>(l, n, ws, mo, eps, 0, steps, coefficients, exponent, s);
-    if (dtype == 1) return ns_run<f16_t, false>(l, n, ws, mo, eps, 0, steps, coefficients, exponent, s);
-    return ns_run<float, false>(l, n, ws, mo, eps, 0, steps, coefficients, exponent, s);
+    if (dtype == 0) return ns_run<bf16_t, false>(l, n, ws, mo, eps, 0, steps, coefficients, s);
+    if (dtype == 1) return ns_run<f16_t, false>(l, n, ws, mo, eps, 0, steps, coefficients, s);
+    return ns_run<float, false>(l, n, ws, mo, eps, 0, steps, coefficients, s);
 }
 
 extern "C" int v1t_muon_step(const v1t_muon_range* units, int n, float momentum, int nesterov, int steps, const float* coefficients, float eps, int zero_grad,
                              void* workspace, long long ws_bytes, void* stream) {
     if (n < 0 || (n > 0 && !units) || steps < 0 || steps > NS_MAX_STEPS || (steps > 0 && !coefficients) || !(eps >= 0.f) || !std::isfinite(momentum)) return V1T_ERR_ARG;
     int exponent = 0;
-    if (!ns_exponent(coefficients, steps, &exponent)) return V1T_ERR_ARG;
+    if (!ns_exponent(coefficients, steps, false, &exponent)) return V1T_ERR_ARG;
     for (int i = 0; i < n; ++i)
         if (!units[i].p || !units[i].g || !units[i].m) return V1T_ERR_ARG;
     if (n == 0) return V1T_OK;
@@ -825,5 +883,5 @@ extern "C" int v1t_muon_step(const v1t_muon_range* units, int n, float momentum,
                         u.lr = units[i].lr; u.decay = units[i].decay; u.l1 = units[i].l1;
                     },
                     workspace, ws_bytes, l, s));
-    return ns_run<float, true>(l, n, (char*)workspace, NsMomentum{momentum, nesterov}, eps, zero_grad, steps, coefficients, exponent, s);
+    return ns_run<float, true>(l, n, (char*)workspace, NsMomentum{momentum, nesterov}, eps, zero_grad, steps, coefficients, s);
 }
