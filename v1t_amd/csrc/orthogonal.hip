@@ -51,29 +51,48 @@ struct NsChunk {
     NsUnit u[NS_CHUNK];
 };
 
-__global__ void ns_table_kernel(NsChunk c, int n, NsUnit* to) {
+// What a workgroup finds its unit by: per launch (0 .. 2 the products', 3 the partial sums', 4 the first planes') and unit its first workgroup, and the run of units of
+// its size. Apart from the units, so that a wave reads 64 of them at once from few lines
+typedef int ns_head __attribute__((ext_vector_type(4)));  // first, the run's first, the run's tiles, -
+
+struct NsTable {
+    const NsUnit* units;
+    const ns_head* heads;  // [5][n]
+    int n;
+};
+
+__global__ void ns_table_kernel(NsChunk c, int n, int at, int all, NsUnit* units, ns_head* heads) {
     // 4-byte words, one per lane: the argument is read as an array
     const uint32_t* src = (const uint32_t*)&c;
-    for (int i = threadIdx.x; i < n * (int)(sizeof(NsUnit) / 4); i += blockDim.x) ((uint32_t*)to)[i] = src[i];
+    for (int i = threadIdx.x; i < n * (int)(sizeof(NsUnit) / 4); i += blockDim.x) ((uint32_t*)(units + at))[i] = src[i];
+    for (int i = threadIdx.x; i < 5 * n; i += blockDim.x) {
+        const int k = i / n, e = i % n;
+        const NsUnit& u = c.u[e];
+        heads[(size_t)k * all + at + e] = k < 3 ? ns_head{u.first[k], u.group0[k], u.group[k], 0} : ns_head{k == 3 ? u.part0 : u.prep0, 0, 0, 0};
+    }
 }
 
-// the unit whose range of workgroups `block` falls into: the last one that begins at or before it. 64 units' beginnings are read at once - a search would wait
-// for one read after another. W: the launch - 0 .. 2 the products', 3 the partial sums', 4 the first planes'
+// the unit whose range of workgroups `block` falls into - the last one that begins at or before it - and its head
 template <int W>
-DEVFN int ns_find(const NsUnit* u, int n, int block) {
+DEVFN int ns_find(const NsTable& t, int block, ns_head& head) {
     const int lane = threadIdx.x & 63;
-    int found = -1;
-    for (int i = 0; i < n; i += 64) {
-        bool before = false;
-        if (i + lane < n) {
-            const NsUnit& x = u[i + lane];
-            before = (W < 3 ? x.first[W < 3 ? W : 0] : W == 3 ? x.part0 : x.prep0) <= block;
-        }
-        const int k = __popcll(__ballot(before));
+    const ns_head* h = t.heads + (size_t)W * t.n;
+    int found = -1, i = 0;
+    ns_head mine{};
+    for (;; i += 64) {
+        mine = i + lane < t.n ? h[i + lane] : ns_head{0x7fffffff, 0, 0, 0};
+        const int k = __popcll(__ballot(mine[0] <= block));
         found += k;
-        if (k < 64) break;
+        if (k < 64 || i + 64 >= t.n) break;
     }
-    return __builtin_amdgcn_readfirstlane(found);
+    found = __builtin_amdgcn_readfirstlane(found);
+    if (found < i) {  // the last one of the 64 before
+        head = h[found];
+        return found;
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e) head[e] = __builtin_amdgcn_readlane(mine[e], found - i);
+    return found;
 }
 
 struct NsMomentum {
@@ -120,9 +139,10 @@ struct NsBatch {
 
 // partial sums of squares, in 64 bits (their range is that of the inputs squared); MOM: momentum <- mu momentum + gradient on the way
 template <typename T, bool MOM>
-__global__ __launch_bounds__(256) void ns_norm_kernel(const NsUnit* units, int n, NsMomentum mo, double* parts) {
+__global__ __launch_bounds__(256) void ns_norm_kernel(NsTable tab, NsMomentum mo, double* parts) {
     constexpr int N = 8;
-    const NsUnit& u = units[ns_find<3>(units, n, blockIdx.x)];
+    ns_head head;
+    const NsUnit& u = tab.units[ns_find<3>(tab, blockIdx.x, head)];
     const long long all = (long long)u.rows * u.cols, i0 = (long long)(blockIdx.x - u.part0) * u.part;
     const int len = (int)min((long long)u.part, all - i0);
     const bool flat = u.cs == 1 && u.rs == u.cols;
@@ -164,8 +184,9 @@ DEVFN void ns_split(float v, f16_t& hi, f16_t& lo) {
 // the first planes: 64 x 64 tiles of X, read along the update's rows and turned through LDS where X is its transpose. MOM && zero: the gradient is
 // cleared behind its last reader
 template <typename T, bool MOM>
-__global__ __launch_bounds__(256) void ns_prep_kernel(const NsUnit* units, int n, NsMomentum mo, const double* parts, char* ws, float eps, float scale, int zero) {
-    const NsUnit& u = units[ns_find<4>(units, n, blockIdx.x)];
+__global__ __launch_bounds__(256) void ns_prep_kernel(NsTable tab, NsMomentum mo, const double* parts, char* ws, float eps, float scale, int zero) {
+    ns_head head;
+    const NsUnit& u = tab.units[ns_find<4>(tab, blockIdx.x, head)];
     __shared__ float s[NS_TILE_PREP][NS_TILE_PREP + 1];
     double sum = 0.0;
     for (int i = threadIdx.x; i < u.nparts; i += 256) sum += parts[u.part0 + i];
@@ -400,7 +421,7 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
 }
 
 template <int TW, int KIND, typename T>
-__global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(const NsUnit* units, int n, char* ws, NsStep st) {
+__global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(NsTable tab, char* ws, NsStep st) {
     constexpr bool SYM = KIND == NS_GRAM || KIND == NS_SQUARE, TR = !SYM;  // TR: Q is stored [k][j]
     using Tile = NsTile<TW>;
     constexpr int B = Tile::B, PL = Tile::PL, PIECES = Tile::PIECES, NST = Tile::NST;
@@ -409,15 +430,15 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(const NsU
     constexpr int W = ns_launch(KIND);
     const int b = blockIdx.x, over = b - st.whole;
     const bool piece = SYM && over >= 0;  // workgroup-uniform
-    int number = b;
-    if (piece) {
-        number = st.whole + over / st.split;
-    } else {
-        const NsUnit& g = units[ns_find<W>(units, n, b)];
-        number = g.group0[W] + ns_deal(b - g.group0[W], g.group0[W], SYM ? min(g.group[W], st.whole - g.group0[W]) : g.group[W]);
+    ns_head head;
+    int number = piece ? st.whole + over / st.split : b;
+    int unit = ns_find<W>(tab, number, head);
+    if (!piece) {
+        number = head[1] + ns_deal(b - head[1], head[1], SYM ? min(head[2], st.whole - head[1]) : head[2]);
+        unit = ns_find<W>(tab, number, head);
     }
-    const NsUnit& u = units[ns_find<W>(units, n, number)];
-    const NsWhere w = ns_where<TW, KIND>(u, ws, st, number - u.first[W]);
+    const NsUnit& u = tab.units[unit];
+    const NsWhere w = ns_where<TW, KIND>(u, ws, st, number - head[0]);
     const int steps = (KIND == NS_GRAM ? u.np : u.mp) / NS_BK, each = piece ? (steps + st.split - 1) / st.split : steps;
     const int t0 = piece ? over % st.split * each : 0, nk = max(0, min(each, steps - t0));  // this workgroup's K steps
     const f16_t* X = (const f16_t*)(ws + u.x[st.from]);
@@ -536,12 +557,13 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(const NsU
 
 // The pieces of the split tiles, added up in their order, and the epilogue: one wave per quarter of a tile
 template <int TW, int KIND>
-__global__ __launch_bounds__(64) void ns_join_kernel(const NsUnit* units, int n, char* ws, NsStep st) {
+__global__ __launch_bounds__(64) void ns_join_kernel(NsTable tab, char* ws, NsStep st) {
     constexpr int W = ns_launch(KIND);
     __shared__ __attribute__((aligned(16))) float lds[32 * TW * 32 * TW];
     const int lane = threadIdx.x, wave = blockIdx.x & 3, tile = blockIdx.x >> 2;
-    const NsUnit& u = units[ns_find<W>(units, n, st.whole + tile)];
-    const NsWhere w = ns_where<TW, KIND>(u, ws, st, st.whole + tile - u.first[W]);
+    ns_head head;
+    const NsUnit& u = tab.units[ns_find<W>(tab, st.whole + tile, head)];
+    const NsWhere w = ns_where<TW, KIND>(u, ws, st, st.whole + tile - head[0]);
     f32x16 acc[TW][TW];
 #pragma unroll
     for (int i = 0; i < TW; ++i)
@@ -567,8 +589,9 @@ __global__ __launch_bounds__(64) void ns_join_kernel(const NsUnit* units, int n,
 
 // no steps: the normalised update itself
 template <typename T>
-__global__ __launch_bounds__(256) void ns_copy_kernel(const NsUnit* units, int n, const char* ws, float inv) {
-    const NsUnit& u = units[ns_find<4>(units, n, blockIdx.x)];
+__global__ __launch_bounds__(256) void ns_copy_kernel(NsTable tab, const char* ws, float inv) {
+    ns_head head;
+    const NsUnit& u = tab.units[ns_find<4>(tab, blockIdx.x, head)];
     const int tj = (u.np + NS_TILE_PREP - 1) / NS_TILE_PREP, t = blockIdx.x - u.prep0;
     const int i0 = t / tj * NS_TILE_PREP, j0 = t % tj * NS_TILE_PREP;
     const f16_t* hi = (const f16_t*)(ws + u.x[0]);
@@ -593,7 +616,7 @@ struct NsPlan {
     long long slab() const { return split > 1 ? (long long)(tiles - whole) * split * 16384ll * tw * tw : 0; }
 };
 struct NsLayout {
-    long long table = 0, parts = 0, slab = 0, bytes = 0;
+    long long table = 0, heads = 0, parts = 0, slab = 0, bytes = 0;
     int nparts = 0, nprep = 0;
     bool pairs = false;  // two steps at once
     NsPlan gram, poly, full;
@@ -667,7 +690,8 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
     // two steps: gram, poly, full each twice, or gram, five m x m products, full; 3 us a launch
     l.pairs = l.gram.us + 5 * l.poly.us + l.full.us + 21.0 < 0.9 * (2 * (l.gram.us + l.poly.us + l.full.us) + 18.0);
     l.table = 0;
-    l.parts = ns_align((long long)n * (long long)sizeof(NsUnit));
+    l.heads = ns_align((long long)n * (long long)sizeof(NsUnit));
+    l.parts = ns_align(l.heads + 5ll * n * (long long)sizeof(ns_head));
     l.slab = ns_align(l.parts + 8 * nparts);
     long long at = ns_align(l.slab + std::max(l.gram.slab(), l.poly.slab()));
     int part = 0, first = 0, next[3] = {}, group0[3] = {}, group[3] = {};
@@ -744,15 +768,15 @@ bool ns_exponent(const float* coefficients, int steps, bool pairs, int* exponent
 }
 
 template <int KIND, typename T>
-int ns_gemm(const NsLayout& l, const NsUnit* table, int n, char* ws, NsStep st, hipStream_t s) {
+int ns_gemm(const NsLayout& l, const NsTable& table, char* ws, NsStep st, hipStream_t s) {
     const NsPlan& p = KIND == NS_GRAM ? l.gram : KIND == NS_SQUARE ? l.poly : l.full;
     st.whole = p.whole; st.split = p.split; st.slab = (float*)(ws + l.slab);
-    if (p.tw == 2) hipLaunchKernelGGL((ns_gemm_kernel<2, KIND, T>), dim3(p.grid()), dim3(256), 0, s, table, n, ws, st);
-    else hipLaunchKernelGGL((ns_gemm_kernel<1, KIND, T>), dim3(p.grid()), dim3(256), 0, s, table, n, ws, st);
+    if (p.tw == 2) hipLaunchKernelGGL((ns_gemm_kernel<2, KIND, T>), dim3(p.grid()), dim3(256), 0, s, table, ws, st);
+    else hipLaunchKernelGGL((ns_gemm_kernel<1, KIND, T>), dim3(p.grid()), dim3(256), 0, s, table, ws, st);
     if constexpr (KIND == NS_GRAM || KIND == NS_SQUARE)
         if (p.joined()) {
-            if (p.tw == 2) hipLaunchKernelGGL((ns_join_kernel<2, KIND>), dim3(4 * p.joined()), dim3(64), 0, s, table, n, ws, st);
-            else hipLaunchKernelGGL((ns_join_kernel<1, KIND>), dim3(4 * p.joined()), dim3(64), 0, s, table, n, ws, st);
+            if (p.tw == 2) hipLaunchKernelGGL((ns_join_kernel<2, KIND>), dim3(4 * p.joined()), dim3(64), 0, s, table, ws, st);
+            else hipLaunchKernelGGL((ns_join_kernel<1, KIND>), dim3(4 * p.joined()), dim3(64), 0, s, table, ws, st);
         }
     return hipGetLastError() == hipSuccess ? V1T_OK : V1T_ERR_LAUNCH;
 }
@@ -766,7 +790,7 @@ NsStep ns_square(int out, int p, int q, float alpha, int d, float beta, int d2 =
 }
 
 template <typename T>
-int ns_steps(const NsLayout& l, const NsUnit* table, int n, char* ws, int steps, const float* co, bool pairs, int exponent, hipStream_t s) {
+int ns_steps(const NsLayout& l, const NsTable& table, char* ws, int steps, const float* co, bool pairs, int exponent, hipStream_t s) {
     enum { A = 0, S = 1, U = 2, S1 = 3 };  // the m x m matrices; U holds T, then Q
     const float inv = std::ldexp(1.f, -exponent);
     int from = 0;
@@ -774,20 +798,20 @@ int ns_steps(const NsLayout& l, const NsUnit* table, int n, char* ws, int steps,
         const float a = co[3 * k], b = co[3 * k + 1], c = co[3 * k + 2];
         NsStep st{};
         st.alpha = inv; st.from = from; st.inv = inv;
-        NS_TRY((ns_gemm<NS_GRAM, float>(l, table, n, ws, st, s)));
-        NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, n, ws, ns_square(S, A, A, c * inv, A, b), s)));
+        NS_TRY((ns_gemm<NS_GRAM, float>(l, table, ws, st, s)));
+        NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, ws, ns_square(S, A, A, c * inv, A, b), s)));
         st.p = S; st.beta = a;
         if (pairs && k + 1 < steps) {
             const float a1 = co[3 * k + 3], b1 = co[3 * k + 4], c1 = co[3 * k + 5];
-            NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, n, ws, ns_square(U, S, A, inv, A, a), s)));
-            NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, n, ws, ns_square(A, S, U, inv, U, a), s)));
-            NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, n, ws, ns_square(S1, A, A, c1 * inv, A, b1), s)));
-            NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, n, ws, ns_square(U, S1, S, inv, S, a1, S1, a, k == 0 ? 0.f : std::ldexp(a * a1, exponent)), s)));
+            NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, ws, ns_square(U, S, A, inv, A, a), s)));
+            NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, ws, ns_square(A, S, U, inv, U, a), s)));
+            NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, ws, ns_square(S1, A, A, c1 * inv, A, b1), s)));
+            NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, ws, ns_square(U, S1, S, inv, S, a1, S1, a, k == 0 ? 0.f : std::ldexp(a * a1, exponent)), s)));
             st.p = U; st.beta = k == 0 ? a * a1 : 0.f;
             ++k;
         }
-        if (k + 1 < steps) NS_TRY((ns_gemm<NS_APPLY, float>(l, table, n, ws, st, s)));
-        else NS_TRY((ns_gemm<NS_LAST, T>(l, table, n, ws, st, s)));
+        if (k + 1 < steps) NS_TRY((ns_gemm<NS_APPLY, float>(l, table, ws, st, s)));
+        else NS_TRY((ns_gemm<NS_LAST, T>(l, table, ws, st, s)));
         from ^= 1;
     }
     return V1T_OK;
@@ -798,16 +822,16 @@ int ns_run(const NsLayout& l, int n, char* ws, const NsMomentum& mo, float eps, 
     int exponent = 0;
     const bool pairs = l.pairs && ns_exponent(co, steps, true, &exponent);  // coefficients whose pairs would leave the planes' range go step by step
     if (!pairs && !ns_exponent(co, steps, false, &exponent)) return V1T_ERR_ARG;
-    const NsUnit* table = (const NsUnit*)(ws + l.table);
+    const NsTable table{(const NsUnit*)(ws + l.table), (const ns_head*)(ws + l.heads), n};
     double* parts = (double*)(ws + l.parts);
-    hipLaunchKernelGGL((ns_norm_kernel<T, MOM>), dim3(l.nparts), dim3(256), 0, s, table, n, mo, parts);
-    hipLaunchKernelGGL((ns_prep_kernel<T, MOM>), dim3(l.nprep), dim3(256), 0, s, table, n, mo, parts, ws, eps, std::ldexp(1.f, exponent), zero);
+    hipLaunchKernelGGL((ns_norm_kernel<T, MOM>), dim3(l.nparts), dim3(256), 0, s, table, mo, parts);
+    hipLaunchKernelGGL((ns_prep_kernel<T, MOM>), dim3(l.nprep), dim3(256), 0, s, table, mo, parts, ws, eps, std::ldexp(1.f, exponent), zero);
     if (hipGetLastError() != hipSuccess) return V1T_ERR_LAUNCH;
     if (steps == 0) {
-        hipLaunchKernelGGL((ns_copy_kernel<T>), dim3(l.nprep), dim3(256), 0, s, table, n, ws, std::ldexp(1.f, -exponent));
+        hipLaunchKernelGGL((ns_copy_kernel<T>), dim3(l.nprep), dim3(256), 0, s, table, ws, std::ldexp(1.f, -exponent));
         return hipGetLastError() == hipSuccess ? V1T_OK : V1T_ERR_LAUNCH;
     }
-    return ns_steps<T>(l, table, n, ws, steps, co, pairs, exponent, s);
+    return ns_steps<T>(l, table, ws, steps, co, pairs, exponent, s);
 }
 
 // lays out the units, checks the workspace, writes the table
@@ -825,7 +849,7 @@ int ns_begin(int n, Shape shape, Fill fill, void* workspace, long long ws_bytes,
         c.u[i % NS_CHUNK] = u;
         if (i % NS_CHUNK == NS_CHUNK - 1 || i == n - 1) {
             const int k = i % NS_CHUNK + 1;
-            hipLaunchKernelGGL(ns_table_kernel, dim3(1), dim3(256), 0, s, c, k, table + (i - k + 1));
+            hipLaunchKernelGGL(ns_table_kernel, dim3(1), dim3(256), 0, s, c, k, i - k + 1, n, table, (ns_head*)((char*)workspace + l.heads));
             if (hipGetLastError() != hipSuccess) rc = V1T_ERR_LAUNCH;
         }
     }, again);

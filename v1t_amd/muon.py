@@ -104,36 +104,45 @@ def muon_step(params: t.Sequence[torch.Tensor], grads: t.Sequence[torch.Tensor],
     params, grads, moments = list(params), list(grads), list(moments)
     if not len(params) == len(grads) == len(moments):
         raise ValueError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(moments)} momenta")
-    lrs = list(lr) if isinstance(lr, (list, tuple)) else [lr] * len(params)
+    lrs = [float(x) for x in lr] if isinstance(lr, (list, tuple)) else [float(lr)] * len(params)
     if len(lrs) != len(params):
         raise ValueError(f"muon_step: {len(lrs)} learning rates for {len(params)} parameters")
     co = _coefficients(coefficients, steps)
-    if not 0.0 <= float(eps) < math.inf or not all(math.isfinite(float(x)) for x in (momentum, weight_decay, l1, *lrs)):
+    eps, momentum, weight_decay, l1 = float(eps), float(momentum), float(weight_decay), float(l1)
+    if not 0.0 <= eps < math.inf or not all(map(math.isfinite, (momentum, weight_decay, l1, *lrs))):
         raise ValueError("muon_step: eps is non-negative, every coefficient is finite")
-    for p, g, m in zip(params, grads, moments):
-        if p.dim() < 2:
-            raise ValueError(f"muon_step: a parameter of shape {tuple(p.shape)} is no matrix")
-        for x in (p, g, m):
-            if x.dtype != torch.float32:
-                raise TypeError(f"muon_step: fp32 tensors are needed, got {x.dtype}")
-            if x.shape != p.shape or not x.is_contiguous() or x.device != params[0].device:
-                raise ValueError(f"muon_step: parameter, gradient and momentum are contiguous tensors of one shape on one device, got {[tuple(y.shape) for y in (p, g, m)]}")
-    spans = sorted((x.data_ptr(), x.data_ptr() + 4 * x.numel()) for x in params + grads + moments if x.numel())
-    if any(b < e for (_, e), (b, _) in zip(spans, spans[1:])):
-        raise ValueError("muon_step: tensors of the call share memory")
-    triples = [x for x in zip(params, grads, moments, lrs) if x[0].numel()]
-    if not triples:
+    rs, spans, device = [], [], params[0].get_device() if params else 0
+    for p, g, m, a in zip(params, grads, moments, lrs):
+        shape = p.shape
+        if len(shape) < 2:
+            raise ValueError(f"muon_step: a parameter of shape {tuple(shape)} is no matrix")
+        if not p.dtype is g.dtype is m.dtype is torch.float32:
+            raise TypeError(f"muon_step: fp32 tensors are needed, got {[x.dtype for x in (p, g, m)]}")
+        if not (g.shape == shape == m.shape and p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and p.get_device() == g.get_device() == m.get_device() == device):
+            raise ValueError(f"muon_step: parameter, gradient and momentum are contiguous tensors of one shape on one device, got {[(tuple(x.shape), str(x.device)) for x in (p, g, m)]}")
+        size = p.numel()
+        if size == 0:
+            continue
+        rows, at = shape[0], (p.data_ptr(), g.data_ptr(), m.data_ptr())
+        cols = size // rows
+        spans += [(x, x + 4 * size) for x in at]
+        rs.append(L.MuonRange(*at, rows, cols, a * (rows / cols) ** 0.5 if rows > cols else a, 1.0 - a * weight_decay, l1, 0))
+    spans.sort()
+    end = 0
+    for x, y in spans:
+        if x < end:
+            raise ValueError("muon_step: tensors of the call share memory")
+        end = y
+    if not rs:
         return
     L.require_cuda(params[0], "muon_step")
-    rs = []
-    for p, g, m, a in triples:
-        rows, cols = p.shape[0], p.numel() // p.shape[0]
-        rs.append(L.MuonRange(p.data_ptr(), g.data_ptr(), m.data_ptr(), rows, cols, float(a) * math.sqrt(max(1.0, rows / cols)), 1.0 - float(a) * weight_decay, l1, 0))
-    with torch.cuda.device(params[0].device):
-        muon_ranges(rs, momentum, nesterov, int(steps), co, float(eps), zero_grad, params[0].device)
-    for x in params + moments + (grads if zero_grad else []):
-        if not x.is_inference():
-            torch.autograd.graph.increment_version(x)
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            muon_ranges(rs, momentum, nesterov, int(steps), co, eps, zero_grad, params[0].device)
+    else:
+        muon_ranges(rs, momentum, nesterov, int(steps), co, eps, zero_grad, params[0].device)
+    touched = params + moments + (grads if zero_grad else [])
+    torch.autograd.graph.increment_version([x for x in touched if not x.is_inference()])
 
 
 def muon_ranges(rs: t.Sequence[L.MuonRange], momentum: float, nesterov: bool, steps: int, co, eps: float, zero_grad: bool, device) -> None:
