@@ -445,7 +445,8 @@ typedef struct v1t_rotary_operand {
     const void* x;
     void* y;
     long long x_stride_b, x_stride_t, x_stride_h, y_stride_b, y_stride_t, y_stride_h;
-    int heads, pad_;
+    int heads;
+    int y_room; /* features of a head's row of y that may be written, >= D (those behind D: any value); 0: D. Room to the next 8 spares odd D a pass by features */
 } v1t_rotary_operand;
 int v1t_rotary(const v1t_rotary_operand* operands, int n_operands, int dtype, int B, int T, int D, const int* sections, int n_axes, double base, int shared,
                int halves, int inverse, const void* positions, int position_type, long long pos_stride_b, long long pos_stride_t, long long pos_stride_a,

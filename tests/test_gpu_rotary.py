@@ -162,7 +162,7 @@ def test_gradients(layout):
             step[i] = 1.0
             plus, minus = (v1t_amd.rotary(q + s * step.view_as(q), at, **arguments) for s in (1.0, -1.0))
             slope = float((wq.double() * (plus.double() - minus.double())).sum() / 2)
-            assert abs(slope - float(dq.view(-1)[i])) < 64 * 8 * 4e-7
+            assert abs(slope - float(dq.reshape(-1)[i])) < 64 * 8 * 4e-7
 
 
 def test_second_derivative():

@@ -3,10 +3,10 @@
 //     y0 = x0 cos - x1 sin,  y1 = x0 sin + x1 cos        (backward: the same with the angle negated - a rotation's transpose is its inverse)
 // Features behind the 2 * pairs rotated ones pass through. One pass: every element is read once and written once.
 //
-// Bound: HBM (2 B of flops per byte). A workgroup owns a run of tokens. It writes their (cos, sin) to LDS once and applies them to every head
-// of q and of k, and to every sequence of its batch chunk where the sequences share their positions: the angle (a 64-bit product, below)
-// would otherwise cost as much as the memory traffic of the element it turns. A thread moves "slots" of 4 pairs, the unit at which one
-// 16-byte access of 16-bit pairs is whole.
+// Bound: HBM (2 B of flops per byte). A thread owns a "slot" of 4 pairs of one token - 16 B of 16-bit features - and with it 4 angles, whose cosines and
+// sines stay in its registers while it walks over the heads of q and of k, and over the sequences of its batch chunk where these share their positions:
+// the angle, a 64-bit product (below), costs as much as several slots' traffic, and the walk costs two address additions a slot. Four heads' loads
+// stand together.
 //
 // Numerics: the angle is held as a number of turns in 64 bits, p * (rate / 2 pi), and reduced to [-1/2, 1/2] before it is rounded to 32: a
 // 32-bit product is off by 0.03 rad at position 10^6. Products and sums of the rotation are fp32, rounded once to the tensor's type.
@@ -22,7 +22,6 @@ namespace {
 
 constexpr int ROT_MAX_PAIRS = 256;
 constexpr int ROT_THREADS = 256;
-constexpr int ROT_LDS_PAIRS = 2048;  // (token, pair) entries of the table in LDS: 16 KB
 
 struct RotRates {  // kernel argument: a captured graph keeps it, no device memory behind it
     double turns[ROT_MAX_PAIRS];
@@ -36,128 +35,163 @@ struct RotArgs {
     int heads[2];
     const void* pos;
     long long pb, pt, pa;
-    int B, T, D, pairs, halves, inverse;
-    int nt, nb;          // tokens and sequences per workgroup
-    int slots, tails;    // per head: slots of 4 pairs, and groups of 8 features behind the rotated ones
-    unsigned items_mul, row_mul;  // divide an item's number by (slots + tails) * heads and by (slots + tails) (division_multiplier)
+    int B, T, D, pairs, inverse;
+    int slots, turned;   // slots of a token's head; the first `turned` of them turn, the others copy
+    int nt;              // tokens per workgroup
+    int nb, hc;          // sequences and heads (of q and k together) per workgroup
+    int overlap;         // the last slot of a number of pairs that a slot's does not divide lies over the one before it (out of place: both write the same)
+    int tail, tail_at;   // features behind the last slot that are copied
+    unsigned pairs_mul;  // divides an entry's number by pairs
+    unsigned tail_mul, per_mul;  // divide a copied feature's number by tail and by tail * heads (division_multiplier)
 };
 
 DEVFN int quotient(int x, int d, unsigned mul) { return mul ? (int)__umulhi((unsigned)x, mul) : x / d; }
 
-template <typename T> DEVFN float to_f(T v) { return (float)v; }
-
-// n elements from p in accesses of VB bytes (the launcher's guarantee: every run starts at a multiple of VB)
-template <typename T, int N, int VB>
-DEVFN void load_run(const T* p, float (&v)[N]) {
-    constexpr int E = VB / (int)sizeof(T);
-    typedef T vec __attribute__((ext_vector_type(E == 1 ? 2 : E)));
-    if constexpr (E == 1) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = to_f(p[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i += E) {
-            const vec a = *reinterpret_cast<const vec*>(p + i);
-#pragma unroll
-            for (int j = 0; j < E; ++j) v[i + j] = to_f(a[j]);
-        }
-    }
-}
-template <typename T, int N, int VB>
-DEVFN void store_run(T* p, const float (&v)[N]) {
-    constexpr int E = VB / (int)sizeof(T);
-    typedef T vec __attribute__((ext_vector_type(E == 1 ? 2 : E)));
-    if constexpr (E == 1) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) p[i] = (T)v[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i += E) {
-            vec a;
-#pragma unroll
-            for (int j = 0; j < E; ++j) a[j] = (T)v[i + j];
-            *reinterpret_cast<vec*>(p + i) = a;
-        }
-    }
+// One rotation, the same operations wherever it stands: in place and out of place agree to the bit
+DEVFN void rotate(float& p, float& q, float c, float s) {
+    const float u = fmaf(p, c, -__fmul_rn(q, s)), v = fmaf(p, s, __fmul_rn(q, c));
+    p = u;
+    q = v;
 }
 
-template <typename T, int VB, bool HALVES, typename P>
-__global__ __launch_bounds__(ROT_THREADS) void rotary_kernel(RotArgs g, RotRates rates) {
-    __shared__ __attribute__((aligned(16))) float s_cos[ROT_LDS_PAIRS], s_sin[ROT_LDS_PAIRS];
-    const int t0 = blockIdx.x * g.nt, b0 = blockIdx.y * g.nb;
-    const int nt = min(g.nt, g.T - t0), nb = min(g.nb, g.B - b0);
-    const int row = g.slots + g.tails, per_token = row * (g.heads[0] + g.heads[1]);
-    const int ldp = (g.pairs + 3) & ~3;
-    const bool same_place = g.pb == 0;
-    auto table = [&](int b) {
-        const P* pos = (const P*)g.pos + (long long)b * g.pb;
-        for (int i = threadIdx.x; i < nt * ldp; i += ROT_THREADS) {
-            const int t = i / ldp, j = i - t * ldp;
-            if (j < g.pairs) {
-                const double turns = (double)pos[(long long)(t0 + t) * g.pt + rates.axis[j] * g.pa] * rates.turns[j];
-                const float r = (float)(turns - rint(turns));
-                float s, c;
-                sincospif(2.f * r, &s, &c);
-                s_cos[i] = c;
-                s_sin[i] = g.inverse ? -s : s;
-            }
-        }
-    };
-    if (same_place) {
-        table(0);
-        __syncthreads();
+// In memory a slot is one run of features, or ("halves") two. The vector types ask for an element's alignment only: the compiler's 16-byte accesses take any,
+// and rows of odd lengths, or views, start anywhere
+template <typename T, bool HALVES>
+struct Slot {
+    static constexpr int PAIRS = 4, RUN = HALVES ? 4 : 8;
+    typedef T vec __attribute__((ext_vector_type(RUN), aligned(sizeof(T))));
+    vec a, b;
+    DEVFN void load(const T* x, int apart) {  // apart: from the first run to the second
+        a = *(const vec*)x;
+        if constexpr (HALVES) b = *(const vec*)(x + apart);
     }
-    for (int b = b0; b < b0 + nb; ++b) {
-        if (!same_place) {
-            __syncthreads();
-            table(b);
-            __syncthreads();
-        }
-        for (int i = threadIdx.x; i < nt * per_token; i += ROT_THREADS) {
-            const int t = quotient(i, per_token, g.items_mul), r = i - t * per_token;
-            const int hh = quotient(r, row, g.row_mul), v = r - hh * row;
-            const int w = hh >= g.heads[0], h = w ? hh - g.heads[0] : hh;
-            const T* x = (const T*)g.x[w] + (long long)b * g.xb[w] + (long long)(t0 + t) * g.xt[w] + (long long)h * g.xh[w];
-            T* y = (T*)g.y[w] + (long long)b * g.yb[w] + (long long)(t0 + t) * g.yt[w] + (long long)h * g.yh[w];
-            if (v < g.slots) {
-                const int j = 4 * v;
-                const f32x4 c = *(const f32x4*)&s_cos[t * ldp + j], s = *(const f32x4*)&s_sin[t * ldp + j];
-                if (j + 4 <= g.pairs) {
-                    if constexpr (HALVES) {
-                        float a[4], d[4];
-                        load_run<T, 4, VB>(x + j, a);
-                        load_run<T, 4, VB>(x + g.pairs + j, d);
+    DEVFN void store(T* y, int apart) const {
+        *(vec*)y = a;
+        if constexpr (HALVES) *(vec*)(y + apart) = b;
+    }
+    DEVFN void up(int n) {  // feature e + n at e
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float p = a[e] * c[e] - d[e] * s[e], q = a[e] * s[e] + d[e] * c[e];
-                            a[e] = p;
-                            d[e] = q;
-                        }
-                        store_run<T, 4, VB>(y + j, a);
-                        store_run<T, 4, VB>(y + g.pairs + j, d);
-                    } else {
-                        float a[8];
-                        load_run<T, 8, VB>(x + 2 * j, a);
+        for (int step = 4; step > 0; step >>= 1)
+            if (n & step)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float p = a[2 * e] * c[e] - a[2 * e + 1] * s[e], q = a[2 * e] * s[e] + a[2 * e + 1] * c[e];
-                            a[2 * e] = p;
-                            a[2 * e + 1] = q;
-                        }
-                        store_run<T, 8, VB>(y + 2 * j, a);
-                    }
-                } else {  // the last slot of a number of pairs that 4 does not divide
-                    for (int e = 0; j + e < g.pairs; ++e) {
-                        const int i0 = HALVES ? j + e : 2 * (j + e), i1 = HALVES ? g.pairs + j + e : i0 + 1;
-                        const float a = to_f(x[i0]), d = to_f(x[i1]);
-                        y[i0] = (T)(a * c[e] - d * s[e]);
-                        y[i1] = (T)(a * s[e] + d * c[e]);
-                    }
+                for (int e = 0; e + step < 8; ++e) {
+                    const T x = !HALVES || e + step < 4 ? a[HALVES ? (e + step) & 3 : e + step] : b[(e + step) & 3];
+                    if (!HALVES || e < 4) a[HALVES ? e & 3 : e] = x;
+                    else b[e & 3] = x;
                 }
+    }
+    DEVFN void turn(const float (&c)[PAIRS], const float (&s)[PAIRS]) {
+#pragma unroll
+        for (int e = 0; e < PAIRS; ++e) {
+            float p = (float)(HALVES ? a[e] : a[2 * e]), q = (float)(HALVES ? b[e] : a[2 * e + 1]);
+            rotate(p, q, c[e], s[e]);
+            if constexpr (HALVES) {
+                a[e] = (T)p;
+                b[e] = (T)q;
             } else {
-                const int j = 2 * g.pairs + 8 * (v - g.slots);
-                for (int e = j; e < min(j + 8, g.D); ++e) y[e] = x[e];
+                a[2 * e] = (T)p;
+                a[2 * e + 1] = (T)q;
             }
+        }
+    }
+};
+
+template <typename T, bool HALVES, typename P>
+__global__ __launch_bounds__(ROT_THREADS, 4) void rotary_kernel(RotArgs g, RotRates rates) {
+    const int t = threadIdx.x / g.slots, v = threadIdx.x - t * g.slots, t0 = blockIdx.x * g.nt;
+    const bool mine = t < g.nt && t0 + t < g.T;
+    using Part = Slot<T, HALVES>;
+    constexpr int S = Part::PAIRS, N = 4;  // N heads' loads stand together
+    const bool turns = v < g.turned;
+    const int j = g.overlap ? min(S * v, g.pairs - S) : S * v, whole = turns ? min(S, g.pairs - j) : S;
+    // the last of the copying slots may reach into y's room behind the features: it reads the row's last 8 and moves them up
+    const int at = !turns ? 2 * g.pairs + 2 * S * (v - g.turned) : HALVES ? j : 2 * j, apart = turns ? g.pairs : Part::RUN;
+    const int over = !turns ? max(0, at + 2 * S - g.D) : 0;
+    const int h0 = blockIdx.z * g.hc, h1 = min(h0 + g.hc, g.heads[0] + g.heads[1]);
+    // the cosines and sines of the workgroup's tokens, each computed once, then a thread's own in its registers
+    __shared__ float s_cos[ROT_THREADS * S], s_sin[ROT_THREADS * S];
+    float c[S], s[S];
+    auto angles = [&](int b) {
+        const P* pos = (const P*)g.pos + (long long)b * g.pb + (long long)t0 * g.pt;
+        const int entries = min(g.nt, g.T - t0) * g.pairs;
+        for (int i = threadIdx.x; i < entries; i += ROT_THREADS) {
+            const int ti = quotient(i, g.pairs, g.pairs_mul), k = i - ti * g.pairs;
+            const double turns = (double)pos[(long long)ti * g.pt + rates.axis[k] * g.pa] * rates.turns[k];
+            float sine, cosine;
+            sincospif(2.f * (float)(turns - rint(turns)), &sine, &cosine);
+            s_cos[i] = cosine;
+            s_sin[i] = g.inverse ? -sine : sine;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < S; ++e) {
+            const int i = t * g.pairs + min(j + e, g.pairs - 1);
+            c[e] = mine && turns ? s_cos[i] : 1.f;
+            s[e] = mine && turns ? s_sin[i] : 0.f;
+        }
+        __syncthreads();
+    };
+    // the features behind the last slot, one a thread, densely: in their slots' place they would leave most lanes of a wave waiting
+    const int copies = g.tail > 0 ? min(g.nt, g.T - t0) * (h1 - h0) * g.tail : 0;
+    auto copied = [&](int i, const T*& from, T*& to) {
+        const int per = (h1 - h0) * g.tail, ti = g.hc == h1 - h0 ? quotient(i, per, g.per_mul) : i / per, r = i - ti * per;
+        const int hh = quotient(r, g.tail, g.tail_mul), f = g.tail_at + r - hh * g.tail, w = h0 + hh >= g.heads[0], h = w ? h0 + hh - g.heads[0] : h0 + hh;
+        from = (const T*)g.x[w] + (long long)(t0 + ti) * g.xt[w] + (long long)h * g.xh[w] + f;
+        to = (T*)g.y[w] + (long long)(t0 + ti) * g.yt[w] + (long long)h * g.yh[w] + f;
+        return w;
+    };
+    const int b0 = blockIdx.y * g.nb, b1 = min(b0 + g.nb, g.B);
+    if (g.pb == 0) angles(0);
+    for (int b = b0; b < b1; ++b) {
+        if (g.pb != 0) angles(b);
+#pragma unroll 1
+        for (int w = 0; w < 2; ++w) {
+            if (!mine) break;
+            const int first = w ? g.heads[0] : 0, lo = max(h0, first) - first, hi = min(h1 - first, g.heads[w]);
+            const T* x = (const T*)g.x[w] + (long long)b * g.xb[w] + (long long)(t0 + t) * g.xt[w] + (long long)lo * g.xh[w] + at;
+            T* y = (T*)g.y[w] + (long long)b * g.yb[w] + (long long)(t0 + t) * g.yt[w] + (long long)lo * g.yh[w] + at;
+            if (whole == S) {
+                int h = lo;
+#pragma unroll 1
+                for (; h + N <= hi; h += N) {
+                    Part slot[N];
+#pragma unroll
+                    for (int n = 0; n < N; ++n) slot[n].load(x + n * g.xh[w] - over, apart);
+#pragma unroll
+                    for (int n = 0; n < N; ++n) {
+                        if (turns) slot[n].turn(c, s);
+                        else slot[n].up(over);
+                        slot[n].store(y + n * g.yh[w], apart);
+                    }
+                    x += N * g.xh[w];
+                    y += N * g.yh[w];
+                }
+#pragma unroll 1
+                for (; h < hi; ++h, x += g.xh[w], y += g.yh[w]) {
+                    Part slot;
+                    slot.load(x - over, apart);
+                    if (turns) slot.turn(c, s);
+                    else slot.up(over);
+                    slot.store(y, apart);
+                }
+            } else {  // in place, or fewer pairs than a slot in all
+#pragma unroll 1
+                for (int i = 0; i < (hi - lo) * whole; ++i) {
+                    const int h = i / whole, e = i - h * whole, i0 = HALVES ? e : 2 * e, i1 = HALVES ? g.pairs + e : i0 + 1;
+                    const T* xh = x + (long long)h * g.xh[w];
+                    T* yh = y + (long long)h * g.yh[w];
+                    float p = (float)xh[i0], q = (float)xh[i1];
+                    rotate(p, q, s_cos[t * g.pairs + j + e], s_sin[t * g.pairs + j + e]);
+                    yh[i0] = (T)p;
+                    yh[i1] = (T)q;
+                }
+            }
+        }
+        for (int i = threadIdx.x; i < copies; i += ROT_THREADS) {
+            const T* p;
+            T* q;
+            const int w = copied(i, p, q);
+            q[(long long)b * g.yb[w]] = p[(long long)b * g.xb[w]];
         }
     }
 }
@@ -170,24 +204,16 @@ unsigned division_multiplier(long long d, long long limit) {
     return e && (unsigned long long)limit > ((1ull << 32) - 1) / e ? 0 : (unsigned)m;
 }
 
-template <typename T, int VB, bool HALVES>
+template <typename T, bool HALVES>
 int launch_p(const RotArgs& a, const RotRates& r, int pos_type, dim3 grid, hipStream_t s) {
-    if (pos_type == 0) hipLaunchKernelGGL((rotary_kernel<T, VB, HALVES, int>), grid, dim3(ROT_THREADS), 0, s, a, r);
-    else if (pos_type == 1) hipLaunchKernelGGL((rotary_kernel<T, VB, HALVES, long long>), grid, dim3(ROT_THREADS), 0, s, a, r);
-    else hipLaunchKernelGGL((rotary_kernel<T, VB, HALVES, float>), grid, dim3(ROT_THREADS), 0, s, a, r);
+    if (pos_type == 0) hipLaunchKernelGGL((rotary_kernel<T, HALVES, int>), grid, dim3(ROT_THREADS), 0, s, a, r);
+    else if (pos_type == 1) hipLaunchKernelGGL((rotary_kernel<T, HALVES, long long>), grid, dim3(ROT_THREADS), 0, s, a, r);
+    else hipLaunchKernelGGL((rotary_kernel<T, HALVES, float>), grid, dim3(ROT_THREADS), 0, s, a, r);
     return hipGetLastError() == hipSuccess ? V1T_OK : V1T_ERR_LAUNCH;
 }
-template <typename T, bool HALVES>
-int launch_v(const RotArgs& a, const RotRates& r, int pos_type, int vb, dim3 grid, hipStream_t s) {
-    if (!HALVES || sizeof(T) == 4)
-        if (vb == 16) return launch_p<T, 16, HALVES>(a, r, pos_type, grid, s);
-    if (vb >= 8) return launch_p<T, 8, HALVES>(a, r, pos_type, grid, s);
-    if (sizeof(T) == 2 && vb >= 4) return launch_p<T, 4, HALVES>(a, r, pos_type, grid, s);
-    return launch_p<T, (int)sizeof(T), HALVES>(a, r, pos_type, grid, s);
-}
 template <typename T>
-int launch_t(const RotArgs& a, const RotRates& r, int pos_type, int vb, dim3 grid, hipStream_t s) {
-    return a.halves ? launch_v<T, true>(a, r, pos_type, vb, grid, s) : launch_v<T, false>(a, r, pos_type, vb, grid, s);
+int launch_t(const RotArgs& a, const RotRates& r, int halves, int pos_type, dim3 grid, hipStream_t s) {
+    return halves ? launch_p<T, true>(a, r, pos_type, grid, s) : launch_p<T, false>(a, r, pos_type, grid, s);
 }
 
 }  // namespace
@@ -204,7 +230,6 @@ extern "C" int v1t_rotary(const v1t_rotary_operand* ops, int n_ops, int dtype, i
     }
     if (pairs < 1 || 2 * pairs > D) return V1T_ERR_ARG;
     if (pairs > ROT_MAX_PAIRS) return V1T_ERR_UNSUPPORTED;
-    if (B == 0 || T == 0) return V1T_OK;
     RotArgs g{};
     RotRates r{};
     for (int a = 0, j = 0; a < n_axes; ++a)
@@ -213,44 +238,55 @@ extern "C" int v1t_rotary(const v1t_rotary_operand* ops, int n_ops, int dtype, i
             r.turns[j] = std::pow(base, -part) / 6.283185307179586476925286766559;
             r.axis[j] = (unsigned char)a;
         }
-    const int es = dtype == 2 ? 4 : 2;
-    int vb = 16;
     bool in_place = true;
-    auto aligned = [&](long long bytes) {
-        while (vb > es && (bytes & (vb - 1))) vb >>= 1;
-    };
+    long long heads = 0;
+    int room = 1 << 30;
     for (int o = 0; o < n_ops; ++o) {
         const v1t_rotary_operand& p = ops[o];
         if (!p.x || !p.y || p.heads < 1) return V1T_ERR_ARG;
         g.x[o] = p.x; g.y[o] = p.y; g.heads[o] = p.heads;
         g.xb[o] = p.x_stride_b; g.xt[o] = p.x_stride_t; g.xh[o] = p.x_stride_h;
         g.yb[o] = p.y_stride_b; g.yt[o] = p.y_stride_t; g.yh[o] = p.y_stride_h;
-        aligned((long long)(uintptr_t)p.x);
-        aligned((long long)(uintptr_t)p.y);
-        for (long long st : {p.x_stride_b, p.x_stride_t, p.x_stride_h, p.y_stride_b, p.y_stride_t, p.y_stride_h}) aligned(st * es);
-        in_place = in_place && p.x == p.y && p.x_stride_b == p.y_stride_b && p.x_stride_t == p.y_stride_t && p.x_stride_h == p.y_stride_h;
+        heads += p.heads;
+        if (p.y_room < 0 || (p.y_room > 0 && p.y_room < D)) return V1T_ERR_ARG;
+        room = std::min(room, p.y_room > 0 ? p.y_room : D);
+        const bool same = p.x == p.y;
+        if (o > 0 && same != in_place) return V1T_ERR_ARG;
+        in_place = same;
+        if (same && (p.x_stride_b != p.y_stride_b || p.x_stride_t != p.y_stride_t || p.x_stride_h != p.y_stride_h)) return V1T_ERR_ARG;
     }
-    if (halves) aligned(pairs * es);
+    if (B == 0 || T == 0) return V1T_OK;
     g.pos = positions; g.pb = B == 1 ? 0 : pos_stride_b; g.pt = pos_stride_t; g.pa = pos_stride_a;
-    g.B = B; g.T = T; g.D = D; g.pairs = (int)pairs; g.halves = halves != 0; g.inverse = inverse != 0;
-    g.slots = (int)((pairs + 3) / 4);
-    g.tails = in_place ? 0 : (D - 2 * (int)pairs + 7) / 8;
-    const long long row = g.slots + g.tails, heads = (long long)g.heads[0] + g.heads[1], per_token = row * heads;
-    if (per_token > (1 << 20)) return V1T_ERR_UNSUPPORTED;
-    // tokens per workgroup: enough items for its threads to have several each, as the table in LDS allows
-    const int ldp = ((int)pairs + 3) & ~3;
-    long long nt = std::max(1ll, std::min<long long>(ROT_LDS_PAIRS / ldp, 4 * ROT_THREADS / per_token));
-    nt = std::min<long long>(nt, T);
-    // sequences per workgroup: the table is computed once for all of them; at least 2048 workgroups (8 a CU) are kept
-    const long long gx = (T + nt - 1) / nt;
+    g.B = B; g.T = T; g.D = D; g.pairs = (int)pairs; g.inverse = inverse != 0;
+    constexpr int slot = 4;  // Slot::PAIRS
+    g.turned = (int)((pairs + slot - 1) / slot);
+    g.overlap = !in_place && pairs >= slot;
+    const int rest = in_place ? 0 : D - 2 * (int)pairs;  // copied: by slots, and the remainder - if y's rows have no room for a whole one - by features
+    const bool whole = room >= 2 * (int)pairs + (rest + 2 * slot - 1) / (2 * slot) * (2 * slot) && D >= 2 * slot;
+    g.slots = std::min(g.turned + (whole ? rest + 2 * slot - 1 : rest) / (2 * slot), ROT_THREADS);
+    g.tail_at = 2 * (int)pairs + 2 * slot * (g.slots - g.turned);
+    g.tail = in_place ? 0 : std::max(0, D - g.tail_at);
+    g.nt = std::max(1, std::min(ROT_THREADS / g.slots, T));
+    g.pairs_mul = division_multiplier(pairs, g.nt * pairs);
+    // A workgroup takes all heads and as many sequences as share their positions with it, while 2048 workgroups (8 a CU) are left; fewer tokens than that: the heads
+    // are dealt out, down to the 4 whose loads stand together
+    const long long gx = ((long long)T + g.nt - 1) / g.nt;
     long long nb = g.pb == 0 ? std::max(1ll, std::min<long long>(16, gx * B / 2048)) : 1;
     nb = std::max(nb, ((long long)B + 65534) / 65535);
-    g.nt = (int)nt; g.nb = (int)nb;
-    g.items_mul = division_multiplier(per_token, nt * per_token);
-    g.row_mul = division_multiplier(row, per_token);
-    const dim3 grid((unsigned)gx, (unsigned)((B + nb - 1) / nb));
+    const long long gy = ((long long)B + nb - 1) / nb;
+    long long hc = heads;
+    while (hc > 4 && gx * gy * ((heads + hc - 1) / hc) < 2048) hc = (hc + 1) / 2;
+    hc = std::max(hc, (heads + 65534) / 65535);
+    if (heads > (1 << 24)) return V1T_ERR_UNSUPPORTED;
+    g.nb = (int)nb; g.hc = (int)hc;
+    if (g.tail > 0) {
+        if ((long long)g.nt * hc * g.tail > (1ll << 30)) return V1T_ERR_UNSUPPORTED;
+        g.tail_mul = division_multiplier(g.tail, hc * g.tail);
+        g.per_mul = division_multiplier(hc * g.tail, g.nt * hc * g.tail);
+    }
+    const dim3 grid((unsigned)gx, (unsigned)gy, (unsigned)((heads + hc - 1) / hc));
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == 0) return launch_t<bf16_t>(g, r, position_type, vb, grid, st);
-    if (dtype == 1) return launch_t<f16_t>(g, r, position_type, vb, grid, st);
-    return launch_t<float>(g, r, position_type, vb, grid, st);
+    if (dtype == 0) return launch_t<bf16_t>(g, r, halves, position_type, grid, st);
+    if (dtype == 1) return launch_t<f16_t>(g, r, halves, position_type, grid, st);
+    return launch_t<float>(g, r, halves, position_type, grid, st);
 }

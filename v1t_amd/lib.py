@@ -53,7 +53,7 @@ class AdamRange(C.Structure):
 
 class RotaryOperand(C.Structure):
     """`v1t_rotary_operand`: one tensor of `v1t_rotary`, its strides in elements."""
-    _fields_ = [("x", c_void_p), ("y", c_void_p), ("xb", c_ll), ("xt", c_ll), ("xh", c_ll), ("yb", c_ll), ("yt", c_ll), ("yh", c_ll), ("heads", c_int), ("pad_", c_int)]
+    _fields_ = [("x", c_void_p), ("y", c_void_p), ("xb", c_ll), ("xt", c_ll), ("xh", c_ll), ("yb", c_ll), ("yt", c_ll), ("yh", c_ll), ("heads", c_int), ("y_room", c_int)]
 
 
 class Matrix(C.Structure):

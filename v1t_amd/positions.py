@@ -60,7 +60,7 @@ def _check(q: torch.Tensor, k: t.Optional[torch.Tensor], positions: torch.Tensor
 
 
 def _launch(turn: _Turn, positions: torch.Tensor, pairs_of: t.Sequence[t.Tuple[torch.Tensor, torch.Tensor]]) -> None:
-    """One launch over [(x, y), ...]; x and y have unit stride in their last dimension."""
+    """One launch over [(x, y), ...]; x and y have unit stride in their last dimension, y is x or `_like` it."""
     x0 = pairs_of[0][0]
     if x0.numel() == 0:
         return
@@ -71,7 +71,7 @@ def _launch(turn: _Turn, positions: torch.Tensor, pairs_of: t.Sequence[t.Tuple[t
     ops = (L.RotaryOperand * len(pairs_of))()
     for o, (x, y) in zip(ops, pairs_of):
         sx, sy = x.stride(), y.stride()
-        o.x, o.y, o.heads = x.data_ptr(), y.data_ptr(), x.shape[-2]
+        o.x, o.y, o.heads, o.y_room = x.data_ptr(), y.data_ptr(), x.shape[-2], 0 if x is y else (x.shape[-1] + 7) // 8 * 8
         o.xb, o.xt, o.xh = (sx[0], sx[1], sx[2]) if four else (0, sx[0], sx[1])
         o.yb, o.yt, o.yh = (sy[0], sy[1], sy[2]) if four else (0, sy[0], sy[1])
     sp = positions.stride()
@@ -79,6 +79,13 @@ def _launch(turn: _Turn, positions: torch.Tensor, pairs_of: t.Sequence[t.Tuple[t
     L.check(L.load().v1t_rotary(ops, len(pairs_of), _DTYPES[x0.dtype], x0.shape[0] if four else 1, x0.shape[-3], x0.shape[-1], (C.c_int * n)(*turn.sections), n,
                                 turn.base, turn.shared, turn.halves, turn.inverse, positions.data_ptr(), _POSITION_TYPES[positions.dtype],
                                 sp[0] if positions.dim() == 3 else 0, sp[-2], sp[-1], L.stream()), "rotary")
+
+
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """x's shape with room for a multiple of 8 features a head: what lies behind the last whole 8 is moved as one store, too."""
+    d = x.shape[-1]
+    y = torch.empty((*x.shape[:-1], (d + 7) // 8 * 8), dtype=x.dtype, device=x.device)
+    return y if y.shape[-1] == d else y[..., :d]
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -95,7 +102,7 @@ class _RotaryFn(torch.autograd.Function):
                 L.leaf_in_capture(x, "rotary")
         ctx.save_for_backward(positions)
         xs = [_rows(x) for x in (q, k) if x is not None]
-        ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+        ys = [_like(x) for x in xs]
         _launch(turn, positions, list(zip(xs, ys)))
         return ys[0] if k is None else tuple(ys)
 
@@ -115,7 +122,8 @@ class _RotaryFn(torch.autograd.Function):
 
 def rotary(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int], k: t.Optional[torch.Tensor] = None, base: float = 10000.0,
            layout: str = "pairs", shared: bool = False, inverse: bool = False):
-    """q (and k) turned by their tokens' positions: new contiguous tensors; differentiable in q and k.
+    """q (and k) turned by their tokens' positions: new tensors; differentiable in q and k. Where 8 does not divide the number of features, the
+    result is a view of rows that have room for the next multiple (`reshape`, not `view`, joins its heads).
 
     q: (batch, tokens, heads, features) or (tokens, heads, features), bf16 / fp16 / fp32, any strides; k: the same with its own number of heads.
     positions: (tokens, axes) for all sequences, or (batch, tokens, axes); int32, int64 or fp32, negative ones too. A token at 0 on every axis is
@@ -130,7 +138,7 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _RotaryFn.apply(turn, positions, q, k)
     xs = [_rows(x) for x in (q, k) if x is not None]
-    ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+    ys = [_like(x) for x in xs]
     _launch(turn, positions, list(zip(xs, ys)))
     return ys[0] if k is None else tuple(ys)
 
