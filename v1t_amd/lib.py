@@ -203,6 +203,13 @@ def stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # current_stream().cuda_stream without the Python object: 0.3 instead of 3 us
+
+
+def stream_of(device: int) -> int:
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 def require_cuda(x: torch.Tensor, what: str) -> None:
     if not x.is_cuda:
         raise RuntimeError(f"v1t_amd {what}: tensor is on {x.device}; the HIP path needs a GPU tensor (no CPU fallback).")
@@ -215,7 +222,7 @@ def leaf_in_capture(x: torch.Tensor, what: str) -> None:
     stream, and a captured pass that finds another stream's mark is refused."""
     if not (x.is_leaf and x.requires_grad):
         return
-    here = torch.cuda.current_stream(x.device).cuda_stream
+    here = stream_of(x.get_device())
     made_on = torch.autograd.graph.get_gradient_edge(x).node.metadata.setdefault("v1t_stream", here)
     if made_on != here and torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"v1t_amd {what}: a graph of an earlier pass over the same leaf tensor is still alive on another stream; its backward cannot be "

@@ -81,8 +81,8 @@ def _orthogonalize(pairs, steps: int, co, eps: float) -> None:
     if not pairs:
         return
     u0 = pairs[0][0]
-    if u0.device.index != torch.cuda.current_device():
-        with torch.cuda.device(u0.device):
+    if u0.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(u0.get_device()):
             return _orthogonalize(pairs, steps, co, eps)
     units = (L.Matrix * len(pairs))()
     for m, (u, o) in zip(units, pairs):
@@ -90,7 +90,7 @@ def _orthogonalize(pairs, steps: int, co, eps: float) -> None:
         m.row_stride, m.col_stride = u.stride()
         m.rows, m.cols = u.shape
     ws = _workspace([tuple(u.shape) for u, _ in pairs], u0.device)
-    _refused(L.load().v1t_orthogonalize(units, len(pairs), _DTYPES[u0.dtype], steps, co, eps, ws.data_ptr(), ws.numel(), L.stream()), "orthogonalize")
+    _refused(L.load().v1t_orthogonalize(units, len(pairs), _DTYPES[u0.dtype], steps, co, eps, ws.data_ptr(), ws.numel(), L.stream_of(u0.get_device())), "orthogonalize")
 
 
 def muon_step(params: t.Sequence[torch.Tensor], grads: t.Sequence[torch.Tensor], moments: t.Sequence[torch.Tensor], *, lr, momentum: float = 0.95,

@@ -6,6 +6,7 @@ and any clip length. `ViTCore` / `CCTCore` run it in every block (`args.rotary`)
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import typing as t
 
 import torch
@@ -64,21 +65,26 @@ def _launch(turn: _Turn, positions: torch.Tensor, pairs_of: t.Sequence[t.Tuple[t
     x0 = pairs_of[0][0]
     if x0.numel() == 0:
         return
-    if x0.device.index != torch.cuda.current_device():
-        with torch.cuda.device(x0.device):
+    device = x0.get_device()
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
             return _launch(turn, positions, pairs_of)
-    four = x0.dim() == 4
-    ops = (L.RotaryOperand * len(pairs_of))()
-    for o, (x, y) in zip(ops, pairs_of):
-        sx, sy = x.stride(), y.stride()
-        o.x, o.y, o.heads, o.y_room = x.data_ptr(), y.data_ptr(), x.shape[-2], 0 if x is y else (x.shape[-1] + 7) // 8 * 8
-        o.xb, o.xt, o.xh = (sx[0], sx[1], sx[2]) if four else (0, sx[0], sx[1])
-        o.yb, o.yt, o.yh = (sy[0], sy[1], sy[2]) if four else (0, sy[0], sy[1])
+    ops = []
+    for x, y in pairs_of:
+        shape, sx, sy = x.shape, x.stride(), y.stride()
+        if len(shape) == 3:
+            shape, sx, sy = (1, *shape), (0, *sx), (0, *sy)
+        ops.append(L.RotaryOperand(x.data_ptr(), y.data_ptr(), *sx[:3], *sy[:3], shape[2], 0 if x is y else (shape[3] + 7) // 8 * 8))
     sp = positions.stride()
-    n = len(turn.sections)
-    L.check(L.load().v1t_rotary(ops, len(pairs_of), _DTYPES[x0.dtype], x0.shape[0] if four else 1, x0.shape[-3], x0.shape[-1], (C.c_int * n)(*turn.sections), n,
-                                turn.base, turn.shared, turn.halves, turn.inverse, positions.data_ptr(), _POSITION_TYPES[positions.dtype],
-                                sp[0] if positions.dim() == 3 else 0, sp[-2], sp[-1], L.stream()), "rotary")
+    n, sections = len(turn.sections), _sections(turn.sections)
+    L.check(L.load().v1t_rotary((L.RotaryOperand * len(ops))(*ops), len(ops), _DTYPES[x0.dtype], shape[0], shape[1], shape[3], sections, n, turn.base, turn.shared,
+                                turn.halves, turn.inverse, positions.data_ptr(), _POSITION_TYPES[positions.dtype], sp[0] if len(sp) == 3 else 0, sp[-2], sp[-1],
+                                L.stream_of(device)), "rotary")
+
+
+@functools.lru_cache(maxsize=64)
+def _sections(sections: t.Tuple[int, ...]):
+    return (C.c_int * len(sections))(*sections)
 
 
 def _like(x: torch.Tensor) -> torch.Tensor:
@@ -113,7 +119,14 @@ class _RotaryFn(torch.autograd.Function):
         back = ctx.turn._replace(inverse=1 - ctx.turn.inverse)
         out: t.List[t.Optional[torch.Tensor]] = [None, None]
         which = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[2 + i]]
-        if len(which) == 2:
+        if not torch.is_grad_enabled():
+            xs = [_rows(grads[i]) for i in which]
+            ys = [_like(x) for x in xs]
+            if which:
+                _launch(back, positions, list(zip(xs, ys)))
+            for i, y in zip(which, ys):
+                out[i] = y
+        elif len(which) == 2:
             out = list(_RotaryFn.apply(back, positions, *grads))
         elif which:
             out[which[0]] = _RotaryFn.apply(back, positions, grads[which[0]], None)
