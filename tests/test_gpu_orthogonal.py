@@ -53,7 +53,7 @@ def update(rows, cols, seed=0, kind="gauss"):
 
 
 SHAPES = [(1, 1), (1, 7), (7, 1), (2, 3), (31, 33), (32, 32), (33, 31), (64, 155), (155, 64), (65, 64), (155, 620), (620, 155), (200, 200), (129, 257), (1, 1000), (1000, 1),
-          (300, 1000), (128, 128), (97, 4096)]
+          (300, 1000), (128, 128), (97, 4096), (64, 448), (64, 449), (449, 60), (31, 1024), (1025, 32), (96, 192), (90, 193), (192, 96), (65, 160), (24, 500)]
 
 
 @pytest.mark.parametrize("rows,cols", SHAPES)

@@ -64,7 +64,7 @@ def ints(*v):
 def test_c_entry_refusals():
     lib = L.load()
     size = lib.v1t_orthogonalize_ws_bytes
-    assert size(ints(4, 7), ints(6, 5), 2) > size(ints(4), ints(6), 1) > 0
+    assert size(ints(400, 700), ints(600, 500), 2) > size(ints(400), ints(600), 1) > size(ints(4), ints(6), 1) > 0
     assert size(None, None, 0) >= 0 and size(None, None, 1) == -1 and size(ints(4), ints(6), -1) == -1
     assert size(ints(0), ints(6), 1) == -1 and size(ints(4), ints(-6), 1) == -1
     assert size(ints(40000), ints(40000), 1) == -2 and size(ints(1), ints(1 << 23), 1) == -2

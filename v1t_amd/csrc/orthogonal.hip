@@ -102,12 +102,13 @@ struct NsMomentum {
 
 DEVFN float ns_sign(float x) { return (float)((x > 0.f) - (x < 0.f)); }
 
-// sum over the workgroup of 256, in a fixed order
+// sum over the workgroup of NT, in a fixed order
+template <int NT = 256>
 DEVFN double ns_block_sum(double v) {
-    __shared__ double s[256];
+    __shared__ double s[NT];
     s[threadIdx.x] = v;
     __syncthreads();
-    for (int o = 128; o > 0; o >>= 1) {
+    for (int o = NT / 2; o > 0; o >>= 1) {
         if ((int)threadIdx.x < o) s[threadIdx.x] += s[threadIdx.x + o];
         __syncthreads();
     }
@@ -587,6 +588,216 @@ __global__ __launch_bounds__(64) void ns_join_kernel(NsTable tab, char* ws, NsSt
     ns_epilogue<TW, KIND, float>(u, w, st, acc, lds, wave >> 1, wave & 1, lane);
 }
 
+// ---- small matrices -----------------------------------------------------------------------
+// A matrix whose planes fit a CU's LDS goes through all its steps in one workgroup: what the products above cost there is their launches (155 x 64:
+// 18 launches, 75 us; this 19). X, A and S lie in LDS as two planes each, rows 16 B longer than their numbers, so that neighbouring rows start in other
+// banks. The waves share the 32 x 32 tiles of A, S and X; a single tile of A
+// is computed in quarters of K by four of them.
+constexpr int NS_LDS = 150 * 1024, NS_PAD = 8, NS_SCRATCH = 4 * 32 * 32 * 4;
+constexpr int ns_small_bytes(int mp, int np) { return 4 * mp * (np + NS_PAD) + 8 * mp * (mp + NS_PAD) + (mp == 32 ? NS_SCRATCH : 0); }
+bool ns_small(int rows, int cols) {
+    const int m = std::min(rows, cols), n = std::max(rows, cols);
+    return m <= 96 && n <= 2048 && ns_small_bytes(round_up(m, 32), round_up(n, 32)) <= NS_LDS;
+}
+
+constexpr int ns_small_threads(int t32) { return t32 == 3 ? 512 : 1024; }
+
+struct NsCoefficients {
+    float c[3 * NS_MAX_STEPS];
+};
+
+template <int T32, typename T, bool MOM>
+__global__ __launch_bounds__(ns_small_threads(T32)) void ns_small_kernel(NsChunk units, NsMomentum mo, NsCoefficients co, int steps, float eps, float scale, int zero) {
+    constexpr int MP = 32 * T32, LDA = MP + NS_PAD, NT = ns_small_threads(T32), WAVES = NT / 64;
+    __shared__ __attribute__((aligned(16))) char lds[NS_LDS];
+    const NsUnit& u = units.u[blockIdx.x];
+    const int LDX = u.np + NS_PAD, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+    f16_t* const X = (f16_t*)lds;             // hi, lo: [MP][LDX]
+    f16_t* const A = X + 2 * MP * LDX;        // hi, lo: [MP][LDA]
+    f16_t* const S = A + 2 * MP * LDA;
+    float* const scratch = (float*)(S + 2 * MP * LDA);
+    const int xlo = MP * LDX, alo = MP * LDA;
+    const float inv = 1.f / scale;            // a power of two
+    const int all = u.rows * u.cols;
+
+    auto row_of = [&](int k) { return u.cols == 1 ? k : (int)__umulhi((unsigned)k, (unsigned)u.part); };  // part: 2^32 / cols, rounded up
+    // the norm (and the momentum), then the planes
+    constexpr int N = 8;
+    auto batch = [&](int k0, NsBatch<T, MOM, N>& b, long long (&src)[N], long long (&at)[N], bool (&on)[N]) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int k = k0 + NT * e + (int)threadIdx.x, row = row_of(k);
+            on[e] = k < all;
+            at[e] = k;
+            src[e] = (long long)row * u.rs + (long long)(k - row * u.cols) * u.cs;
+        }
+        b.load(u, src, at, on);
+    };
+    double sum = 0.0;
+    for (int k0 = 0; k0 < all; k0 += NT * N) {
+        NsBatch<T, MOM, N> b;
+        long long src[N], at[N];
+        bool on[N];
+        batch(k0, b, src, at, on);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            if constexpr (MOM) {
+                b.m[e] = mo.mu * b.m[e] + b.g[e];
+                if (on[e]) u.mom[at[e]] = b.m[e];
+            }
+            const double v = (double)b.update(mo, e);
+            sum += v * v;
+        }
+    }
+    sum = ns_block_sum<NT>(sum);
+    const double mul = (double)scale / (sqrt(sum) + (double)eps);
+    for (int k = threadIdx.x; k < 2 * MP * LDX / 8; k += NT) *(f16x8*)(X + 8 * k) = f16x8{};
+    __syncthreads();
+    for (int k0 = 0; k0 < all; k0 += NT * N) {  // the momentum was written by this thread
+        NsBatch<T, MOM, N> b;
+        long long src[N], at[N];
+        bool on[N];
+        batch(k0, b, src, at, on);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            if (!on[e]) continue;
+            if constexpr (MOM) {
+                if (zero) ((T*)u.in)[src[e]] = (T)0.f;
+            }
+            const int row = row_of((int)at[e]), col = (int)at[e] - row * u.cols, x = u.trans ? col * LDX + row : row * LDX + col;
+            ns_split((float)((double)b.update(mo, e) * mul), X[x], X[xlo + x]);
+        }
+    }
+    __syncthreads();
+
+    auto row_frag = [&](const f16_t* img, int ld, int row0, int k) -> bf16x8 { return *(const bf16x8*)(img + (row0 + r) * ld + k + 8 * h); };
+    auto zeros = [](f32x16& a) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) a[e] = 0.f;
+    };
+    // 4 of a row in two planes
+    auto get = [&](const f16_t* img, int lo, int x, int e) { return (float)img[x + e] + (float)img[lo + x + e]; };
+    auto put = [&](f16_t* img, int lo, int x, const f32x4& v) {
+        f16x4 a, b;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            f16_t p, q;
+            ns_split(v[e], p, q);
+            a[e] = p;
+            b[e] = q;
+        }
+        *(f16x4*)(img + x) = a;
+        *(f16x4*)(img + lo + x) = b;
+    };
+    // tile (ti, tj) of P P^T over k in [k0, k1): i on the lanes, j in the registers
+    auto product = [&](const f16_t* P, int ld, int lo, int ti, int tj, int k0, int k1) {
+        f32x16 acc;
+        zeros(acc);
+#pragma unroll 4
+        for (int k = k0; k < k1; k += 16) {
+            const bf16x8 ph = row_frag(P, ld, 32 * ti, k), pl = row_frag(P + lo, ld, 32 * ti, k);
+            const bf16x8 qh = row_frag(P, ld, 32 * tj, k), ql = row_frag(P + lo, ld, 32 * tj, k);
+            acc = mfma32h(ql, ph, acc);
+            acc = mfma32h(qh, pl, acc);
+            acc = mfma32h(qh, ph, acc);
+        }
+        return acc;
+    };
+    for (int step = 0; step < steps; ++step) {
+        const float a = co.c[3 * step], b = co.c[3 * step + 1], c = co.c[3 * step + 2];
+        if constexpr (T32 == 1) {
+            const int quarter = (u.np / 16 + 3) / 4 * 16;
+            if (wave < 4) {
+                const f32x16 acc = product(X, LDX, xlo, 0, 0, min(u.np, wave * quarter), min(u.np, (wave + 1) * quarter));
+#pragma unroll
+                for (int e = 0; e < 16; ++e) scratch[(wave * 16 + e) * 64 + lane] = acc[e];
+            }
+            __syncthreads();
+            if (wave == 0) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    f32x4 v{};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] += inv * scratch[(w * 16 + 4 * q + e) * 64 + lane];
+                    put(A, alo, r * LDA + 8 * q + 4 * h, v);
+                }
+            }
+        } else {
+            for (int t = wave; t < T32 * T32; t += WAVES) {
+                const f32x16 acc = product(X, LDX, xlo, t / T32, t % T32, 0, u.np);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    put(A, alo, (32 * (t / T32) + r) * LDA + 32 * (t % T32) + 8 * q + 4 * h,
+                        f32x4{inv * acc[4 * q], inv * acc[4 * q + 1], inv * acc[4 * q + 2], inv * acc[4 * q + 3]});
+            }
+        }
+        __syncthreads();
+        for (int t = wave; t < T32 * T32; t += WAVES) {
+            const f32x16 acc = product(A, LDA, alo, t / T32, t % T32, 0, MP);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int x = (32 * (t / T32) + r) * LDA + 32 * (t % T32) + 8 * q + 4 * h;
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = c * inv * acc[4 * q + e] + b * get(A, alo, x, e);
+                put(S, alo, x, v);
+            }
+        }
+        __syncthreads();
+        // tile (i, j) of X: all its tiles are computed before the first is written
+        constexpr int MOST = T32 == 3 ? 3 : 2;  // tiles a wave, at the widest X that fits
+        const int tiles = T32 * (u.np / 32);
+        f32x16 acc[MOST];
+#pragma unroll
+        for (int n = 0; n < MOST; ++n) {
+            const int t = wave + WAVES * n, i = t % T32, j0 = 32 * (t / T32);
+            zeros(acc[n]);
+            if (t < tiles)
+#pragma unroll
+                for (int k = 0; k < MP; k += 16) {
+                    const bf16x8 qh = lds_tr_frag_nat((const bf16_t*)X, LDX, k, j0, lane), ql = lds_tr_frag_nat((const bf16_t*)(X + xlo), LDX, k, j0, lane);
+                    const bf16x8 ph = row_frag(S, LDA, 32 * i, k), pl = row_frag(S + alo, LDA, 32 * i, k);
+                    acc[n] = mfma32h(ql, ph, acc[n]);
+                    acc[n] = mfma32h(qh, pl, acc[n]);
+                    acc[n] = mfma32h(qh, ph, acc[n]);
+                }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < MOST; ++n) {
+            const int t = wave + WAVES * n, i = t % T32, j0 = 32 * (t / T32);
+            if (t < tiles)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int x = (32 * i + r) * LDX + j0 + 8 * q + 4 * h;
+                    f32x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = inv * acc[n][4 * q + e] + a * get(X, xlo, x, e);
+                    put(X, xlo, x, v);
+                }
+        }
+        __syncthreads();
+    }
+    for (int k0 = threadIdx.x; k0 < all; k0 += NT * N) {
+        float wt[N];
+        if (!u.out) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) wt[e] = k0 + NT * e < all ? u.w[k0 + NT * e] : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int k = k0 + NT * e;
+            if (k >= all) continue;
+            const int row = row_of(k), col = k - row * u.cols, x = u.trans ? col * LDX + row : row * LDX + col;
+            const float o = get(X, xlo, x, 0) * inv;
+            if (u.out) ((T*)u.out)[k] = (T)o;
+            else u.w[k] = u.decay * wt[e] - u.lr * o;
+        }
+    }
+}
+
 // no steps: the normalised update itself
 template <typename T>
 __global__ __launch_bounds__(256) void ns_copy_kernel(NsTable tab, const char* ws, float inv) {
@@ -738,7 +949,7 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
 // The exponent of the planes' common scale: 2^15 over the largest number of any plane. A step maps a singular value s in [0, top] to a s + b s^3 + c s^5;
 // X, A = X X^T, S and, where steps are taken in pairs, T, the next A, S' and Q are bounded by their spectral norms. The maxima are sampled, 0.1 % of a
 // singular value and 1 % of the rest are added for what lies between the samples and for rounding.
-bool ns_exponent(const float* coefficients, int steps, bool pairs, int* exponent) {
+bool ns_exponent_of(const float* coefficients, int steps, bool pairs, int* exponent) {
     double top = 1.001, most = top;
     for (int k = 0; k < steps; ++k) {
         const float* f = coefficients + 3 * k;
@@ -765,6 +976,25 @@ bool ns_exponent(const float* coefficients, int steps, bool pairs, int* exponent
     }
     *exponent = (int)std::floor(std::log2(32768.0 / (1.01 * most)));
     return true;
+}
+
+// the same, remembered for the coefficients of the calling thread's last calls (the samples cost more than the launches)
+bool ns_exponent(const float* coefficients, int steps, bool pairs, int* exponent) {
+    struct Known {
+        float c[3 * NS_MAX_STEPS];
+        int steps = -1, exponent = 0;
+        bool ok = false;
+    };
+    static thread_local Known known[2];
+    Known& k = known[pairs];
+    if (k.steps != steps || (steps > 0 && std::memcmp(k.c, coefficients, sizeof(float) * 3 * steps) != 0)) {
+        k.steps = -1;
+        k.ok = ns_exponent_of(coefficients, steps, pairs, &k.exponent);
+        if (steps > 0) std::memcpy(k.c, coefficients, sizeof(float) * 3 * steps);
+        k.steps = steps;
+    }
+    *exponent = k.exponent;
+    return k.ok;
 }
 
 template <int KIND, typename T>
@@ -834,37 +1064,98 @@ int ns_run(const NsLayout& l, int n, char* ws, const NsMomentum& mo, float eps, 
     return ns_steps<T>(l, table, ws, steps, co, pairs, exponent, s);
 }
 
-// lays out the units, checks the workspace, writes the table
-template <typename Shape, typename Fill>
-int ns_begin(int n, Shape shape, Fill fill, void* workspace, long long ws_bytes, NsLayout& l, hipStream_t s) try {
-    NS_TRY(ns_layout(n, shape, [](int, int, NsUnit&) {}, l));
+// the matrices that go through the products, by their numbers
+template <typename Shape>
+std::vector<int> ns_large(int n, Shape shape) {
+    std::vector<int> large;
+    for (int i = 0; i < n; ++i) {
+        int rows, cols;
+        shape(i, rows, cols);
+        if (rows < 1 || cols < 1 || !ns_small(rows, cols)) large.push_back(i);
+    }
+    return large;
+}
+template <typename Shape>
+int ns_layout_large(const std::vector<int>& large, Shape shape, NsLayout& l) {
+    l.bytes = 256;
+    return ns_layout((int)large.size(), [&](int i, int& r, int& c) { shape(large[i], r, c); }, [](int, int, NsUnit&) {}, l);
+}
+
+template <int T32, typename T, bool MOM>
+int ns_launch_small(const NsChunk& c, int k, const NsMomentum& mo, const NsCoefficients& co, int steps, float eps, int exponent, int zero, hipStream_t s) {
+    hipLaunchKernelGGL((ns_small_kernel<T32, T, MOM>), dim3(k), dim3(ns_small_threads(T32)), 0, s, c, mo, co, steps, eps, std::ldexp(1.f, exponent), zero);
+    return hipGetLastError() == hipSuccess ? V1T_OK : V1T_ERR_LAUNCH;
+}
+
+// All of a call: checks, then the small matrices (by their sides: the kernel's tiles), then the table and the products of the large ones
+template <typename T, bool MOM, typename Shape, typename Fill>
+int ns_call(int n, Shape shape, Fill fill, const NsMomentum& mo, float eps, int zero, int steps, const float* co, void* workspace, long long ws_bytes,
+            hipStream_t s) try {
+    if (n > NS_MAX_UNITS) return V1T_ERR_UNSUPPORTED;
+    const std::vector<int> large = ns_large(n, shape);
+    NsLayout l;
+    NS_TRY(ns_layout_large(large, shape, l));
     if (!workspace || ws_bytes < l.bytes) return V1T_ERR_WORKSPACE;
     if ((uintptr_t)workspace & 15) return V1T_ERR_ARG;
+    int exponent = 0;
+    if (!ns_exponent(co, steps, false, &exponent)) return V1T_ERR_ARG;
+    NsCoefficients cs{};
+    for (int i = 0; i < 3 * steps; ++i) cs.c[i] = co[i];
     NsChunk c;
+    for (int t32 = 1; t32 <= 3; ++t32) {
+        int k = 0;
+        for (int i = 0; i <= n; ++i) {
+            NsUnit u{};
+            bool mine = false;
+            if (i < n) {
+                shape(i, u.rows, u.cols);
+                u.m = std::min(u.rows, u.cols); u.n = std::max(u.rows, u.cols);
+                u.mp = round_up(u.m, 32); u.np = round_up(u.n, 32);
+                u.trans = u.rows > u.cols;
+                mine = u.mp == 32 * t32 && ns_small(u.rows, u.cols);
+            }
+            if (mine) {
+                u.part = (int)(u.cols == 1 ? 0 : ((1ull << 32) + u.cols - 1) / u.cols);  // exact: below 2^18 numbers, a rest below 2^11
+                fill(i, u);
+                c.u[k++] = u;
+            }
+            if (k == NS_CHUNK || (i == n && k > 0)) {
+                NS_TRY(t32 == 1 ? (ns_launch_small<1, T, MOM>(c, k, mo, cs, steps, eps, exponent, zero, s))
+                     : t32 == 2 ? (ns_launch_small<2, T, MOM>(c, k, mo, cs, steps, eps, exponent, zero, s))
+                                : (ns_launch_small<3, T, MOM>(c, k, mo, cs, steps, eps, exponent, zero, s)));
+                k = 0;
+            }
+        }
+    }
+    if (large.empty()) return V1T_OK;
     NsUnit* table = (NsUnit*)((char*)workspace + l.table);
+    const int m = (int)large.size();
     int rc = V1T_OK;
     NsLayout again;
-    ns_layout(n, shape, [&](int i, int from, NsUnit& u) {
-        fill(from, u);
+    ns_layout(m, [&](int i, int& r, int& cl) { shape(large[i], r, cl); }, [&](int i, int from, NsUnit& u) {
+        fill(large[from], u);
         c.u[i % NS_CHUNK] = u;
-        if (i % NS_CHUNK == NS_CHUNK - 1 || i == n - 1) {
+        if (i % NS_CHUNK == NS_CHUNK - 1 || i == m - 1) {
             const int k = i % NS_CHUNK + 1;
-            hipLaunchKernelGGL(ns_table_kernel, dim3(1), dim3(256), 0, s, c, k, i - k + 1, n, table, (ns_head*)((char*)workspace + l.heads));
+            hipLaunchKernelGGL(ns_table_kernel, dim3(1), dim3(256), 0, s, c, k, i - k + 1, m, table, (ns_head*)((char*)workspace + l.heads));
             if (hipGetLastError() != hipSuccess) rc = V1T_ERR_LAUNCH;
         }
     }, again);
-    return rc;
+    if (rc != V1T_OK) return rc;
+    return ns_run<T, MOM>(l, m, (char*)workspace, mo, eps, zero, steps, co, s);
 } catch (...) {
-    return V1T_ERR_WORKSPACE;
+    return V1T_ERR_WORKSPACE;  // (the host's own tables: nothing leaves a C entry but a code)
 }
 
 }  // namespace
 
 extern "C" long long v1t_orthogonalize_ws_bytes(const int* rows, const int* cols, int n) {
     if (n < 0 || (n > 0 && (!rows || !cols))) return V1T_ERR_ARG;
-    try {  // (the layout's own tables: nothing leaves a C entry but a code)
+    if (n > NS_MAX_UNITS) return V1T_ERR_UNSUPPORTED;
+    try {
+        auto shape = [&](int i, int& r, int& c) { r = rows[i]; c = cols[i]; };
         NsLayout l;
-        const int rc = ns_layout(n, [&](int i, int& r, int& c) { r = rows[i]; c = cols[i]; }, [](int, int, NsUnit&) {}, l);
+        const int rc = ns_layout_large(ns_large(n, shape), shape, l);
         return rc == V1T_OK ? l.bytes : rc;
     } catch (...) {
         return V1T_ERR_WORKSPACE;
@@ -879,16 +1170,13 @@ extern "C" int v1t_orthogonalize(const v1t_matrix* units, int n, int dtype, int 
     for (int i = 0; i < n; ++i)
         if (!units[i].in || !units[i].out) return V1T_ERR_ARG;
     if (n == 0) return V1T_OK;
-    NsLayout l;
-    hipStream_t s = (hipStream_t)stream;
-    NS_TRY(ns_begin(n, [&](int i, int& r, int& c) { r = units[i].rows; c = units[i].cols; },
-                    [&](int i, NsUnit& u) { u.in = units[i].in; u.out = units[i].out; u.rs = units[i].row_stride; u.cs = units[i].col_stride; },
-                    workspace, ws_bytes, l, s));
+    auto shape = [&](int i, int& r, int& c) { r = units[i].rows; c = units[i].cols; };
+    auto fill = [&](int i, NsUnit& u) { u.in = units[i].in; u.out = units[i].out; u.rs = units[i].row_stride; u.cs = units[i].col_stride; };
     const NsMomentum mo{0.f, 0};
-    char* ws = (char*)workspace;
-    if (dtype == 0) return ns_run<bf16_t, false>(l, n, ws, mo, eps, 0, steps, coefficients, s);
-    if (dtype == 1) return ns_run<f16_t, false>(l, n, ws, mo, eps, 0, steps, coefficients, s);
-    return ns_run<float, false>(l, n, ws, mo, eps, 0, steps, coefficients, s);
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == 0) return ns_call<bf16_t, false>(n, shape, fill, mo, eps, 0, steps, coefficients, workspace, ws_bytes, s);
+    if (dtype == 1) return ns_call<f16_t, false>(n, shape, fill, mo, eps, 0, steps, coefficients, workspace, ws_bytes, s);
+    return ns_call<float, false>(n, shape, fill, mo, eps, 0, steps, coefficients, workspace, ws_bytes, s);
 }
 
 extern "C" int v1t_muon_step(const v1t_muon_range* units, int n, float momentum, int nesterov, int steps, const float* coefficients, float eps, int zero_grad,
@@ -899,13 +1187,10 @@ extern "C" int v1t_muon_step(const v1t_muon_range* units, int n, float momentum,
     for (int i = 0; i < n; ++i)
         if (!units[i].p || !units[i].g || !units[i].m) return V1T_ERR_ARG;
     if (n == 0) return V1T_OK;
-    NsLayout l;
-    hipStream_t s = (hipStream_t)stream;
-    NS_TRY(ns_begin(n, [&](int i, int& r, int& c) { r = units[i].rows; c = units[i].cols; },
-                    [&](int i, NsUnit& u) {
-                        u.in = units[i].g; u.rs = units[i].cols; u.cs = 1; u.mom = units[i].m; u.w = units[i].p;
-                        u.lr = units[i].lr; u.decay = units[i].decay; u.l1 = units[i].l1;
-                    },
-                    workspace, ws_bytes, l, s));
-    return ns_run<float, true>(l, n, (char*)workspace, NsMomentum{momentum, nesterov}, eps, zero_grad, steps, coefficients, s);
+    auto shape = [&](int i, int& r, int& c) { r = units[i].rows; c = units[i].cols; };
+    auto fill = [&](int i, NsUnit& u) {
+        u.in = units[i].g; u.rs = units[i].cols; u.cs = 1; u.mom = units[i].m; u.w = units[i].p;
+        u.lr = units[i].lr; u.decay = units[i].decay; u.l1 = units[i].l1;
+    };
+    return ns_call<float, true>(n, shape, fill, NsMomentum{momentum, nesterov}, eps, zero_grad, steps, coefficients, workspace, ws_bytes, (hipStream_t)stream);
 }

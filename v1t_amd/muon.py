@@ -6,6 +6,7 @@ far, whatever its scale. The products are Newton-Schulz steps, all matrices of a
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 import typing as t
 
@@ -21,17 +22,27 @@ MAX_STEPS = 32
 def _coefficients(coefficients, steps: int) -> t.Any:
     if not 0 <= int(steps) <= MAX_STEPS:
         raise ValueError(f"orthogonalize: 0 to {MAX_STEPS} steps, got {steps}")
-    c = list(coefficients)
+    c = tuple(coefficients)
     if len(c) == 3 and all(isinstance(x, (int, float)) for x in c):
-        c = [c] * steps
+        c = (c,) * int(steps)
     if len(c) != steps or any(len(x) != 3 for x in c):
         raise ValueError(f"orthogonalize: coefficients are (a, b, c) or one such triple for each of the {steps} steps")
-    return (C.c_float * max(1, 3 * steps))(*[float(v) for x in c for v in x])
+    return _floats(tuple(float(v) for x in c for v in x))
+
+
+@functools.lru_cache(maxsize=32)
+def _floats(values: t.Tuple[float, ...]):
+    return (C.c_float * max(1, len(values)))(*values)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(shapes: t.Tuple[t.Tuple[int, int], ...]) -> int:
+    n = len(shapes)
+    return int(L.load().v1t_orthogonalize_ws_bytes((C.c_int * n)(*[r for r, _ in shapes]), (C.c_int * n)(*[c for _, c in shapes]), n))
 
 
 def _workspace(shapes: t.Sequence[t.Tuple[int, int]], device) -> torch.Tensor:
-    n = len(shapes)
-    nbytes = int(L.load().v1t_orthogonalize_ws_bytes((C.c_int * n)(*[r for r, _ in shapes]), (C.c_int * n)(*[c for _, c in shapes]), n))
+    nbytes = _workspace_bytes(tuple(shapes))
     L.check(min(nbytes, 0), "orthogonalize")
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
