@@ -504,30 +504,30 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(NsTable t
         for (int j = 0; j < TW; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    auto compute = [&](int buf) {
+    // a stage's fragments: [K half][plane][32-block]
+    struct Frags {
+        bf16x8 ph[TW], pl[TW], qh[TW], ql[TW];
+    };
+    auto read = [&](Frags& f, int buf, int s) {
         const f16_t* img = lds + buf * 4 * PL;
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            bf16x8 ph[TW], pl[TW], qh[TW], ql[TW];
-#pragma unroll
-            for (int i = 0; i < TW; ++i) {
-                ph[i] = row_frag(img, 32 * (TW * wi + i), s);
-                pl[i] = row_frag(img + PL, 32 * (TW * wi + i), s);
-                if constexpr (TR) {
-                    qh[i] = col_frag(img + 2 * PL, 32 * (TW * wj + i), s);
-                    ql[i] = col_frag(img + 3 * PL, 32 * (TW * wj + i), s);
-                } else {
-                    qh[i] = row_frag(img + 2 * PL, 32 * (TW * wj + i), s);
-                    ql[i] = row_frag(img + 3 * PL, 32 * (TW * wj + i), s);
-                }
-            }
-#pragma unroll
-            for (int x = 0; x < 3; ++x)
-#pragma unroll
-                for (int i = 0; i < TW; ++i)
-#pragma unroll
-                    for (int j = 0; j < TW; ++j) acc[i][j] = mfma32h(x == 0 ? ql[j] : qh[j], x == 1 ? pl[i] : ph[i], acc[i][j]);
+        for (int i = 0; i < TW; ++i) {
+            f.ph[i] = row_frag(img, 32 * (TW * wi + i), s);
+            f.ql[i] = TR ? col_frag(img + 3 * PL, 32 * (TW * wj + i), s) : row_frag(img + 3 * PL, 32 * (TW * wj + i), s);
         }
+#pragma unroll
+        for (int i = 0; i < TW; ++i) {
+            f.qh[i] = TR ? col_frag(img + 2 * PL, 32 * (TW * wj + i), s) : row_frag(img + 2 * PL, 32 * (TW * wj + i), s);
+            f.pl[i] = row_frag(img + PL, 32 * (TW * wi + i), s);
+        }
+    };
+    auto multiply = [&](const Frags& f) {
+#pragma unroll
+        for (int x = 0; x < 3; ++x)
+#pragma unroll
+            for (int i = 0; i < TW; ++i)
+#pragma unroll
+                for (int j = 0; j < TW; ++j) acc[i][j] = mfma32h(x == 0 ? f.ql[j] : f.qh[j], x == 2 ? f.pl[i] : f.ph[i], acc[i][j]);
     };
     // every wave issues 4 PIECES operations per stage: "all but the newest NST - 2 stages have landed" is one counted wait
 #pragma unroll
@@ -538,8 +538,20 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(NsTable t
         if (t + NST - 1 <= nk) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * PIECES * (NST - 2)) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();  // stage t is there for all; the stage before it has been read by all
+        Frags f0, f1;
+        read(f0, buf, 0);
         if (t + NST - 1 < nk) issue(t + NST - 1, buf == 0 ? NST - 1 : buf - 1);
-        compute(buf);
+        // the second half's reads go out between the first half's products
+        read(f1, buf, 1);
+        multiply(f0);
+        multiply(f1);
+        constexpr int READS = TR ? 6 * TW : 4 * TW, MF = 3 * TW * TW;
+#pragma unroll
+        for (int x = 0; x < (READS < MF ? READS : MF); ++x) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, READS > MF ? 2 : 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * MF, 0);
         buf = buf + 1 == NST ? 0 : buf + 1;
     }
     if (piece) {  // its sums in the accumulators' order; ns_join_kernel adds the pieces up
