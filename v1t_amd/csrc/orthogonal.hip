@@ -39,7 +39,7 @@ struct NsUnit {
     void* out;        // the result, or nullptr: w is updated
     float *mom, *w;
     long long rs, cs;                // element strides of `in`; out, mom and w are row-major without gaps
-    long long x[2], sq[4];           // byte offsets of the planes in the workspace (hi, and lo behind it): X twice, the m x m matrices
+    long long x[2], sq[4];           // byte offsets in the workspace: X twice, the m x m matrices
     int rows, cols, m, n, mp, np, trans;
     int part, part0, nparts, prep0;  // elements per partial sum; first workgroup of this unit in the launches of each kind
     int first[3];                    // first tile in the products' launches: gram, poly, apply / last
@@ -177,6 +177,11 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsTable tab, NsMomentum mo
     if (threadIdx.x == 0) parts[blockIdx.x] = sum;
 }
 
+// A matrix in the workspace, rows x ld (multiples of 32): 32 numbers of a row lie as 64 fp16, their 32 hi in front of their 32 lo, so that the 32 numbers of a row that a K step
+// reads are one line of 128 B. Where number (i, j)'s hi lies; its lo is 32 behind
+DEVFN size_t ns_at(int i, int j, int ld) { return (size_t)i * (2 * ld) + (j >> 5) * 64 + (j & 31); }
+constexpr int NS_LO = 32;
+
 DEVFN void ns_split(float v, f16_t& hi, f16_t& lo) {
     hi = (f16_t)v;
     lo = (f16_t)(v - (float)hi);
@@ -220,8 +225,7 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(NsTable tab, NsMomentum mo
         }
     }
     __syncthreads();
-    f16_t* hi = (f16_t*)(ws + u.x[0]);
-    f16_t* lo = hi + (size_t)u.mp * u.np;
+    f16_t* const X = (f16_t*)(ws + u.x[0]);
     for (int k = threadIdx.x; k < NS_TILE_PREP * NS_TILE_PREP / 8; k += 256) {
         const int i = k / (NS_TILE_PREP / 8), j = 8 * (k % (NS_TILE_PREP / 8));
         if (i0 + i >= u.mp || j0 + j >= u.np) continue;  // np is a multiple of 32: groups of 8 are whole
@@ -233,8 +237,9 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(NsTable tab, NsMomentum mo
             h[e] = a;
             l[e] = b;
         }
-        *(f16x8*)(hi + (size_t)(i0 + i) * u.np + j0 + j) = h;
-        *(f16x8*)(lo + (size_t)(i0 + i) * u.np + j0 + j) = l;
+        f16_t* to = X + ns_at(i0 + i, j0 + j, u.np);
+        *(f16x8*)to = h;
+        *(f16x8*)(to + NS_LO) = l;
     }
 }
 
@@ -265,18 +270,18 @@ typedef f16_t f16x4 __attribute__((ext_vector_type(4)));
 
 template <int TW>
 struct NsTile {
-    static constexpr int B = 64 * TW, PL = B * NS_BK, SIDE = 32 * TW;
-    static constexpr int PIECES = PL * 2 / 1024 / 4;      // LDS-DMA instructions per wave and plane: one per 64 rows
+    static constexpr int B = 64 * TW, PL = 2 * B * NS_BK, SIDE = 32 * TW;  // PL: elements of an operand's stage, hi and lo
+    static constexpr int PIECES = PL * 2 / 1024 / 4;      // LDS-DMA instructions per wave and operand
     static constexpr int NST = TW == 1 ? 4 : TW == 2 ? 2 : 3;
-    static constexpr int LDS = NST * 4 * PL;              // elements; the epilogue's fp32 tile fits
+    static constexpr int LDS = NST * 2 * PL;              // elements; the epilogue's fp32 tile fits
     static_assert(4 * SIDE * SIDE * 4 <= LDS * 2, "epilogue");
 };
 
 // where a tile lies and what it reads and writes
 struct NsWhere {
     int bi, bj, i0, j0;
-    const f16_t *D, *Dl, *D2, *D2l;
-    f16_t *C, *Cl;
+    const f16_t *D, *D2;
+    f16_t* C;
     int ldd, cols;
 };
 template <int TW, int KIND>
@@ -296,14 +301,10 @@ DEVFN NsWhere ns_where(const NsUnit& u, char* ws, const NsStep& st, int t) {  //
     }
     w.i0 = w.bi * B;
     w.j0 = w.bj * B;
-    const size_t xlo = (size_t)u.mp * u.np, alo = (size_t)u.mp * u.mp;
     w.D = KIND == NS_SQUARE ? (const f16_t*)(ws + u.sq[st.d]) : (const f16_t*)(ws + u.x[st.from]);
-    w.Dl = w.D + (KIND == NS_SQUARE ? alo : xlo);
     w.D2 = (const f16_t*)(ws + u.sq[st.d2]);
-    w.D2l = w.D2 + alo;
     w.ldd = KIND == NS_SQUARE ? u.mp : u.np;
     w.C = (f16_t*)(ws + (KIND == NS_GRAM ? u.sq[0] : KIND == NS_SQUARE ? u.sq[st.out] : u.x[st.from ^ 1]));
-    w.Cl = w.C + (SYM ? alo : xlo);
     w.cols = SYM ? u.mp : u.np;
     return w;
 }
@@ -335,7 +336,8 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
         if (i >= u.mp || j >= w.cols) continue;  // both are multiples of 32: groups of 8 are whole
         f32x4 v0 = *(const f32x4*)(img + chunk(il, jl / 4)), v1 = *(const f32x4*)(img + chunk(il, jl / 4 + 1));
         if constexpr (KIND != NS_GRAM) {
-            const f16x8 dh = *(const f16x8*)(w.D + (size_t)i * w.ldd + j), dl = *(const f16x8*)(w.Dl + (size_t)i * w.ldd + j);
+            const f16_t* d = w.D + ns_at(i, j, w.ldd);
+            const f16x8 dh = *(const f16x8*)d, dl = *(const f16x8*)(d + NS_LO);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 v0[e] += st.beta * ((float)dh[e] + (float)dl[e]);
@@ -344,7 +346,8 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
         }
         if constexpr (KIND == NS_SQUARE) {
             if (st.beta2 != 0.f) {
-                const f16x8 dh = *(const f16x8*)(w.D2 + (size_t)i * w.ldd + j), dl = *(const f16x8*)(w.D2l + (size_t)i * w.ldd + j);
+                const f16_t* d = w.D2 + ns_at(i, j, w.ldd);
+                const f16x8 dh = *(const f16x8*)d, dl = *(const f16x8*)(d + NS_LO);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     v0[e] += st.beta2 * ((float)dh[e] + (float)dl[e]);
@@ -366,8 +369,9 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
                 ch[e] = a;
                 cl[e] = b;
             }
-            *(f16x8*)(w.C + (size_t)i * w.cols + j) = ch;
-            *(f16x8*)(w.Cl + (size_t)i * w.cols + j) = cl;
+            f16_t* to = w.C + ns_at(i, j, w.cols);
+            *(f16x8*)to = ch;
+            *(f16x8*)(to + NS_LO) = cl;
         }
         if (KIND == NS_LAST || (KIND == NS_SQUARE && mirror)) {
             *(f32x4*)(img + chunk(il, jl / 4)) = v0;
@@ -389,8 +393,9 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
                 ch[e] = a;
                 cl[e] = b;
             }
-            *(f16x8*)(w.C + (size_t)j * w.cols + i) = ch;
-            *(f16x8*)(w.Cl + (size_t)j * w.cols + i) = cl;
+            f16_t* to = w.C + ns_at(j, i, w.cols);
+            *(f16x8*)to = ch;
+            *(f16x8*)(to + NS_LO) = cl;
         }
     } else if constexpr (KIND == NS_LAST) {
         constexpr int N = 8;
@@ -445,28 +450,26 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(NsTable t
     const f16_t* X = (const f16_t*)(ws + u.x[st.from]);
     const f16_t* P = KIND == NS_GRAM ? X : (const f16_t*)(ws + u.sq[st.p]);
     const f16_t* Q = KIND == NS_SQUARE ? (const f16_t*)(ws + u.sq[st.q]) : X;
-    const size_t xlo = (size_t)u.mp * u.np, alo = (size_t)u.mp * u.mp;
     const int ldp = KIND == NS_GRAM ? u.np : u.mp, ldq = KIND == NS_SQUARE ? u.mp : u.np;
-    const size_t plo = KIND == NS_GRAM ? xlo : alo, qlo = KIND == NS_SQUARE ? alo : xlo;
 
-    // A 1-KB piece fills 64 16-B chunks of a plane in order; which 16 B of the tile's row a chunk holds is swizzled, so that the fragment reads below spread over
-    // all banks. Rows [.][32]: four chunks a row, chunk c at c ^ (row / 4 % 4). Q as [k][j], B / 8 chunks a row: c ^ 4 (k % 4) - B = 64, where two rows fill
-    // the 64 banks: c ^ 4 (k / 2 % 2). A lane's byte offset from the tile's first row is loop-invariant; piece p of a wave goes by the instruction's offset, which
-    // moves the LDS and the global address alike: the lane offset carries 1024 p less, the base 2048 less.
+    // A 1-KB piece fills 64 16-B chunks of a stage in order; which 16 B of the tile's row a chunk holds is swizzled, so that the fragment reads below spread over all
+    // 64 banks. Rows [.][32 hi, 32 lo]: eight chunks a row, chunk c at c ^ (row / 2 % 8). Q as [k][j]: the row's 64-B granules (32 hi or lo) g at g ^ (k % 4). A lane's
+    // byte offset from the tile's first row is loop-invariant; pieces 1 .. 3 of a group of four go by the instruction's offset, which moves the LDS and the global
+    // address alike: the lane offset carries 1024 (p % 4) less, the base 3072 less.
     unsigned po[PIECES], qo[PIECES];
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-        const int c = 64 * (wave * PIECES + p) + lane;
-        po[p] = (unsigned)min(c / 4, u.mp - 1 - w.i0) * (unsigned)(2 * ldp) + 16 * ((c & 3) ^ (c >> 4 & 3)) + 2048 - 1024 * p;
+        const int c = 64 * (wave * PIECES + p) + lane, row = c / 8, at = 3072 - 1024 * (p & 3) + 16 * ((c & 7) ^ (row >> 1 & 7));
+        po[p] = (unsigned)min(row, u.mp - 1 - w.i0) * (unsigned)(4 * ldp) + at;
         if constexpr (TR) {
-            const int k = c / (B / 8), cc = (c % (B / 8)) ^ (B == 64 ? (k >> 1 & 1) << 2 : (k & 3) << 2);
-            qo[p] = (unsigned)k * (unsigned)(2 * ldq) + 2 * min(8 * cc, u.np - 8 - w.j0) + 2048 - 1024 * p;
+            const int k = c / (B / 4), g = (c % (B / 4) / 4) ^ (k & 3);  // B / 4 chunks a row; granules past the matrix' columns re-read its last block
+            qo[p] = (unsigned)k * (unsigned)(4 * ldq) + 64 * min(g, (u.np - w.j0) / 16 - 2 + (g & 1)) + 16 * (c & 3) + 3072 - 1024 * (p & 3);
         } else {
-            qo[p] = (unsigned)min(c / 4, u.mp - 1 - w.j0) * (unsigned)(2 * ldq) + 16 * ((c & 3) ^ (c >> 4 & 3)) + 2048 - 1024 * p;
+            qo[p] = (unsigned)min(row, u.mp - 1 - w.j0) * (unsigned)(4 * ldq) + at;
         }
     }
-    const char* pb = (const char*)(P + (size_t)w.i0 * ldp) - 2048;
-    const char* qb = (const char*)(TR ? Q + w.j0 : Q + (size_t)w.j0 * ldq) - 2048;
+    const char* pb = (const char*)(P + (size_t)w.i0 * (2 * ldp)) - 3072;
+    const char* qb = (const char*)(TR ? Q + 2 * w.j0 : Q + (size_t)w.j0 * (2 * ldq)) - 3072;
     const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)lds);
     auto uniform = [](const char* p) {
         const unsigned long long b = (unsigned long long)(uintptr_t)p;
@@ -474,26 +477,31 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(NsTable t
         return (const char*)(uintptr_t)(((unsigned long long)hi << 32) | lo);
     };
     auto issue = [&](int t, int buf) {
-        const size_t pk = (size_t)(t0 + t) * (2 * NS_BK), qk = TR ? (size_t)(t0 + t) * (2 * NS_BK) * ldq : (size_t)(t0 + t) * (2 * NS_BK);
+        const size_t pk = (size_t)(t0 + t) * (4 * NS_BK), qk = TR ? (size_t)(t0 + t) * NS_BK * (4 * ldq) : pk;
 #pragma unroll
-        for (int plane = 0; plane < 4; ++plane) {
-            const char* base = uniform(plane == 0 ? pb + pk : plane == 1 ? pb + pk + 2 * plo : plane == 2 ? qb + qk : qb + qk + 2 * qlo);
-            const unsigned m0 = lds0 + 2u * (unsigned)((buf * 4 + plane) * PL) + 1024u * (unsigned)(wave * PIECES);
-            const unsigned* o = plane < 2 ? po : qo;
-            TileDma<32, 32>::template group<PIECES>(base, m0, o[0], o[PIECES > 1 ? 1 : 0], o[PIECES > 2 ? 2 : 0], 0);
+        for (int side = 0; side < 2; ++side) {
+            const char* base = uniform(side ? qb + qk : pb + pk);
+            const unsigned* o = side ? qo : po;
+#pragma unroll
+            for (int p = 0; p < PIECES; p += 4) {
+                constexpr int LAST = PIECES % 4 ? PIECES % 4 : 4;
+                const unsigned m0 = lds0 + 2u * (unsigned)((buf * 2 + side) * PL) + 1024u * (unsigned)(wave * PIECES + p);
+                auto at = [&](int x) { return o[p + x < PIECES ? p + x : PIECES - 1]; };
+                if (p + 4 <= PIECES) TileDma<32, 32>::template group<4>(base, m0, at(0), at(1), at(2), at(3));
+                else TileDma<32, 32>::template group<LAST>(base, m0, at(0), at(1), at(2), at(3));
+            }
         }
     };
 
     const int r = lane & 31, h = lane >> 5;
-    auto row_frag = [&](const f16_t* img, int row0, int s) -> bf16x8 {  // rows row0 + (lane & 31), k = 16 s + 8 h ..
-        return *(const bf16x8*)(img + (row0 + r) * NS_BK + 8 * ((2 * s + h) ^ (r >> 2 & 3)));
+    auto row_frag = [&](const f16_t* img, int row0, int s, int lo) -> bf16x8 {  // rows row0 + (lane & 31), k = 16 s + 8 h ..
+        return *(const bf16x8*)(img + (row0 + r) * (2 * NS_BK) + 8 * ((4 * lo + 2 * s + h) ^ (r >> 1 & 7)));
     };
     const int tg = lane >> 4, tq = lane >> 2 & 3, tp = lane & 3;
-    auto col_frag = [&](const f16_t* img, int col0, int s) -> bf16x8 {  // columns col0 + (lane & 31), the same k
-        const int k = 16 * s + 8 * (tg >> 1) + tq;
-        const int c = (col0 / 8 + 2 * (tg & 1) + (tp >> 1)) ^ (B == 64 ? (tq >> 1) << 2 : tq << 2);
-        const bf16_t* a = (const bf16_t*)img + k * B + 8 * c + 4 * (tp & 1);
-        const bf16x4 x = lds_tr_read(a), y = lds_tr_read(a + 4 * B);
+    auto col_frag = [&](const f16_t* img, int col0, int s, int lo) -> bf16x8 {  // columns col0 + (lane & 31), the same k
+        const int k = 16 * s + 8 * (tg >> 1) + tq, g = (col0 / 16 + lo) ^ tq;
+        const bf16_t* a = (const bf16_t*)img + k * (2 * B) + 32 * g + 16 * (tg & 1) + 4 * tp;
+        const bf16x4 x = lds_tr_read(a), y = lds_tr_read(a + 4 * (2 * B));
         return bf16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
     };
 
@@ -509,16 +517,17 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(NsTable t
         bf16x8 ph[TW], pl[TW], qh[TW], ql[TW];
     };
     auto read = [&](Frags& f, int buf, int s) {
-        const f16_t* img = lds + buf * 4 * PL;
+        const f16_t *p = lds + buf * 2 * PL, *q = p + PL;
+        auto other = [&](int i, int lo) { return TR ? col_frag(q, 32 * (TW * wj + i), s, lo) : row_frag(q, 32 * (TW * wj + i), s, lo); };
 #pragma unroll
         for (int i = 0; i < TW; ++i) {
-            f.ph[i] = row_frag(img, 32 * (TW * wi + i), s);
-            f.ql[i] = TR ? col_frag(img + 3 * PL, 32 * (TW * wj + i), s) : row_frag(img + 3 * PL, 32 * (TW * wj + i), s);
+            f.ph[i] = row_frag(p, 32 * (TW * wi + i), s, 0);
+            f.ql[i] = other(i, 1);
         }
 #pragma unroll
         for (int i = 0; i < TW; ++i) {
-            f.qh[i] = TR ? col_frag(img + 2 * PL, 32 * (TW * wj + i), s) : row_frag(img + 2 * PL, 32 * (TW * wj + i), s);
-            f.pl[i] = row_frag(img + PL, 32 * (TW * wi + i), s);
+            f.qh[i] = other(i, 0);
+            f.pl[i] = row_frag(p, 32 * (TW * wi + i), s, 1);
         }
     };
     auto multiply = [&](const Frags& f) {
@@ -529,30 +538,56 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(NsTable t
 #pragma unroll
                 for (int j = 0; j < TW; ++j) acc[i][j] = mfma32h(x == 0 ? f.ql[j] : f.qh[j], x == 2 ? f.pl[i] : f.ph[i], acc[i][j]);
     };
-    // every wave issues 4 PIECES operations per stage: "all but the newest NST - 2 stages have landed" is one counted wait
-#pragma unroll
-    for (int t = 0; t < NST - 1; ++t)
-        if (t < nk) issue(t, t);
-    int buf = 0;
-    for (int t = 0; t < nk; ++t) {
-        if (t + NST - 1 <= nk) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * PIECES * (NST - 2)) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();  // stage t is there for all; the stage before it has been read by all
-        Frags f0, f1;
-        read(f0, buf, 0);
-        if (t + NST - 1 < nk) issue(t + NST - 1, buf == 0 ? NST - 1 : buf - 1);
-        // the second half's reads go out between the first half's products
-        read(f1, buf, 1);
-        multiply(f0);
-        multiply(f1);
-        constexpr int READS = TR ? 6 * TW : 4 * TW, MF = 3 * TW * TW;
+    // every wave issues 2 PIECES operations per stage: "all but the newest stages have landed" is one counted wait
+    constexpr int READS = TR ? 6 * TW : 4 * TW, MF = 3 * TW * TW;
+    // the next fragments' reads go out between the products of the last
+    auto interleave = [] {
 #pragma unroll
         for (int x = 0; x < (READS < MF ? READS : MF); ++x) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, READS > MF ? 2 : 1, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, 2 * MF, 0);
-        buf = buf + 1 == NST ? 0 : buf + 1;
+        __builtin_amdgcn_sched_group_barrier(0x008, MF, 0);
+    };
+#pragma unroll
+    for (int t = 0; t < NST - 1; ++t)
+        if (t < nk) issue(t, t);
+    int buf = 0;
+    if constexpr (TW < 3) {
+        for (int t = 0; t < nk; ++t) {
+            if (t + NST - 1 <= nk) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PIECES * (NST - 2)) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();  // stage t is there for all; the stage before it has been read by all
+            Frags f0, f1;
+            read(f0, buf, 0);
+            if (t + NST - 1 < nk) issue(t + NST - 1, buf == 0 ? NST - 1 : buf - 1);
+            read(f1, buf, 1);
+            multiply(f0);
+            multiply(f1);
+            interleave();
+            buf = buf + 1 == NST ? 0 : buf + 1;
+        }
+    } else if (nk > 0) {
+        // one wave a SIMD: nothing else covers a wait, so fragments are read across the barrier, too. In the middle of stage t, when its second half has been read,
+        // stage t + 1 is waited for and its first half read between the products of t's second
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        Frags f0, f1;
+        read(f0, 0, 0);
+        for (int t = 0; t < nk; ++t) {
+            const int next = buf + 1 == NST ? 0 : buf + 1;
+            if (t + 2 < nk) issue(t + 2, next + 1 == NST ? 0 : next + 1);  // the buffer of stage t - 1: read by all before the barrier below, an iteration ago
+            read(f1, buf, 1);
+            multiply(f0);
+            interleave();
+            if (t + 2 < nk) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PIECES) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (t + 1 < nk) read(f0, next, 0);
+            multiply(f1);
+            interleave();
+            buf = next;
+        }
     }
     if (piece) {  // its sums in the accumulators' order; ns_join_kernel adds the pieces up
         float* to = st.slab + ((size_t)over * 4 + wave) * (TW * TW * 1024) + 4 * lane;
@@ -817,13 +852,13 @@ __global__ __launch_bounds__(256) void ns_copy_kernel(NsTable tab, const char* w
     const NsUnit& u = tab.units[ns_find<4>(tab, blockIdx.x, head)];
     const int tj = (u.np + NS_TILE_PREP - 1) / NS_TILE_PREP, t = blockIdx.x - u.prep0;
     const int i0 = t / tj * NS_TILE_PREP, j0 = t % tj * NS_TILE_PREP;
-    const f16_t* hi = (const f16_t*)(ws + u.x[0]);
-    const f16_t* lo = hi + (size_t)u.mp * u.np;
+    const f16_t* X = (const f16_t*)(ws + u.x[0]);
     for (int k = threadIdx.x; k < NS_TILE_PREP * NS_TILE_PREP; k += 256) {
         const int i = i0 + k / NS_TILE_PREP, j = j0 + k % NS_TILE_PREP;
         if (i >= u.m || j >= u.n) continue;
         const long long at = u.trans ? (long long)j * u.cols + i : (long long)i * u.cols + j;
-        const float o = ((float)hi[(size_t)i * u.np + j] + (float)lo[(size_t)i * u.np + j]) * inv;
+        const f16_t* from = X + ns_at(i, j, u.np);
+        const float o = ((float)from[0] + (float)from[NS_LO]) * inv;
         if (u.out) ((T*)u.out)[at] = (T)o;
         else u.w[at] = u.decay * u.w[at] - u.lr * o;
     }
@@ -855,24 +890,24 @@ long long ns_align(long long x) { return (x + 255) / 256 * 256; }
 // either tile. Measured, us per K step: the larger tile 1.6 with two on a CU and 0.9 alone, the smaller 0.85 and 0.25 (so the larger does twice
 // the work in a time, where there is enough of it), their epilogues 5 and 1.5; the launch that joins pieces 6, and their sums at 3 TB/s. Only the tiles of the last, part-filled round
 // are split, in pieces of at least 4 steps.
-NsPlan ns_plan(long long t64, long long k64, long long t128, long long k128, bool may_split) {
-    constexpr int SLOTS = 512, CUS = 256;
+NsPlan ns_plan(const long long (&t)[3], const long long (&k)[3], bool may_split) {
+    constexpr int CUS = 256;
+    constexpr double FULL[3] = {0.85, 1.6, 1.6}, ALONE[3] = {0.25, 0.9, 1.6}, TAIL[3] = {1.5, 5.0, 9.0};
     NsPlan best;
     double least = 1e30;
-    for (int tw = 1; tw <= 2; ++tw) {
-        const long long tiles = tw == 1 ? t64 : t128;
-        const double steps = (double)(tw == 1 ? k64 : k128) / (double)tiles;
-        const double full = tw == 1 ? 0.85 : 1.6, alone = tw == 1 ? 0.25 : 0.9;
+    for (int tw = 1; tw <= 3; ++tw) {
+        const int slots = tw == 3 ? CUS : 2 * CUS;
+        const long long tiles = t[tw - 1];
+        const double steps = (double)k[tw - 1] / (double)tiles;
+        auto round = [&](double k, long long w) { return w == 0 ? 0.0 : TAIL[tw - 1] + k * (w <= CUS ? ALONE : FULL)[tw - 1]; };
         for (int split = 1; split <= (may_split ? 16 : 1); ++split) {
-            const long long whole = split == 1 ? tiles : tiles / SLOTS * SLOTS, rest = tiles - whole, pieces = rest * split;
-            if (split > 1 && (rest == 0 || pieces > SLOTS || steps < 4 * split)) continue;
-            const double tail = tw == 1 ? 1.5 : 5.0;
-            auto round = [&](double k, long long w) { return w == 0 ? 0.0 : tail + k * (w <= CUS ? alone : full); };
-            double t = (double)(whole / SLOTS) * round(steps, SLOTS) + round(steps, whole % SLOTS);
-            if (split > 1) t += round(steps / split, pieces) + 6.0 + (double)pieces * tw * tw * 16384.0 * 2.0 / 3e6;
-            if (t < least) {
-                least = t;
-                best.us = t; best.tw = tw; best.tiles = (int)tiles; best.whole = (int)whole; best.split = split;
+            const long long whole = split == 1 ? tiles : tiles / slots * slots, rest = tiles - whole, pieces = rest * split;
+            if (split > 1 && (rest == 0 || pieces > slots || steps < 4 * split)) continue;
+            double us = (double)(whole / slots) * round(steps, slots) + round(steps, whole % slots);
+            if (split > 1) us += round(steps / split, pieces) + 6.0 + (double)pieces * tw * tw * 16384.0 * 2.0 / 3e6;
+            if (us < least) {
+                least = us;
+                best.us = us; best.tw = tw; best.tiles = (int)tiles; best.whole = (int)whole; best.split = split;
             }
         }
     }
@@ -884,7 +919,7 @@ template <typename Shape, typename Put>
 int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
     if (n > NS_MAX_UNITS) return V1T_ERR_UNSUPPORTED;
     long long nparts = 0, prep = 0;
-    long long gt[2] = {}, gk[2] = {}, pk[2] = {}, ft[2] = {}, fk[2] = {};  // tiles and K steps: 64, 128
+    long long gt[3] = {}, gk[3] = {}, pk[3] = {}, ft[3] = {}, fk[3] = {};  // tiles and K steps: 64, 128, 192
     std::vector<int> order(n);
     std::vector<std::pair<int, int>> size(n);
     for (int i = 0; i < n; ++i) {
@@ -895,8 +930,8 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
         if (m > 32768 || nn > (1 << 22) || m * nn > (1ll << 31)) return V1T_ERR_UNSUPPORTED;
         size[i] = {(int)nn, (int)m};
         order[i] = i;
-        for (int k = 0; k < 2; ++k) {
-            const long long B = 64 << k, mp = round_up((int)m, NS_BK), np = round_up((int)nn, NS_BK), a = (mp + B - 1) / B, b = (np + B - 1) / B;
+        for (int k = 0; k < 3; ++k) {
+            const long long B = 64 * (k + 1), mp = round_up((int)m, NS_BK), np = round_up((int)nn, NS_BK), a = (mp + B - 1) / B, b = (np + B - 1) / B;
             gt[k] += a * (a + 1) / 2; gk[k] += a * (a + 1) / 2 * (np / NS_BK); pk[k] += a * (a + 1) / 2 * (mp / NS_BK);
             ft[k] += a * b; fk[k] += a * b * (mp / NS_BK);
         }
@@ -907,9 +942,9 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
     if (n == 0) return V1T_OK;
     // the tiles with the longest K first: what is left for the last round is short
     std::sort(order.begin(), order.end(), [&](int a, int b) { return size[a] != size[b] ? size[a] > size[b] : a < b; });
-    l.gram = ns_plan(gt[0], gk[0], gt[1], gk[1], true);
-    l.poly = ns_plan(gt[0], pk[0], gt[1], pk[1], true);
-    l.full = ns_plan(ft[0], fk[0], ft[1], fk[1], false);
+    l.gram = ns_plan(gt, gk, true);
+    l.poly = ns_plan(gt, pk, true);
+    l.full = ns_plan(ft, fk, false);
     // two steps: gram, poly, full each twice, or gram, five m x m products, full; 3 us a launch
     l.pairs = l.gram.us + 5 * l.poly.us + l.full.us + 21.0 < 0.9 * (2 * (l.gram.us + l.poly.us + l.full.us) + 18.0);
     l.table = 0;
@@ -1013,11 +1048,13 @@ template <int KIND, typename T>
 int ns_gemm(const NsLayout& l, const NsTable& table, char* ws, NsStep st, hipStream_t s) {
     const NsPlan& p = KIND == NS_GRAM ? l.gram : KIND == NS_SQUARE ? l.poly : l.full;
     st.whole = p.whole; st.split = p.split; st.slab = (float*)(ws + l.slab);
-    if (p.tw == 2) hipLaunchKernelGGL((ns_gemm_kernel<2, KIND, T>), dim3(p.grid()), dim3(256), 0, s, table, ws, st);
+    if (p.tw == 3) hipLaunchKernelGGL((ns_gemm_kernel<3, KIND, T>), dim3(p.grid()), dim3(256), 0, s, table, ws, st);
+    else if (p.tw == 2) hipLaunchKernelGGL((ns_gemm_kernel<2, KIND, T>), dim3(p.grid()), dim3(256), 0, s, table, ws, st);
     else hipLaunchKernelGGL((ns_gemm_kernel<1, KIND, T>), dim3(p.grid()), dim3(256), 0, s, table, ws, st);
     if constexpr (KIND == NS_GRAM || KIND == NS_SQUARE)
         if (p.joined()) {
-            if (p.tw == 2) hipLaunchKernelGGL((ns_join_kernel<2, KIND>), dim3(4 * p.joined()), dim3(64), 0, s, table, ws, st);
+            if (p.tw == 3) hipLaunchKernelGGL((ns_join_kernel<3, KIND>), dim3(4 * p.joined()), dim3(64), 0, s, table, ws, st);
+            else if (p.tw == 2) hipLaunchKernelGGL((ns_join_kernel<2, KIND>), dim3(4 * p.joined()), dim3(64), 0, s, table, ws, st);
             else hipLaunchKernelGGL((ns_join_kernel<1, KIND>), dim3(4 * p.joined()), dim3(64), 0, s, table, ws, st);
         }
     return hipGetLastError() == hipSuccess ? V1T_OK : V1T_ERR_LAUNCH;
