@@ -289,15 +289,26 @@ DEVFN NsWhere ns_where(const NsUnit& u, char* ws, const NsStep& st, int t) {  //
     constexpr bool SYM = KIND == NS_GRAM || KIND == NS_SQUARE;
     constexpr int B = NsTile<TW>::B;
     NsWhere w;
-    if constexpr (SYM) {  // tile number -> (bi <= bj) of the upper triangle, columns of tiles one after another
-        w.bj = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
-        while ((w.bj + 1) * (w.bj + 2) / 2 <= t) ++w.bj;
-        while (w.bj * (w.bj + 1) / 2 > t) --w.bj;
-        w.bi = t - w.bj * (w.bj + 1) / 2;
+    // tiles in blocks of 8 x 8, so that those that run together on an XCD share rows of P and Q in its L2
+    if constexpr (SYM) {  // bi <= bj: for each 8 columns the rows above their diagonal block, row by row, then the block's own triangle
+        int g = (int)((sqrtf(8.f * t + 1.f) - 1.f) * (0.5f / 8));
+        while (4 * (g + 1) * (8 * (g + 1) + 1) <= t) ++g;
+        while (4 * g * (8 * g + 1) > t) --g;
+        const int width = min(8, (u.mp + B - 1) / B - 8 * g), r = t - 4 * g * (8 * g + 1);
+        if (r < 8 * g * width) {
+            w.bi = r / width;
+            w.bj = 8 * g + r % width;
+        } else {
+            const int q = r - 8 * g * width;
+            int c = 0;
+            while ((c + 1) * (c + 2) / 2 <= q) ++c;
+            w.bi = 8 * g + q - c * (c + 1) / 2;
+            w.bj = 8 * g + c;
+        }
     } else {
-        const int ni = (u.mp + B - 1) / B;
-        w.bi = t % ni;
-        w.bj = t / ni;
+        const int ni = (u.mp + B - 1) / B, nj = (u.np + B - 1) / B, g = t / (8 * nj), r = t - g * 8 * nj, height = min(8, ni - 8 * g);
+        w.bi = 8 * g + r % height;
+        w.bj = r / height;
     }
     w.i0 = w.bi * B;
     w.j0 = w.bj * B;
