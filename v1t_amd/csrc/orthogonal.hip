@@ -135,20 +135,74 @@ struct NsBatch {
             }
         }
     }
+    // N / 4 runs of 4 neighbours: all in, of a tensor whose rows have unit stride (src: in the update, at: in the momentum)
+    DEVFN void load_runs(const NsUnit& u, const long long (&src)[N / 4], const long long (&at)[N / 4]) {
+        typedef T t4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+        typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+        t4 a[N / 4];
+        f4 b[N / 4], w[N / 4];
+#pragma unroll
+        for (int r = 0; r < N / 4; ++r) a[r] = *(const t4*)((const T*)u.in + src[r]);
+        if constexpr (MOM) {
+#pragma unroll
+            for (int r = 0; r < N / 4; ++r) b[r] = *(const f4*)(u.mom + at[r]);
+            if (u.l1 != 0.f) {
+#pragma unroll
+                for (int r = 0; r < N / 4; ++r) w[r] = *(const f4*)(u.w + at[r]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < N / 4; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                g[4 * r + e] = (float)a[r][e];
+                if constexpr (MOM) {
+                    m[4 * r + e] = b[r][e];
+                    if (u.l1 != 0.f) g[4 * r + e] += u.l1 * ns_sign(w[r][e]);
+                }
+            }
+    }
+    DEVFN void next_momentum(const NsMomentum& mo) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) m[e] = mo.mu * m[e] + g[e];
+    }
     DEVFN float update(const NsMomentum& mo, int e) const { return !MOM ? g[e] : mo.nesterov ? g[e] + mo.mu * m[e] : m[e]; }
 };
 
 // partial sums of squares, in 64 bits (their range is that of the inputs squared); MOM: momentum <- mu momentum + gradient on the way
 template <typename T, bool MOM>
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsTable tab, NsMomentum mo, double* parts) {
-    constexpr int N = 8;
+    constexpr int N = 16;
     ns_head head;
     const NsUnit& u = tab.units[ns_find<3>(tab, blockIdx.x, head)];
     const long long all = (long long)u.rows * u.cols, i0 = (long long)(blockIdx.x - u.part0) * u.part;
     const int len = (int)min((long long)u.part, all - i0);
     const bool flat = u.cs == 1 && u.rs == u.cols;
     double sum = 0.0;
-    for (int k0 = 0; k0 < len; k0 += 256 * N) {
+    NsBatch<T, MOM, N> b;
+    auto squares = [&] {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const double v = (double)b.update(mo, e);
+            sum += v * v;
+        }
+    };
+    int k0 = 0;
+    if (flat)
+        for (; k0 + 256 * N <= len; k0 += 256 * N) {
+            long long at[N / 4];
+#pragma unroll
+            for (int r = 0; r < N / 4; ++r) at[r] = i0 + k0 + 1024 * r + 4 * (int)threadIdx.x;
+            b.load_runs(u, at, at);
+            if constexpr (MOM) {
+                b.next_momentum(mo);
+                typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+                for (int r = 0; r < N / 4; ++r) *(f4*)(u.mom + at[r]) = f4{b.m[4 * r], b.m[4 * r + 1], b.m[4 * r + 2], b.m[4 * r + 3]};
+            }
+            squares();
+        }
+    for (; k0 < len; k0 += 256 * N) {
         long long src[N], at[N];
         bool on[N];
 #pragma unroll
@@ -161,17 +215,14 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsTable tab, NsMomentum mo
                 src[e] = r * u.rs + (at[e] - r * u.cols) * u.cs;
             }
         }
-        NsBatch<T, MOM, N> b;
         b.load(u, src, at, on);
+        if constexpr (MOM) {
+            b.next_momentum(mo);
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            if constexpr (MOM) {
-                b.m[e] = mo.mu * b.m[e] + b.g[e];
+            for (int e = 0; e < N; ++e)
                 if (on[e]) u.mom[at[e]] = b.m[e];
-            }
-            const double v = (double)b.update(mo, e);
-            sum += v * v;
         }
+        squares();
     }
     sum = ns_block_sum(sum);
     if (threadIdx.x == 0) parts[blockIdx.x] = sum;
@@ -194,30 +245,52 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(NsTable tab, NsMomentum mo
     ns_head head;
     const NsUnit& u = tab.units[ns_find<4>(tab, blockIdx.x, head)];
     __shared__ float s[NS_TILE_PREP][NS_TILE_PREP + 1];
-    double sum = 0.0;
-    for (int i = threadIdx.x; i < u.nparts; i += 256) sum += parts[u.part0 + i];
-    sum = ns_block_sum(sum);
-    const double mul = (double)scale / (sqrt(sum) + (double)eps);  // 64 bits: a norm may lie outside fp32's range where its elements do not
     const int tj = (u.np + NS_TILE_PREP - 1) / NS_TILE_PREP, t = blockIdx.x - u.prep0;
     const int i0 = t / tj * NS_TILE_PREP, j0 = t % tj * NS_TILE_PREP;  // in X
     const int r0 = u.trans ? j0 : i0, c0 = u.trans ? i0 : j0;            // in the update
-    constexpr int N = 8;
+    constexpr int N = 16;  // all of a thread's; loaded before the norm is added up
+    NsBatch<T, MOM, N> b;
+    const bool whole = u.cs == 1 && r0 + NS_TILE_PREP <= u.rows && c0 + NS_TILE_PREP <= u.cols;  // a whole tile, along its rows: runs of 4
+    const int tr = threadIdx.x / 16, tc = 4 * (threadIdx.x % 16);
+    long long src[N];
+    bool on[N];
+    if (whole) {
+        long long runs[N / 4], at[N / 4];
 #pragma unroll
-    for (int k0 = 0; k0 < NS_TILE_PREP * NS_TILE_PREP; k0 += 256 * N) {
-        long long src[N], at[N];
-        bool on[N];
+        for (int e = 0; e < N / 4; ++e) {
+            runs[e] = src[4 * e] = (long long)(r0 + tr + 16 * e) * u.rs + c0 + tc;
+            at[e] = (long long)(r0 + tr + 16 * e) * u.cols + c0 + tc;
+        }
+        b.load_runs(u, runs, at);
+    } else {
+        long long at[N];
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const int k = k0 + 256 * e + (int)threadIdx.x, r = r0 + k / NS_TILE_PREP, c = c0 + k % NS_TILE_PREP;
+            const int k = 256 * e + (int)threadIdx.x, r = r0 + k / NS_TILE_PREP, c = c0 + k % NS_TILE_PREP;
             on[e] = r < u.rows && c < u.cols;
             src[e] = (long long)r * u.rs + (long long)c * u.cs;
             at[e] = (long long)r * u.cols + c;
         }
-        NsBatch<T, MOM, N> b;
         b.load(u, src, at, on);
+    }
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < u.nparts; i += 256) sum += parts[u.part0 + i];
+    sum = ns_block_sum(sum);
+    const double mul = (double)scale / (sqrt(sum) + (double)eps);  // 64 bits: a norm may lie outside fp32's range where its elements do not
+    if (whole) {
+        if constexpr (MOM) {
+            typedef T t4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+            if (zero) {
+#pragma unroll
+                for (int e = 0; e < N / 4; ++e) *(t4*)((T*)u.in + src[4 * e]) = t4{};
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[tr + 16 * (e / 4)][tc + e % 4] = (float)((double)b.update(mo, e) * mul);
+    } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const int k = k0 + 256 * e + (int)threadIdx.x;
+            const int k = 256 * e + (int)threadIdx.x;
             if constexpr (MOM) {
                 if (zero && on[e]) ((T*)u.in)[src[e]] = (T)0.f;
             }
@@ -268,11 +341,13 @@ DEVFN int ns_deal(int local, int first, int count) {
 }
 typedef f16_t f16x4 __attribute__((ext_vector_type(4)));
 
-template <int TW>
+// Stages of the ring: two where two or more workgroups share a CU and cover each other's waits; four for the 64 tile of symmetric products, whose launches have few of
+// them; three for the 192 tile, alone on its CU
+template <int TW, bool SYM>
 struct NsTile {
     static constexpr int B = 64 * TW, PL = 2 * B * NS_BK, SIDE = 32 * TW;  // PL: elements of an operand's stage, hi and lo
     static constexpr int PIECES = PL * 2 / 1024 / 4;      // LDS-DMA instructions per wave and operand
-    static constexpr int NST = TW == 1 ? 4 : TW == 2 ? 2 : 3;
+    static constexpr int NST = TW == 3 ? 3 : TW == 1 && SYM ? 4 : 2;
     static constexpr int LDS = NST * 2 * PL;              // elements; the epilogue's fp32 tile fits
     static_assert(4 * SIDE * SIDE * 4 <= LDS * 2, "epilogue");
 };
@@ -287,7 +362,7 @@ struct NsWhere {
 template <int TW, int KIND>
 DEVFN NsWhere ns_where(const NsUnit& u, char* ws, const NsStep& st, int t) {  // t: the unit's tile
     constexpr bool SYM = KIND == NS_GRAM || KIND == NS_SQUARE;
-    constexpr int B = NsTile<TW>::B;
+    constexpr int B = 64 * TW;
     NsWhere w;
     // tiles in blocks of 8 x 8, so that those that run together on an XCD share rows of P and Q in its L2
     if constexpr (SYM) {  // bi <= bj: for each 8 columns the rows above their diagonal block, row by row, then the block's own triangle
@@ -409,7 +484,7 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
             *(f16x8*)(to + NS_LO) = cl;
         }
     } else if constexpr (KIND == NS_LAST) {
-        constexpr int N = 8;
+        constexpr int N = 16;
         for (int k0 = lane; k0 < SIDE * SIDE; k0 += 64 * N) {  // a batch's loads of the weights stand together
             long long x[N];
             float o[N], wt[N];
@@ -440,7 +515,7 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
 template <int TW, int KIND, typename T>
 __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(NsTable tab, char* ws, NsStep st) {
     constexpr bool SYM = KIND == NS_GRAM || KIND == NS_SQUARE, TR = !SYM;  // TR: Q is stored [k][j]
-    using Tile = NsTile<TW>;
+    using Tile = NsTile<TW, SYM>;
     constexpr int B = Tile::B, PL = Tile::PL, PIECES = Tile::PIECES, NST = Tile::NST;
     __shared__ __attribute__((aligned(16))) f16_t lds[Tile::LDS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave >> 1, wj = wave & 1;
