@@ -68,7 +68,7 @@ def test_one_matrix(rows, cols, dtype):
 
 @pytest.mark.parametrize("kind", ["gauss", "few"])
 def test_a_list_of_all_shapes_is_each_alone(kind):
-    """More units than one table launch holds; each result bit for bit that of the matrix alone where both take the same tile, and right in any case."""
+    """More units than one table launch holds, small and large ones mixed; the same bits every time."""
     us = [update(r, c, i, kind) for i in range(2) for r, c in SHAPES]
     for u, o in zip(us, v1t_amd.orthogonalize(us)):
         close(o, u)

@@ -246,3 +246,34 @@ def test_version_counter_sees_the_write():
     v1t_amd.rotary_(q, positions((3, 1)), sections=(4,))
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         y.backward()
+
+
+@pytest.mark.parametrize("D", [11, 16])
+def test_results_may_be_changed_in_place(D):
+    q = torch.randn(2, 3, 4, D, device=DEV, requires_grad=True)
+    k = torch.randn(2, 3, 1, D, device=DEV, requires_grad=True)
+    at = positions((3, 1))
+    yq, yk = v1t_amd.rotary(q, at, k=k, sections=(5,))
+    yq.mul_(2.0)
+    w = torch.randn(2, 3, 4, D, device=DEV)
+    (d,) = torch.autograd.grad((yq * w).sum() + yk.sum(), q)
+    close(d, *turned(2 * w, at, (5,), 10000.0, "pairs", False, inverse=True))
+    assert yq.untyped_storage().nbytes() >= 24 * ((D + 7) // 8 * 8) * 4  # the room is the result's own
+
+
+def test_the_c_entry_without_room():
+    """y rows of exactly D features: nothing behind a row's features is written, in any order of the rows."""
+    import ctypes as C
+    from v1t_amd import lib as L
+
+    for D, room in ((11, 0), (11, 11), (11, 13), (21, 0), (3, 3)):
+        B, T, H = 2, 5, 3
+        x = torch.randn(B, T, H, D, device=DEV, dtype=torch.bfloat16)
+        gap = 2 if room > D else 0
+        buffer = torch.full((B * T * H * (D + gap) + 64,), 7.0, device=DEV, dtype=torch.bfloat16)
+        y = buffer[32:-32].view(B, T, H, D + gap)
+        at = positions((T, 1))
+        op = (L.RotaryOperand * 1)(L.RotaryOperand(x.data_ptr(), y.data_ptr(), *x.stride()[:3], *y.stride()[:3], H, room))
+        L.check(L.load().v1t_rotary(op, 1, 0, B, T, D, (C.c_int * 1)(1), 1, 10.0, 0, 0, 0, at.data_ptr(), 0, 0, 1, 1, L.stream()))
+        close(y[..., :D], *turned(x, at, (1,), 10.0, "pairs", False))
+        assert bool((buffer[:32] == 7.0).all()) and bool((buffer[-32:] == 7.0).all()) and bool((y[..., D:] == 7.0).all())

@@ -88,10 +88,11 @@ def _sections(sections: t.Tuple[int, ...]):
 
 
 def _like(x: torch.Tensor) -> torch.Tensor:
-    """x's shape with room for a multiple of 8 features a head: what lies behind the last whole 8 is moved as one store, too."""
-    d = x.shape[-1]
-    y = torch.empty((*x.shape[:-1], (d + 7) // 8 * 8), dtype=x.dtype, device=x.device)
-    return y if y.shape[-1] == d else y[..., :d]
+    """x's shape with room for a multiple of 8 features a head: what lies behind the last whole 8 is moved as one store, too. Not a view of the wider tensor but
+    one over its storage: autograd lets a view that a function returns not be changed in place."""
+    shape, d = x.shape, x.shape[-1]
+    y = torch.empty((*shape[:-1], (d + 7) // 8 * 8), dtype=x.dtype, device=x.device)
+    return y if d % 8 == 0 else torch.empty(0, dtype=x.dtype, device=x.device).set_(y.untyped_storage(), 0, shape, y.stride())
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -136,7 +137,7 @@ class _RotaryFn(torch.autograd.Function):
 def rotary(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int], k: t.Optional[torch.Tensor] = None, base: float = 10000.0,
            layout: str = "pairs", shared: bool = False, inverse: bool = False):
     """q (and k) turned by their tokens' positions: new tensors; differentiable in q and k. Where 8 does not divide the number of features, the
-    result is a view of rows that have room for the next multiple (`reshape`, not `view`, joins its heads).
+    result has rows with room for the next multiple: it is not contiguous (`reshape`, not `view`, joins its heads).
 
     q: (batch, tokens, heads, features) or (tokens, heads, features), bf16 / fp16 / fp32, any strides; k: the same with its own number of heads.
     positions: (tokens, axes) for all sequences, or (batch, tokens, axes); int32, int64 or fp32, negative ones too. A token at 0 on every axis is
