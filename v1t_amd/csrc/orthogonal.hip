@@ -31,7 +31,7 @@ namespace {
 constexpr int NS_BK = 32;            // K step of the products; planes are padded to it with zeros both ways
 constexpr int NS_PART = 4096;        // least number of elements per partial sum of squares; at most 1024 partial sums a unit
 constexpr int NS_TILE_PREP = 64;     // the first planes are written in 64 x 64 tiles
-constexpr int NS_CHUNK = 16;         // units per table launch (kernel arguments)
+constexpr int NS_CHUNK = 24;         // units per table launch (kernel arguments: below 4 KB)
 constexpr int NS_MAX_STEPS = 32, NS_MAX_UNITS = 1 << 16;
 
 struct NsUnit {
@@ -39,7 +39,7 @@ struct NsUnit {
     void* out;        // the result, or nullptr: w is updated
     float *mom, *w;
     long long rs, cs;                // element strides of `in`; out, mom and w are row-major without gaps
-    long long x[2], sq[4];           // byte offsets in the workspace: X twice, the m x m matrices
+    long long base;                  // byte offset in the workspace: X twice, then the m x m matrices (ns_x, ns_square_at)
     int rows, cols, m, n, mp, np, trans;
     int part, part0, nparts, prep0;  // elements per partial sum; first workgroup of this unit in the launches of each kind
     int first[3];                    // first tile in the products' launches: gram, poly, apply / last
@@ -47,9 +47,14 @@ struct NsUnit {
     float lr, decay, l1;             // w <- decay w - lr O;  gradient + l1 sign(w)
 };
 
+__host__ __device__ inline long long ns_align(long long x) { return (x + 255) / 256 * 256; }
+__host__ __device__ inline long long ns_x(const NsUnit& u, int which) { return u.base + which * ns_align(4ll * u.mp * u.np); }
+__host__ __device__ inline long long ns_square_at(const NsUnit& u, int which) { return ns_x(u, 2) + which * ns_align(4ll * u.mp * u.mp); }
+
 struct NsChunk {
     NsUnit u[NS_CHUNK];
 };
+static_assert(sizeof(NsChunk) + 3 * 4 * NS_MAX_STEPS + 64 <= 4096, "kernel arguments");
 
 // What a workgroup finds its unit by: per launch (0 .. 2 the products', 3 the partial sums', 4 the first planes') and unit its first workgroup, and the run of units of
 // its size. Apart from the units, so that a wave reads 64 of them at once from few lines
@@ -105,14 +110,15 @@ DEVFN float ns_sign(float x) { return (float)((x > 0.f) - (x < 0.f)); }
 // sum over the workgroup of NT, in a fixed order
 template <int NT = 256>
 DEVFN double ns_block_sum(double v) {
-    __shared__ double s[NT];
-    s[threadIdx.x] = v;
+    __shared__ double s[NT / 64];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
     __syncthreads();
-    for (int o = NT / 2; o > 0; o >>= 1) {
-        if ((int)threadIdx.x < o) s[threadIdx.x] += s[threadIdx.x + o];
-        __syncthreads();
-    }
-    return s[0];
+    v = 0.0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) v += s[w];
+    return v;
 }
 
 // N elements of the update: gradient with its L1 term, momentum (MOM), then U. The loads of a batch stand together: each of a tensor that is written, too, would
@@ -298,7 +304,7 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(NsTable tab, NsMomentum mo
         }
     }
     __syncthreads();
-    f16_t* const X = (f16_t*)(ws + u.x[0]);
+    f16_t* const X = (f16_t*)(ws + ns_x(u, 0));
     for (int k = threadIdx.x; k < NS_TILE_PREP * NS_TILE_PREP / 8; k += 256) {
         const int i = k / (NS_TILE_PREP / 8), j = 8 * (k % (NS_TILE_PREP / 8));
         if (i0 + i >= u.mp || j0 + j >= u.np) continue;  // np is a multiple of 32: groups of 8 are whole
@@ -387,10 +393,10 @@ DEVFN NsWhere ns_where(const NsUnit& u, char* ws, const NsStep& st, int t) {  //
     }
     w.i0 = w.bi * B;
     w.j0 = w.bj * B;
-    w.D = KIND == NS_SQUARE ? (const f16_t*)(ws + u.sq[st.d]) : (const f16_t*)(ws + u.x[st.from]);
-    w.D2 = (const f16_t*)(ws + u.sq[st.d2]);
+    w.D = KIND == NS_SQUARE ? (const f16_t*)(ws + ns_square_at(u, st.d)) : (const f16_t*)(ws + ns_x(u, st.from));
+    w.D2 = (const f16_t*)(ws + ns_square_at(u, st.d2));
     w.ldd = KIND == NS_SQUARE ? u.mp : u.np;
-    w.C = (f16_t*)(ws + (KIND == NS_GRAM ? u.sq[0] : KIND == NS_SQUARE ? u.sq[st.out] : u.x[st.from ^ 1]));
+    w.C = (f16_t*)(ws + (KIND == NS_GRAM ? ns_square_at(u, 0) : KIND == NS_SQUARE ? ns_square_at(u, st.out) : ns_x(u, st.from ^ 1)));
     w.cols = SYM ? u.mp : u.np;
     return w;
 }
@@ -533,9 +539,9 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(NsTable t
     const NsWhere w = ns_where<TW, KIND>(u, ws, st, number - head[0]);
     const int steps = (KIND == NS_GRAM ? u.np : u.mp) / NS_BK, each = piece ? (steps + st.split - 1) / st.split : steps;
     const int t0 = piece ? over % st.split * each : 0, nk = max(0, min(each, steps - t0));  // this workgroup's K steps
-    const f16_t* X = (const f16_t*)(ws + u.x[st.from]);
-    const f16_t* P = KIND == NS_GRAM ? X : (const f16_t*)(ws + u.sq[st.p]);
-    const f16_t* Q = KIND == NS_SQUARE ? (const f16_t*)(ws + u.sq[st.q]) : X;
+    const f16_t* X = (const f16_t*)(ws + ns_x(u, st.from));
+    const f16_t* P = KIND == NS_GRAM ? X : (const f16_t*)(ws + ns_square_at(u, st.p));
+    const f16_t* Q = KIND == NS_SQUARE ? (const f16_t*)(ws + ns_square_at(u, st.q)) : X;
     const int ldp = KIND == NS_GRAM ? u.np : u.mp, ldq = KIND == NS_SQUARE ? u.mp : u.np;
 
     // A 1-KB piece fills 64 16-B chunks of a stage in order; which 16 B of the tile's row a chunk holds is swizzled, so that the fragment reads below spread over all
@@ -938,7 +944,7 @@ __global__ __launch_bounds__(256) void ns_copy_kernel(NsTable tab, const char* w
     const NsUnit& u = tab.units[ns_find<4>(tab, blockIdx.x, head)];
     const int tj = (u.np + NS_TILE_PREP - 1) / NS_TILE_PREP, t = blockIdx.x - u.prep0;
     const int i0 = t / tj * NS_TILE_PREP, j0 = t % tj * NS_TILE_PREP;
-    const f16_t* X = (const f16_t*)(ws + u.x[0]);
+    const f16_t* X = (const f16_t*)(ws + ns_x(u, 0));
     for (int k = threadIdx.x; k < NS_TILE_PREP * NS_TILE_PREP; k += 256) {
         const int i = i0 + k / NS_TILE_PREP, j = j0 + k % NS_TILE_PREP;
         if (i >= u.m || j >= u.n) continue;
@@ -970,7 +976,6 @@ std::pair<int, int> ns_parts(long long elements) {
     const long long part = std::max<long long>(NS_PART, (elements + 1023) / 1024);
     return {(int)part, (int)((elements + part - 1) / part)};
 }
-long long ns_align(long long x) { return (x + 255) / 256 * 256; }
 
 // Tile and split of a product with t64 / t128 tiles of each size whose K steps sum to k64 / k128, at the least estimated time. A CU holds two workgroups of
 // either tile. Measured, us per K step: the larger tile 1.6 with two on a CU and 0.9 alone, the smaller 0.85 and 0.25 (so the larger does twice
@@ -1045,10 +1050,8 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
         u.trans = u.rows > u.cols;
         u.m = std::min(u.rows, u.cols); u.n = std::max(u.rows, u.cols);
         u.mp = round_up(u.m, NS_BK); u.np = round_up(u.n, NS_BK);
-        const long long xb = ns_align(4ll * u.mp * u.np), ab = ns_align(4ll * u.mp * u.mp);
-        u.x[0] = at; u.x[1] = at + xb;
-        at += 2 * xb;
-        for (int q = 0; q < (l.pairs ? 4 : 2); ++q, at += ab) u.sq[q] = at;
+        u.base = at;
+        at = ns_square_at(u, l.pairs ? 4 : 2);
         const auto ps = ns_parts((long long)u.rows * u.cols);
         u.part = ps.first; u.nparts = ps.second; u.part0 = part; u.prep0 = first;
         part += u.nparts;
