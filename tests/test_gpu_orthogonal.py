@@ -84,6 +84,32 @@ def test_large_tiles():
     close(v1t_amd.orthogonalize(u), u)
 
 
+@pytest.mark.parametrize("count,rows,cols", [(4, 1300, 1300), (1, 1500, 1500), (2, 1000, 1900), (1, 100, 20000), (1, 4001, 4100)])
+def test_tiles_and_pieces(count, rows, cols):
+    """Symmetric products in tiles of 192 split over K, of 128 split, of 128 and 64 side by side, of 64 in 16 pieces, of 192 whole; the same bits every time."""
+    us = [update(rows, cols, i) for i in range(count)]
+    os = v1t_amd.orthogonalize(us)
+    for u, o in zip(us, os):
+        close(o, u)
+    assert all(torch.equal(a, b) for a, b in zip(os, v1t_amd.orthogonalize(us)))
+
+
+@pytest.mark.parametrize("rows,cols", [(700, 2900), (2900, 700), (1000, 8100)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("steps", [1, 2, 4, 5])
+def test_steps_in_pairs(rows, cols, dtype, steps):
+    """Long matrices, whose steps go two at a time: one, two, two pairs, and a step left over."""
+    u = update(rows, cols, kind="few").to(dtype)
+    close(v1t_amd.orthogonalize(u, steps=steps), u, steps=steps)
+
+
+def test_pairs_that_would_leave_the_planes_range():
+    """12 * 12 at zero is more than a pair's matrix may hold: such steps go one by one, also where the sizes would have them in pairs."""
+    u, co = update(700, 2900), [(12.0, -20.0, 9.0), (12.0, -2.0, 0.0)]
+    close(v1t_amd.orthogonalize(u, steps=2, coefficients=co), u, steps=2, coefficients=co)
+    close(v1t_amd.orthogonalize(u), u)  # and the usual ones again
+
+
 def test_stack_strides_and_views():
     stack = torch.stack([update(40, 50, i) for i in range(5)])
     o = v1t_amd.orthogonalize(stack)
@@ -196,7 +222,7 @@ def test_muon_step(nesterov, decay, l1):
 def test_muon_step_captured_and_replayed():
     """Replays between eager work, against the same steps run eagerly, bit for bit."""
     gen = torch.Generator(device=DEV).manual_seed(4)
-    shapes = [(155, 64), (70, 200)] * 10  # two table launches
+    shapes = [(155, 64), (170, 200)] * 30  # two table launches
     ps, gs, ms = ([torch.randn(s, device=DEV, generator=gen) for s in shapes] for _ in range(3))
     qs, ns = [p.clone() for p in ps], [m.clone() for m in ms]
     v1t_amd.muon_step([p.clone() for p in ps], gs, [m.clone() for m in ms], lr=0.02)
