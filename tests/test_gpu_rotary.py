@@ -227,6 +227,17 @@ def test_another_stream():
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("D,sections", [(6, (3,)), (14, (4, 3))])
+def test_many_sequences_with_positions_of_their_own(D, sections):
+    """More sequences than a launch has workgroups along one dimension: a workgroup goes over several, each with its own angles."""
+    g = torch.Generator().manual_seed(9)
+    q = torch.randn(140000, 2, 3, D, generator=g).to(DEV)
+    at = positions((140000, 2, len(sections)), seed=2)
+    y = v1t_amd.rotary(q, at, sections=sections)
+    close(y, *turned(q, at, sections, 10000.0, "pairs", False))
+    assert torch.equal(v1t_amd.rotary_(q.clone(), at, sections=sections), y)
+
+
 def test_offsets_past_32_bits():
     """A cache of 2^31 + elements: the last sequence lies behind the first 4 GB."""
     big = torch.empty(3, 1100, 1000, 1000, dtype=torch.bfloat16, device=DEV)

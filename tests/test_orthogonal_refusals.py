@@ -24,6 +24,21 @@ def test_orthogonalize_refusals(error, change):
         v1t_amd.orthogonalize(arguments.pop("updates"), **arguments)
 
 
+def test_sizes_that_do_not_fit_32_bits():
+    """2^32 + 5 columns are not 5."""
+    wide = torch.zeros(1).expand(1, 2**32 + 5)
+    with pytest.raises(ValueError, match="at most"):
+        v1t_amd.orthogonalize(wide)
+    wide = torch.empty(1, 2**32 + 5, device="meta")
+    with pytest.raises(ValueError, match="at most"):
+        v1t_amd.muon_step([wide], [wide], [wide], lr=0.1)
+    from v1t_amd import muon
+
+    for shape in ((40000, 40000), (1, 2**22 + 1), (2**31, 2), (2**16, 2**15 + 1)):
+        with pytest.raises(ValueError, match="at most"):
+            muon._workspace_bytes((shape,))
+
+
 def test_nothing_to_do():
     assert v1t_amd.orthogonalize([]) == []
     v1t_amd.muon_step([], [], [], lr=0.1)

@@ -34,6 +34,14 @@ def test_too_many_pairs():
         v1t_amd.rotary(torch.zeros(1, 1, 600), torch.zeros(1, 1, dtype=torch.int32), sections=(257,))
 
 
+@pytest.mark.parametrize("call", ["rotary", "rotary_"])
+@pytest.mark.parametrize("shape", [(2**32 + 1, 1, 8), (2**32 + 1, 1, 1, 8), (1, 2**32 + 1, 8), (1, 1, 2**32 + 8)])
+def test_sizes_that_do_not_fit_32_bits(call, shape):
+    """2^32 + 1 tokens are not one."""
+    with pytest.raises(ValueError, match="less than"):
+        getattr(v1t_amd, call)(torch.zeros(1).expand(shape), torch.zeros(1, 1, dtype=torch.int32).expand(shape[-3], 1), sections=(4,))
+
+
 def test_in_place_refusals():
     at = dict(positions=AT, sections=(3, 4))
     with pytest.raises(RuntimeError, match="requires grad"):
@@ -71,5 +79,6 @@ def test_c_entry_refusals():
         assert call(**change) == -1, change
     assert call(D=1024, sections=(C.c_int * 2)(200, 57)) == -2  # more pairs than a kernel argument holds
     assert call(B=0) == 0 and call(T=0) == 0  # nothing to do
+    assert call(D=2048, T=(1 << 31) - 1, sections=(C.c_int * 2)(100, 100)) == -2  # a launch of more than 2^32 threads
     ops[1].heads = 0
     assert call() == -1

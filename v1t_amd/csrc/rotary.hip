@@ -143,7 +143,10 @@ __global__ __launch_bounds__(ROT_THREADS, 4) void rotary_kernel(RotArgs g, RotRa
     const int b0 = blockIdx.y * g.nb, b1 = min(b0 + g.nb, g.B);
     if (g.pb == 0) angles(0);
     for (int b = b0; b < b1; ++b) {
-        if (g.pb != 0) angles(b);
+        if (g.pb != 0) {
+            if (b > b0) __syncthreads();  // the last sequence's have been read by all: those in place read them here, not in registers
+            angles(b);
+        }
 #pragma unroll 1
         for (int w = 0; w < 2; ++w) {
             if (!mine) break;
@@ -271,6 +274,7 @@ extern "C" int v1t_rotary(const v1t_rotary_operand* ops, int n_ops, int dtype, i
     // A workgroup takes all heads and as many sequences as share their positions with it, while 2048 workgroups (8 a CU) are left; fewer tokens than that: the heads
     // are dealt out, down to the 4 whose loads stand together
     const long long gx = ((long long)T + g.nt - 1) / g.nt;
+    if (gx >= (1 << 24)) return V1T_ERR_UNSUPPORTED;  // a launch has less than 2^32 threads
     long long nb = g.pb == 0 ? std::max(1ll, std::min<long long>(16, gx * B / 2048)) : 1;
     nb = std::max(nb, ((long long)B + 65534) / 65535);
     const long long gy = ((long long)B + nb - 1) / nb;

@@ -17,6 +17,8 @@ from . import lib as L
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # drive singular values to about 1 (0.7 to 1.2) within five steps from 0.003 on
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_STEPS = 32
+MAX_SIDE, MAX_LENGTH, MAX_ELEMENTS = 1 << 15, 1 << 22, 1 << 31
+_SIZES = f"matrices have at most {MAX_ELEMENTS} elements, {MAX_SIDE} rows or columns of the shorter side and {MAX_LENGTH} of the longer"
 
 
 def _coefficients(coefficients, steps: int) -> t.Any:
@@ -38,6 +40,9 @@ def _floats(values: t.Tuple[float, ...]):
 @functools.lru_cache(maxsize=256)
 def _workspace_bytes(shapes: t.Tuple[t.Tuple[int, int], ...]) -> int:
     n = len(shapes)
+    for s in shapes:
+        if min(s) > MAX_SIDE or max(s) > MAX_LENGTH or s[0] * s[1] > MAX_ELEMENTS:
+            raise ValueError(f"orthogonalize: {_SIZES}, got {s}")
     return int(L.load().v1t_orthogonalize_ws_bytes((C.c_int * n)(*[r for r, _ in shapes]), (C.c_int * n)(*[c for _, c in shapes]), n))
 
 
@@ -71,6 +76,8 @@ def orthogonalize(updates, *, steps: int = 5, coefficients=COEFFICIENTS, eps: fl
             raise ValueError("orthogonalize: every update is a matrix")
         if u.dtype not in _DTYPES or u.dtype != us[0].dtype:
             raise TypeError(f"orthogonalize: updates share one of {list(_DTYPES)}, got {sorted({str(x.dtype) for x in us})}")
+        if u.numel() > MAX_ELEMENTS:  # a size could wrap in the C entry's 32 bits; `_workspace` checks the sides
+            raise ValueError(f"orthogonalize: {_SIZES}, got {tuple(u.shape)}")
         if u.device != us[0].device:
             raise ValueError("orthogonalize: updates on several devices")
         if torch.is_grad_enabled() and u.requires_grad:
@@ -134,6 +141,8 @@ def muon_step(params: t.Sequence[torch.Tensor], grads: t.Sequence[torch.Tensor],
         size = p.numel()
         if size == 0:
             continue
+        if size > MAX_ELEMENTS:
+            raise ValueError(f"muon_step: {_SIZES}, got {tuple(shape)}")
         rows, at = shape[0], (p.data_ptr(), g.data_ptr(), m.data_ptr())
         cols = size // rows
         spans += [(x, x + 4 * size) for x in at]

@@ -17,6 +17,7 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 _LAYOUTS = {"pairs": 0, "halves": 1}
 MAX_PAIRS = 256
+MAX_SIZE = 1 << 31  # the C entry's sizes have 32 bits
 
 
 class _Turn(t.NamedTuple):
@@ -50,6 +51,8 @@ def _check(q: torch.Tensor, k: t.Optional[torch.Tensor], positions: torch.Tensor
             raise ValueError(f"rotary: q and k share device, batch, tokens and features, got {tuple(q.shape)} on {q.device} and {tuple(x.shape)} on {x.device}")
         if x.shape[-2] < 1:
             raise ValueError("rotary: no heads")
+        if max(x.shape) >= MAX_SIZE:
+            raise ValueError(f"rotary: batch, tokens, heads and features are less than {MAX_SIZE} each, got {tuple(x.shape)}")
     if positions.dtype not in _POSITION_TYPES:
         raise TypeError(f"rotary: positions are one of {list(_POSITION_TYPES)}, got {positions.dtype}")
     if positions.requires_grad:
@@ -176,7 +179,8 @@ def _apart(q: torch.Tensor, k: torch.Tensor) -> bool:
 
 def rotary_(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int], k: t.Optional[torch.Tensor] = None, base: float = 10000.0,
             layout: str = "pairs", shared: bool = False, inverse: bool = False):
-    """`rotary` in place, outside autograd (a new token's q and k, a projection's buffer): the same values, features behind the turned ones untouched."""
+    """`rotary` in place, outside autograd (a new token's q and k, a projection's buffer): the same values, features behind the turned ones untouched.
+    Positions lie in memory of their own."""
     sections = _check(q, k, positions, sections, base, layout)
     xs = [x for x in (q, k) if x is not None]
     for x in xs:
