@@ -145,6 +145,19 @@ def test_fused_muon_refusals():
     assert [(r, c) for _, r, c in muon.matrices()] == [(256, 64)] * 3 + [(64, 256), (128, 64), (64, 128)]
 
 
+def test_fused_muon_restores_its_rates():
+    """The matrices' rate is muon_lr where the core's is core_lr, also for an optimizer that was made with other rates than its checkpoint's."""
+    model, _, _ = small()
+    saved = v1t_amd.FusedMuon.for_model(model, lr=1e-3, core_lr=2e-3, muon_lr=0.05)
+    saved.param_groups[[g["name"] for g in saved.param_groups].index("core")]["lr"] = 5e-4  # a scheduler's quarter
+    other = v1t_amd.FusedMuon.for_model(model, lr=1e-3, core_lr=1e-3, muon_lr=0.01)
+    other.load_state_dict(saved.state_dict())
+    (group,) = [g for g in other.param_groups if "muon" in g]
+    assert group["name"] == "core" and group["lr"] == 5e-4 and group["muon"] == {"lr": 0.05, "core_lr": 2e-3}
+    group["muon"]["lr"] = 1.0
+    assert [g["muon"]["lr"] for g in saved.param_groups if "muon" in g] == [0.05]  # a copy
+
+
 def test_rotary_core_refusals():
     with pytest.raises(ValueError, match="head dim 3"):
         small(rotary=True, emb_dim=3, num_heads=1)

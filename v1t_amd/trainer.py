@@ -227,7 +227,7 @@ class FusedMuon(FusedAdamW):
 
     `muon_lr` is the matrices' learning rate where the core's group has `core_lr`; a scheduler that scales the group's "lr" scales both. A matrix's momentum lives
     in its slice of the arena's `exp_avg`, its slice of `exp_avg_sq` stays zero: checkpoints keep torch.optim's format, and the "muon" entry of the core's
-    group tells them from AdamW's (`load_state_dict` refuses the other kind). Ranks of a data-parallel step that hold the same gradients compute the same update."""
+    group - the two rates that belong together; restored with "lr" - tells them from AdamW's (`load_state_dict` refuses the other kind). Ranks of a data-parallel step that hold the same gradients compute the same update."""
 
     def __init__(self, lr: float, betas=(0.9, 0.9999), eps: float = 1e-8, weight_decay: float = 0.0, muon_lr: float = 0.02, momentum: float = 0.95,
                  nesterov: bool = True, steps: int = 5):
@@ -248,11 +248,17 @@ class FusedMuon(FusedAdamW):
         if not core_lr > 0.0:
             raise ValueError(f"FusedMuon: the matrices' learning rate follows the core's, which must be positive, got {core_lr}")
         super().bind(model, core_lr)
-        self._per_core_lr = self.muon_lr / float(core_lr)
         for g in self.param_groups:
             if g["name"] == "core":
-                g["muon"] = {"lr": self.muon_lr, "momentum": self.momentum, "nesterov": self.nesterov, "steps": self.steps}
+                g["muon"] = {"lr": self.muon_lr, "core_lr": float(core_lr)}
         self._matrices: t.Optional[t.List[t.Tuple[int, int, int]]] = None
+
+    def load_state_dict(self, sd: t.Dict[str, t.Any]) -> None:
+        super().load_state_dict(sd)
+        saved = [g["muon"] for g in sd["param_groups"] if g.get("muon")]
+        for g in self.param_groups:
+            if "muon" in g:
+                g["muon"] = dict(saved[0])
 
     def matrices(self) -> t.List[t.Tuple[int, int, int]]:
         """(offset, rows, cols) in the core's arena of every matrix that takes the momentum step, in order."""
@@ -277,6 +283,7 @@ class FusedMuon(FusedAdamW):
         m, v = arena.moments()
         p_, g_, m_, v_ = (x.data_ptr() for x in (arena.data, arena.grad, m, v))
         rest, mats = [], []
+        (rates,) = [g["muon"] for g in self.param_groups if "muon" in g]
         for start, n, l1, lr in ranges:
             at, end = start, start + n
             for off, rows, cols in self.matrices():
@@ -287,7 +294,7 @@ class FusedMuon(FusedAdamW):
                     raise RuntimeError("FusedMuon: a range of the core's arena ends inside a matrix")
                 if off > at:
                     rest.append((at, off - at, l1, lr))
-                a = lr * self._per_core_lr
+                a = lr * (rates["lr"] / rates["core_lr"])
                 mats.append(L.MuonRange(p_ + 4 * off, g_ + 4 * off, m_ + 4 * off, rows, cols, a * math.sqrt(max(1.0, rows / cols)), 1.0 - a * self.weight_decay, l1, 0))
                 at = off + size
             if end > at:
