@@ -147,6 +147,18 @@ def test_scale(scale):
     close(o, u * scale, eps=0.0)
 
 
+@pytest.mark.parametrize("rows,cols", [(50, 70), (20, 500), (90, 100), (155, 620), (400, 170), (700, 2900)])
+@pytest.mark.parametrize("scale", [1e-9, 1e-11, 1e-15, 1e-25])
+def test_eps_that_outweighs_the_norm(rows, cols, scale):
+    """The iterate is a polynomial of a small number then, as exact as any other; beside a matrix of the usual size."""
+    u = update(rows, cols)
+    o, other = v1t_amd.orthogonalize([u * scale, u])
+    close(o, u * scale)
+    close(other, u)
+    for steps, co in ((0, COEFFICIENTS), (1, COEFFICIENTS), (4, COEFFICIENTS), (3, [(0.5, 0.25, 0.25), (1.0, 0.0, -1.0), (8.0, -3.0, 0.0)])):
+        close(v1t_amd.orthogonalize(u * scale, steps=steps, coefficients=co), u * scale, steps=steps, coefficients=co)
+
+
 def test_zeros_nan_and_infinity_stay_in_their_matrix():
     us = [update(33, 40, i) for i in range(4)]
     clean = v1t_amd.orthogonalize(us)

@@ -12,7 +12,9 @@
 // hi hi + hi lo + lo hi, accumulated in fp32: three MFMAs where fp16 has one, at a sixteenth of the time of an fp32 one. The term that is left out
 // and the two roundings are 2^-22 of a product each, of random sign: the error of fp32 operands (the steps amplify what is lost on the small
 // singular values up to a^5 = 480 times: one fp16 plane leaves 2e-3 of the result's norm, two leave what fp32 does, 2e-6).
-// The common exponent e makes every scale of the chain 2^-e.
+// The common exponent e makes every scale of the chain 2^-e. Where eps outweighs the norm, X is too small for planes of that scale: with x0 = -log2 of
+// |U| / (|U| + eps), no singular value of X before step k is above 2^(lg_k - x0), lg_k from the largest factors of the steps before, and X's planes - of all
+// matrices - are 2^floor(x0 - lg_k) larger, if that is more than one (ns_extra). A and S, small against a, need no more.
 //
 // All matrices of a call ("units") go through each product in one launch: the shared core's matrices are small, and launches are what they cost.
 #include <hip/hip_runtime.h>
@@ -40,21 +42,30 @@ struct NsUnit {
     float *mom, *w;
     long long rs, cs;                // element strides of `in`; out, mom and w are row-major without gaps
     long long base;                  // byte offset in the workspace: X twice, then the m x m matrices (ns_x, ns_square_at)
-    int rows, cols, m, n, mp, np, trans;
+    int rows, cols, n, mp, np;       // n: the longer side; mp, np: X's sides, in whole K steps
     int part, part0, nparts, prep0;  // elements per partial sum; first workgroup of this unit in the launches of each kind
     int first[3];                    // first tile in the products' launches: gram, poly, apply / last
     int group0[3], group[3];         // first tile and tiles of the run of units of this size
     float lr, decay, l1;             // w <- decay w - lr O;  gradient + l1 sign(w)
+    __host__ __device__ int m() const { return rows < cols ? rows : cols; }
+    __host__ __device__ bool trans() const { return rows > cols; }  // X is the update's transpose
+    float x0;                        // -log2 of the norm of the first X; written by ns_prep_kernel
 };
 
 __host__ __device__ inline long long ns_align(long long x) { return (x + 255) / 256 * 256; }
 __host__ __device__ inline long long ns_x(const NsUnit& u, int which) { return u.base + which * ns_align(4ll * u.mp * u.np); }
 __host__ __device__ inline long long ns_square_at(const NsUnit& u, int which) { return ns_x(u, 2) + which * ns_align(4ll * u.mp * u.mp); }
 
+// by what power of two X's planes are larger than the common scale
+__host__ __device__ inline int ns_extra(float x0, float lg) {
+    const float e = floorf(x0 - lg);
+    return e > 0.f ? (int)(e < 100.f ? e : 100.f) : 0;  // (x0 is infinite for a matrix of zeros, NaN beside one)
+}
+
 struct NsChunk {
     NsUnit u[NS_CHUNK];
 };
-static_assert(sizeof(NsChunk) + 3 * 4 * NS_MAX_STEPS + 64 <= 4096, "kernel arguments");
+static_assert(sizeof(NsChunk) + 4 * (4 * NS_MAX_STEPS + 1) + 64 <= 4096, "kernel arguments");
 
 // What a workgroup finds its unit by: per launch (0 .. 2 the products', 3 the partial sums', 4 the first planes') and unit its first workgroup, and the run of units of
 // its size. Apart from the units, so that a wave reads 64 of them at once from few lines
@@ -120,6 +131,16 @@ DEVFN double ns_block_sum(double v) {
     for (int w = 0; w < NT / 64; ++w) v += s[w];
     return v;
 }
+
+struct NsNorm {  // 64 bits: a norm may lie outside fp32's range where its elements do not
+    float x0;
+    double mul;  // the first planes are the update times this
+    DEVFN NsNorm(double squares, float eps, float scale) {
+        const double norm = sqrt(squares), by = 1.0 / (norm + (double)eps);
+        x0 = -log2f((float)(norm * by));
+        mul = ldexp((double)scale, ns_extra(x0, 0.f)) * by;
+    }
+};
 
 // N elements of the update: gradient with its L1 term, momentum (MOM), then U. The loads of a batch stand together: each of a tensor that is written, too, would
 // wait for the store before it
@@ -253,7 +274,7 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(NsTable tab, NsMomentum mo
     __shared__ float s[NS_TILE_PREP][NS_TILE_PREP + 1];
     const int tj = (u.np + NS_TILE_PREP - 1) / NS_TILE_PREP, t = blockIdx.x - u.prep0;
     const int i0 = t / tj * NS_TILE_PREP, j0 = t % tj * NS_TILE_PREP;  // in X
-    const int r0 = u.trans ? j0 : i0, c0 = u.trans ? i0 : j0;            // in the update
+    const int r0 = u.trans() ? j0 : i0, c0 = u.trans() ? i0 : j0;            // in the update
     constexpr int N = 16;  // all of a thread's; loaded before the norm is added up
     NsBatch<T, MOM, N> b;
     const bool whole = u.cs == 1 && r0 + NS_TILE_PREP <= u.rows && c0 + NS_TILE_PREP <= u.cols;  // a whole tile, along its rows: runs of 4
@@ -282,7 +303,9 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(NsTable tab, NsMomentum mo
     double sum = 0.0;
     for (int i = threadIdx.x; i < u.nparts; i += 256) sum += parts[u.part0 + i];
     sum = ns_block_sum(sum);
-    const double mul = (double)scale / (sqrt(sum) + (double)eps);  // 64 bits: a norm may lie outside fp32's range where its elements do not
+    const NsNorm norm(sum, eps, scale);
+    const double mul = norm.mul;
+    if (t == 0 && threadIdx.x == 0) const_cast<NsUnit&>(u).x0 = norm.x0;  // for the launches behind this one
     if (whole) {
         if constexpr (MOM) {
             typedef T t4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
@@ -312,7 +335,7 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(NsTable tab, NsMomentum mo
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             f16_t a, b;
-            ns_split(u.trans ? s[j + e][i] : s[i][j + e], a, b);
+            ns_split(u.trans() ? s[j + e][i] : s[i][j + e], a, b);
             h[e] = a;
             l[e] = b;
         }
@@ -331,6 +354,7 @@ struct NsStep {
     int p, q, d, d2, out;                // which m x m matrices
     int from;            // which of the two X planes is read
     float inv;           // 2^-e
+    float lg, lg_next;   // bounds of X, read and written (ns_extra)
     int whole, split;    // tiles [0, whole) are computed by a workgroup each, the others in `split` pieces of their K steps
     float* slab;         // the pieces' sums
 };
@@ -409,7 +433,9 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
     constexpr bool SYM = KIND == NS_GRAM || KIND == NS_SQUARE;
     constexpr int SIDE = 32 * TW;
     auto chunk = [&](int i, int c) { return i * SIDE + 4 * (TW == 2 ? c ^ (i & 15) : c ^ (i >> 1 & 7)); };
-    const int r = lane & 31, h = lane >> 5;
+    const int r = lane & 31, h = lane >> 5, extra = KIND == NS_SQUARE ? 0 : ns_extra(u.x0, st.lg);
+    const float grown = KIND == NS_APPLY ? ldexpf(1.f, ns_extra(u.x0, st.lg_next) - extra) : KIND == NS_GRAM ? ldexpf(1.f, -2 * extra) : 1.f;
+    const float alpha = st.alpha * grown, beta = st.beta * grown, inv = KIND == NS_LAST ? ldexpf(st.inv, -extra) : 0.f;
 #pragma unroll
     for (int ti = 0; ti < TW; ++ti)
 #pragma unroll
@@ -418,7 +444,7 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
             for (int q = 0; q < 4; ++q) {
                 const f32x16& a = acc[ti][tj];
                 *(f32x4*)(img + chunk(32 * ti + r, 8 * tj + 2 * q + h)) =
-                    f32x4{st.alpha * a[4 * q], st.alpha * a[4 * q + 1], st.alpha * a[4 * q + 2], st.alpha * a[4 * q + 3]};
+                    f32x4{alpha * a[4 * q], alpha * a[4 * q + 1], alpha * a[4 * q + 2], alpha * a[4 * q + 3]};
             }
     __builtin_amdgcn_wave_barrier();
     const int iw = w.i0 + SIDE * wi, jw = w.j0 + SIDE * wj;
@@ -432,8 +458,8 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
             const f16x8 dh = *(const f16x8*)d, dl = *(const f16x8*)(d + NS_LO);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                v0[e] += st.beta * ((float)dh[e] + (float)dl[e]);
-                v1[e] += st.beta * ((float)dh[4 + e] + (float)dl[4 + e]);
+                v0[e] += beta * ((float)dh[e] + (float)dl[e]);
+                v1[e] += beta * ((float)dh[4 + e] + (float)dl[4 + e]);
             }
         }
         if constexpr (KIND == NS_SQUARE) {
@@ -448,8 +474,8 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (i == j + e && i < u.m) v0[e] += st.diagonal;
-                if (i == j + 4 + e && i < u.m) v1[e] += st.diagonal;
+                if (i == j + e && i < u.m()) v0[e] += st.diagonal;
+                if (i == j + 4 + e && i < u.m()) v1[e] += st.diagonal;
             }
         }
         if constexpr (KIND != NS_LAST) {
@@ -491,6 +517,7 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
         }
     } else if constexpr (KIND == NS_LAST) {
         constexpr int N = 16;
+        const bool trans = u.trans();
         for (int k0 = lane; k0 < SIDE * SIDE; k0 += 64 * N) {  // a batch's loads of the weights stand together
             long long x[N];
             float o[N], wt[N];
@@ -498,10 +525,10 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const int a = (k0 + 64 * e) / SIDE, b = (k0 + 64 * e) % SIDE;  // b runs along the result's rows
-                const int row = (u.trans ? jw : iw) + a, col = (u.trans ? iw : jw) + b;
+                const int row = (trans ? jw : iw) + a, col = (trans ? iw : jw) + b;
                 on[e] = row < u.rows && col < u.cols;
                 x[e] = (long long)row * u.cols + col;
-                o[e] = (u.trans ? at(b, a) : at(a, b)) * st.inv;
+                o[e] = (trans ? at(b, a) : at(a, b)) * inv;
             }
             if (u.out) {
 #pragma unroll
@@ -742,7 +769,7 @@ bool ns_small(int rows, int cols) {
 constexpr int ns_small_threads(int t32) { return t32 == 3 ? 512 : 1024; }
 
 struct NsCoefficients {
-    float c[3 * NS_MAX_STEPS];
+    float c[3 * NS_MAX_STEPS], lg[NS_MAX_STEPS + 1];
 };
 
 template <int T32, typename T, bool MOM>
@@ -789,7 +816,9 @@ __global__ __launch_bounds__(ns_small_threads(T32)) void ns_small_kernel(NsChunk
         }
     }
     sum = ns_block_sum<NT>(sum);
-    const double mul = (double)scale / (sqrt(sum) + (double)eps);
+    const NsNorm norm(sum, eps, scale);
+    const double mul = norm.mul;
+    const float x0 = norm.x0;
     for (int k = threadIdx.x; k < 2 * MP * LDX / 8; k += NT) *(f16x8*)(X + 8 * k) = f16x8{};
     __syncthreads();
     for (int k0 = 0; k0 < all; k0 += NT * N) {  // the momentum was written by this thread
@@ -803,7 +832,7 @@ __global__ __launch_bounds__(ns_small_threads(T32)) void ns_small_kernel(NsChunk
             if constexpr (MOM) {
                 if (zero) ((T*)u.in)[src[e]] = (T)0.f;
             }
-            const int row = row_of((int)at[e]), col = (int)at[e] - row * u.cols, x = u.trans ? col * LDX + row : row * LDX + col;
+            const int row = row_of((int)at[e]), col = (int)at[e] - row * u.cols, x = u.trans() ? col * LDX + row : row * LDX + col;
             ns_split((float)((double)b.update(mo, e) * mul), X[x], X[xlo + x]);
         }
     }
@@ -844,6 +873,8 @@ __global__ __launch_bounds__(ns_small_threads(T32)) void ns_small_kernel(NsChunk
     };
     for (int step = 0; step < steps; ++step) {
         const float a = co.c[3 * step], b = co.c[3 * step + 1], c = co.c[3 * step + 2];
+        const int extra = ns_extra(x0, co.lg[step]);
+        const float gram = ldexpf(inv, -2 * extra), grown = ldexpf(1.f, ns_extra(x0, co.lg[step + 1]) - extra);
         if constexpr (T32 == 1) {
             const int quarter = (u.np / 16 + 3) / 4 * 16;
             if (wave < 4) {
@@ -859,7 +890,7 @@ __global__ __launch_bounds__(ns_small_threads(T32)) void ns_small_kernel(NsChunk
 #pragma unroll
                     for (int w = 0; w < 4; ++w)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] += inv * scratch[(w * 16 + 4 * q + e) * 64 + lane];
+                        for (int e = 0; e < 4; ++e) v[e] += gram * scratch[(w * 16 + 4 * q + e) * 64 + lane];
                     put(A, alo, r * LDA + 8 * q + 4 * h, v);
                 }
             }
@@ -869,7 +900,7 @@ __global__ __launch_bounds__(ns_small_threads(T32)) void ns_small_kernel(NsChunk
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                     put(A, alo, (32 * (t / T32) + r) * LDA + 32 * (t % T32) + 8 * q + 4 * h,
-                        f32x4{inv * acc[4 * q], inv * acc[4 * q + 1], inv * acc[4 * q + 2], inv * acc[4 * q + 3]});
+                        f32x4{gram * acc[4 * q], gram * acc[4 * q + 1], gram * acc[4 * q + 2], gram * acc[4 * q + 3]});
             }
         }
         __syncthreads();
@@ -913,12 +944,13 @@ __global__ __launch_bounds__(ns_small_threads(T32)) void ns_small_kernel(NsChunk
                     const int x = (32 * i + r) * LDX + j0 + 8 * q + 4 * h;
                     f32x4 v;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = inv * acc[n][4 * q + e] + a * get(X, xlo, x, e);
+                    for (int e = 0; e < 4; ++e) v[e] = (grown * inv) * acc[n][4 * q + e] + (grown * a) * get(X, xlo, x, e);
                     put(X, xlo, x, v);
                 }
         }
         __syncthreads();
     }
+    const float back = ldexpf(inv, -ns_extra(x0, co.lg[steps]));
     for (int k0 = threadIdx.x; k0 < all; k0 += NT * N) {
         float wt[N];
         if (!u.out) {
@@ -929,8 +961,8 @@ __global__ __launch_bounds__(ns_small_threads(T32)) void ns_small_kernel(NsChunk
         for (int e = 0; e < N; ++e) {
             const int k = k0 + NT * e;
             if (k >= all) continue;
-            const int row = row_of(k), col = k - row * u.cols, x = u.trans ? col * LDX + row : row * LDX + col;
-            const float o = get(X, xlo, x, 0) * inv;
+            const int row = row_of(k), col = k - row * u.cols, x = u.trans() ? col * LDX + row : row * LDX + col;
+            const float o = get(X, xlo, x, 0) * back;
             if (u.out) ((T*)u.out)[k] = (T)o;
             else u.w[k] = u.decay * wt[e] - u.lr * o;
         }
@@ -947,10 +979,10 @@ __global__ __launch_bounds__(256) void ns_copy_kernel(NsTable tab, const char* w
     const f16_t* X = (const f16_t*)(ws + ns_x(u, 0));
     for (int k = threadIdx.x; k < NS_TILE_PREP * NS_TILE_PREP; k += 256) {
         const int i = i0 + k / NS_TILE_PREP, j = j0 + k % NS_TILE_PREP;
-        if (i >= u.m || j >= u.n) continue;
-        const long long at = u.trans ? (long long)j * u.cols + i : (long long)i * u.cols + j;
+        if (i >= u.m() || j >= u.n) continue;
+        const long long at = u.trans() ? (long long)j * u.cols + i : (long long)i * u.cols + j;
         const f16_t* from = X + ns_at(i, j, u.np);
-        const float o = ((float)from[0] + (float)from[NS_LO]) * inv;
+        const float o = ((float)from[0] + (float)from[NS_LO]) * ldexpf(inv, -ns_extra(u.x0, 0.f));
         if (u.out) ((T*)u.out)[at] = (T)o;
         else u.w[at] = u.decay * u.w[at] - u.lr * o;
     }
@@ -1029,7 +1061,7 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
         nparts += ns_parts(m * nn).second;
         prep += (m / NS_TILE_PREP + 1) * (nn / NS_TILE_PREP + 1);
     }
-    if (std::max(std::max(gt[0], ft[0]), std::max(nparts, prep)) > 0x3fffffffll) return V1T_ERR_UNSUPPORTED;
+    if (std::max(std::max(gt[0], ft[0]), std::max(nparts, prep)) >= (1 << 24)) return V1T_ERR_UNSUPPORTED;  // a launch has less than 2^32 threads
     if (n == 0) return V1T_OK;
     // the tiles with the longest K first: what is left for the last round is short
     std::sort(order.begin(), order.end(), [&](int a, int b) { return size[a] != size[b] ? size[a] > size[b] : a < b; });
@@ -1047,9 +1079,8 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
     for (int k = 0; k < n; ++k) {
         NsUnit u{};
         shape(order[k], u.rows, u.cols);
-        u.trans = u.rows > u.cols;
-        u.m = std::min(u.rows, u.cols); u.n = std::max(u.rows, u.cols);
-        u.mp = round_up(u.m, NS_BK); u.np = round_up(u.n, NS_BK);
+        u.n = std::max(u.rows, u.cols);
+        u.mp = round_up(std::min(u.rows, u.cols), NS_BK); u.np = round_up(u.n, NS_BK);
         u.base = at;
         at = ns_square_at(u, l.pairs ? 4 : 2);
         const auto ps = ns_parts((long long)u.rows * u.cols);
@@ -1083,54 +1114,62 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
 }
 
 // The exponent of the planes' common scale: 2^15 over the largest number of any plane. A step maps a singular value s in [0, top] to a s + b s^3 + c s^5;
-// X, A = X X^T, S and, where steps are taken in pairs, T, the next A, S' and Q are bounded by their spectral norms. The maxima are sampled, 0.1 % of a
+// X, A = X X^T, S and, where steps are taken in pairs, T, the next A, S' and Q are bounded by their spectral norms. lg: before each step (and behind the last),
+// the logarithm of the product of the largest factors a + b s^2 + c s^4 so far. The maxima are sampled, 0.1 % of a
 // singular value and 1 % of the rest are added for what lies between the samples and for rounding.
-bool ns_exponent_of(const float* coefficients, int steps, bool pairs, int* exponent) {
-    double top = 1.001, most = top;
+struct NsScale {
+    int exponent = 0;
+    float lg[NS_MAX_STEPS + 1] = {};
+};
+bool ns_scale_of(const float* coefficients, int steps, bool pairs, NsScale& scale) {
+    double top = 1.001, most = top, lg = 0.0;
     for (int k = 0; k < steps; ++k) {
         const float* f = coefficients + 3 * k;
         for (int e = 0; e < 3; ++e)
             if (!std::isfinite(f[e])) return false;
         const bool pair = pairs && k + 1 < steps;
-        double next = 0.0;
+        double next = 0.0, factor = std::ldexp(1.0, -20);
+        scale.lg[k] = (float)lg;
         for (int i = 0; i <= 4096; ++i) {
             const double s = top * i / 4096.0, t = s * s, poly = t * (f[1] + t * f[2]);
-            double end = s * (f[0] + poly);
+            double by = f[0] + poly;
             most = std::max({most, t, std::fabs(poly)});
             if (pair) {
-                const double a1 = f[3], t1 = end * end, poly1 = t1 * (f[4] + t1 * f[5]);
-                most = std::max({most, std::fabs(t * (f[0] + poly)), t1, std::fabs(poly1), std::fabs((a1 + poly1) * (f[0] + poly)),
-                                 std::fabs((a1 + poly1) * (f[0] + poly) - a1 * f[0])});
-                end *= a1 + poly1;
+                const double a1 = f[3], t1 = t * by * by, poly1 = t1 * (f[4] + t1 * f[5]);
+                most = std::max({most, std::fabs(t * by), t1, std::fabs(poly1), std::fabs((a1 + poly1) * by), std::fabs((a1 + poly1) * by - a1 * f[0])});
+                by *= a1 + poly1;
             }
-            next = std::max(next, std::fabs(end));
+            next = std::max(next, std::fabs(s * by));
+            factor = std::max(factor, std::fabs(by));
         }
-        if (pair) ++k;
+        if (pair) scale.lg[++k] = (float)lg;  // not asked for
+        lg += std::log2(1.01 * factor);
         top = 1.001 * next;
         most = std::max(most, top);
         if (!(most < 128.0)) return false;
     }
-    *exponent = (int)std::floor(std::log2(32768.0 / (1.01 * most)));
+    scale.lg[steps] = (float)lg;
+    scale.exponent = (int)std::floor(std::log2(32768.0 / (1.01 * most)));
     return true;
 }
 
-// the same, remembered for the coefficients of the calling thread's last calls (the samples cost more than the launches)
-bool ns_exponent(const float* coefficients, int steps, bool pairs, int* exponent) {
+// the same, remembered for the coefficients of the calling thread's last calls (the samples cost more than the launches); nullptr: refused
+const NsScale* ns_scale(const float* coefficients, int steps, bool pairs) {
     struct Known {
         float c[3 * NS_MAX_STEPS];
-        int steps = -1, exponent = 0;
+        int steps = -1;
         bool ok = false;
+        NsScale scale;
     };
     static thread_local Known known[2];
     Known& k = known[pairs];
     if (k.steps != steps || (steps > 0 && std::memcmp(k.c, coefficients, sizeof(float) * 3 * steps) != 0)) {
         k.steps = -1;
-        k.ok = ns_exponent_of(coefficients, steps, pairs, &k.exponent);
+        k.ok = ns_scale_of(coefficients, steps, pairs, k.scale);
         if (steps > 0) std::memcpy(k.c, coefficients, sizeof(float) * 3 * steps);
         k.steps = steps;
     }
-    *exponent = k.exponent;
-    return k.ok;
+    return k.ok ? &k.scale : nullptr;
 }
 
 template <int KIND, typename T>
@@ -1158,14 +1197,14 @@ NsStep ns_square(int out, int p, int q, float alpha, int d, float beta, int d2 =
 }
 
 template <typename T>
-int ns_steps(const NsLayout& l, const NsTable& table, char* ws, int steps, const float* co, bool pairs, int exponent, hipStream_t s) {
+int ns_steps(const NsLayout& l, const NsTable& table, char* ws, int steps, const float* co, bool pairs, const NsScale& scale, hipStream_t s) {
     enum { A = 0, S = 1, U = 2, S1 = 3 };  // the m x m matrices; U holds T, then Q
-    const float inv = std::ldexp(1.f, -exponent);
+    const float inv = std::ldexp(1.f, -scale.exponent);
     int from = 0;
     for (int k = 0; k < steps; ++k) {
         const float a = co[3 * k], b = co[3 * k + 1], c = co[3 * k + 2];
         NsStep st{};
-        st.alpha = inv; st.from = from; st.inv = inv;
+        st.alpha = inv; st.from = from; st.inv = inv; st.lg = scale.lg[k];
         NS_TRY((ns_gemm<NS_GRAM, float>(l, table, ws, st, s)));
         NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, ws, ns_square(S, A, A, c * inv, A, b), s)));
         st.p = S; st.beta = a;
@@ -1174,10 +1213,11 @@ int ns_steps(const NsLayout& l, const NsTable& table, char* ws, int steps, const
             NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, ws, ns_square(U, S, A, inv, A, a), s)));
             NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, ws, ns_square(A, S, U, inv, U, a), s)));
             NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, ws, ns_square(S1, A, A, c1 * inv, A, b1), s)));
-            NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, ws, ns_square(U, S1, S, inv, S, a1, S1, a, k == 0 ? 0.f : std::ldexp(a * a1, exponent)), s)));
+            NS_TRY((ns_gemm<NS_SQUARE, float>(l, table, ws, ns_square(U, S1, S, inv, S, a1, S1, a, k == 0 ? 0.f : std::ldexp(a * a1, scale.exponent)), s)));
             st.p = U; st.beta = k == 0 ? a * a1 : 0.f;
             ++k;
         }
+        st.lg_next = scale.lg[k + 1];
         if (k + 1 < steps) NS_TRY((ns_gemm<NS_APPLY, float>(l, table, ws, st, s)));
         else NS_TRY((ns_gemm<NS_LAST, T>(l, table, ws, st, s)));
         from ^= 1;
@@ -1187,9 +1227,11 @@ int ns_steps(const NsLayout& l, const NsTable& table, char* ws, int steps, const
 
 template <typename T, bool MOM>
 int ns_run(const NsLayout& l, int n, char* ws, const NsMomentum& mo, float eps, int zero, int steps, const float* co, hipStream_t s) {
-    int exponent = 0;
-    const bool pairs = l.pairs && ns_exponent(co, steps, true, &exponent);  // coefficients whose pairs would leave the planes' range go step by step
-    if (!pairs && !ns_exponent(co, steps, false, &exponent)) return V1T_ERR_ARG;
+    const NsScale* paired = l.pairs ? ns_scale(co, steps, true) : nullptr;  // coefficients whose pairs would leave the planes' range go step by step
+    const NsScale* scale = paired ? paired : ns_scale(co, steps, false);
+    if (!scale) return V1T_ERR_ARG;
+    const bool pairs = paired != nullptr;
+    const int exponent = scale->exponent;
     const NsTable table{(const NsUnit*)(ws + l.table), (const ns_head*)(ws + l.heads), n};
     double* parts = (double*)(ws + l.parts);
     hipLaunchKernelGGL((ns_norm_kernel<T, MOM>), dim3(l.nparts), dim3(256), 0, s, table, mo, parts);
@@ -1199,7 +1241,7 @@ int ns_run(const NsLayout& l, int n, char* ws, const NsMomentum& mo, float eps, 
         hipLaunchKernelGGL((ns_copy_kernel<T>), dim3(l.nprep), dim3(256), 0, s, table, ws, std::ldexp(1.f, -exponent));
         return hipGetLastError() == hipSuccess ? V1T_OK : V1T_ERR_LAUNCH;
     }
-    return ns_steps<T>(l, table, ws, steps, co, pairs, exponent, s);
+    return ns_steps<T>(l, table, ws, steps, co, pairs, *scale, s);
 }
 
 // the matrices that go through the products, by their numbers
@@ -1235,10 +1277,12 @@ int ns_call(int n, Shape shape, Fill fill, const NsMomentum& mo, float eps, int 
     NS_TRY(ns_layout_large(large, shape, l));
     if (!workspace || ws_bytes < l.bytes) return V1T_ERR_WORKSPACE;
     if ((uintptr_t)workspace & 15) return V1T_ERR_ARG;
-    int exponent = 0;
-    if (!ns_exponent(co, steps, false, &exponent)) return V1T_ERR_ARG;
+    const NsScale* scale = ns_scale(co, steps, false);
+    if (!scale) return V1T_ERR_ARG;
+    const int exponent = scale->exponent;
     NsCoefficients cs{};
     for (int i = 0; i < 3 * steps; ++i) cs.c[i] = co[i];
+    for (int i = 0; i <= steps; ++i) cs.lg[i] = scale->lg[i];
     NsChunk c;
     for (int t32 = 1; t32 <= 3; ++t32) {
         int k = 0;
@@ -1247,9 +1291,8 @@ int ns_call(int n, Shape shape, Fill fill, const NsMomentum& mo, float eps, int 
             bool mine = false;
             if (i < n) {
                 shape(i, u.rows, u.cols);
-                u.m = std::min(u.rows, u.cols); u.n = std::max(u.rows, u.cols);
-                u.mp = round_up(u.m, 32); u.np = round_up(u.n, 32);
-                u.trans = u.rows > u.cols;
+                u.n = std::max(u.rows, u.cols);
+                u.mp = round_up(std::min(u.rows, u.cols), 32); u.np = round_up(u.n, 32);
                 mine = u.mp == 32 * t32 && ns_small(u.rows, u.cols);
             }
             if (mine) {
@@ -1303,8 +1346,7 @@ extern "C" long long v1t_orthogonalize_ws_bytes(const int* rows, const int* cols
 extern "C" int v1t_orthogonalize(const v1t_matrix* units, int n, int dtype, int steps, const float* coefficients, float eps, void* workspace, long long ws_bytes,
                                  void* stream) {
     if (n < 0 || (n > 0 && !units) || dtype < 0 || dtype > 2 || steps < 0 || steps > NS_MAX_STEPS || (steps > 0 && !coefficients) || !(eps >= 0.f)) return V1T_ERR_ARG;
-    int exponent = 0;
-    if (!ns_exponent(coefficients, steps, false, &exponent)) return V1T_ERR_ARG;
+    if (!ns_scale(coefficients, steps, false)) return V1T_ERR_ARG;
     for (int i = 0; i < n; ++i)
         if (!units[i].in || !units[i].out) return V1T_ERR_ARG;
     if (n == 0) return V1T_OK;
@@ -1320,8 +1362,7 @@ extern "C" int v1t_orthogonalize(const v1t_matrix* units, int n, int dtype, int 
 extern "C" int v1t_muon_step(const v1t_muon_range* units, int n, float momentum, int nesterov, int steps, const float* coefficients, float eps, int zero_grad,
                              void* workspace, long long ws_bytes, void* stream) {
     if (n < 0 || (n > 0 && !units) || steps < 0 || steps > NS_MAX_STEPS || (steps > 0 && !coefficients) || !(eps >= 0.f) || !std::isfinite(momentum)) return V1T_ERR_ARG;
-    int exponent = 0;
-    if (!ns_exponent(coefficients, steps, false, &exponent)) return V1T_ERR_ARG;
+    if (!ns_scale(coefficients, steps, false)) return V1T_ERR_ARG;
     for (int i = 0; i < n; ++i)
         if (!units[i].p || !units[i].g || !units[i].m) return V1T_ERR_ARG;
     if (n == 0) return V1T_OK;
