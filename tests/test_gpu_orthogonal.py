@@ -255,6 +255,50 @@ def test_muon_step_captured_and_replayed():
         assert all(torch.equal(a, b) for a, b in zip(ps + ms + o, qs + ns + want))
 
 
+@pytest.mark.parametrize("trans", [False, True])
+def test_the_longest(trans):
+    """2^31 - 2^22 elements: byte offsets past 2^32. The iterates in 64 bits are Q X with Q of the short side, so that some columns stand for all. Gaussian rows are all but
+    orthogonal: every singular value is near 1 / sqrt(511) and ends near one, 23 times as large, as do the roundings of 15 products (and half a step of the result's type)."""
+    m, n = 511, 1 << 22
+    g = torch.Generator(device=DEV).manual_seed(11)
+    u = torch.randn((n, m) if trans else (m, n), device=DEV, generator=g, dtype=torch.bfloat16)
+    o = v1t_amd.orthogonalize(u)
+    x, y = (u.t(), o.t()) if trans else (u, o)
+    gram = torch.zeros(m, m, dtype=torch.float64, device=DEV)
+    for c in range(0, n, 1 << 18):
+        part = x[:, c:c + (1 << 18)].double().contiguous()
+        gram += part @ part.t().contiguous()
+    norm = gram.trace().sqrt()
+    q = torch.eye(m, dtype=torch.float64, device=DEV) / norm
+    a, b, c = COEFFICIENTS
+    for _ in range(5):
+        s = q @ gram @ q.t()
+        q = (a * torch.eye(m, dtype=torch.float64, device=DEV) + b * s + c * (s @ s)) @ q
+    for at in (0, 1 << 20, (1 << 21) + 12345, n - 300):
+        want, got = q @ x[:, at:at + 300].double().contiguous(), y[:, at:at + 300].double()
+        assert float((got - want).norm() / want.norm()) <= 2**-8 + 23 * 15 * 4 * 2**-22
+
+
+def test_the_widest():
+    """32768 x 65536 with one number in each row, in columns of their own: the singular values are the numbers', the result has one in each row's place, too. Two steps,
+    each a few roundings of 2^-22 of the value and its factors."""
+    m, n = 1 << 15, 1 << 16
+    g = torch.Generator(device=DEV).manual_seed(12)
+    cols, d = torch.randperm(n, device=DEV, generator=g)[:m], torch.rand(m, device=DEV, generator=g) + 0.5
+    u = torch.zeros(m, n, device=DEV)
+    rows = torch.arange(m, device=DEV)
+    u[rows, cols] = d
+    s = d.double() / d.double().norm()
+    o = v1t_amd.orthogonalize(u, steps=2)
+    a, b, c = COEFFICIENTS
+    for _ in range(2):
+        s = a * s + b * s**3 + c * s**5
+    got = o[rows, cols].double()
+    assert float(((got - s) / s).abs().max()) <= 2 * 8 * 2**-22 + 1e-7 / float(d.norm())
+    o[rows, cols] = 0.0
+    assert not bool(o.any())
+
+
 def test_two_streams_at_once():
     us = [update(300, 200, i) for i in range(4)]
     want = v1t_amd.orthogonalize(us)
