@@ -23,10 +23,13 @@ namespace {
 constexpr int ROT_MAX_PAIRS = 256;
 constexpr int ROT_THREADS = 256;
 
-struct RotRates {  // kernel argument: a captured graph keeps it, no device memory behind it
-    double turns[ROT_MAX_PAIRS];
-    unsigned char axis[ROT_MAX_PAIRS];
+template <int P>
+struct RotRates {  // kernel argument: a captured graph keeps it, no device memory behind it. P: 64 where they suffice - a launch copies all of it; 2.3 KB cost a
+                   // small training pass of two launches 8 of 160 us
+    double turns[P];
+    unsigned char axis[P];
 };
+using RotAllRates = RotRates<ROT_MAX_PAIRS>;
 
 struct RotArgs {
     const void* x[2];
@@ -96,8 +99,8 @@ struct Slot {
     }
 };
 
-template <typename T, bool HALVES, typename P>
-__global__ __launch_bounds__(ROT_THREADS, 4) void rotary_kernel(RotArgs g, RotRates rates) {
+template <typename T, bool HALVES, typename P, int R>
+__global__ __launch_bounds__(ROT_THREADS, 4) void rotary_kernel(RotArgs g, RotRates<R> rates) {
     const int t = threadIdx.x / g.slots, v = threadIdx.x - t * g.slots, t0 = blockIdx.x * g.nt;
     const bool mine = t < g.nt && t0 + t < g.T;
     using Part = Slot<T, HALVES>;
@@ -207,16 +210,23 @@ unsigned division_multiplier(long long d, long long limit) {
     return e && (unsigned long long)limit > ((1ull << 32) - 1) / e ? 0 : (unsigned)m;
 }
 
-template <typename T, bool HALVES>
-int launch_p(const RotArgs& a, const RotRates& r, int pos_type, dim3 grid, hipStream_t s) {
-    if (pos_type == 0) hipLaunchKernelGGL((rotary_kernel<T, HALVES, int>), grid, dim3(ROT_THREADS), 0, s, a, r);
-    else if (pos_type == 1) hipLaunchKernelGGL((rotary_kernel<T, HALVES, long long>), grid, dim3(ROT_THREADS), 0, s, a, r);
-    else hipLaunchKernelGGL((rotary_kernel<T, HALVES, float>), grid, dim3(ROT_THREADS), 0, s, a, r);
+template <typename T, bool HALVES, int R>
+int launch_p(const RotArgs& a, const RotAllRates& all, int pos_type, dim3 grid, hipStream_t s) {
+    RotRates<R> r;
+    std::copy_n(all.turns, R, r.turns);
+    std::copy_n(all.axis, R, r.axis);
+    if (pos_type == 0) hipLaunchKernelGGL((rotary_kernel<T, HALVES, int, R>), grid, dim3(ROT_THREADS), 0, s, a, r);
+    else if (pos_type == 1) hipLaunchKernelGGL((rotary_kernel<T, HALVES, long long, R>), grid, dim3(ROT_THREADS), 0, s, a, r);
+    else hipLaunchKernelGGL((rotary_kernel<T, HALVES, float, R>), grid, dim3(ROT_THREADS), 0, s, a, r);
     return hipGetLastError() == hipSuccess ? V1T_OK : V1T_ERR_LAUNCH;
 }
+template <typename T, bool HALVES>
+int launch_r(const RotArgs& a, const RotAllRates& r, int pos_type, dim3 grid, hipStream_t s) {
+    return a.pairs <= 64 ? launch_p<T, HALVES, 64>(a, r, pos_type, grid, s) : launch_p<T, HALVES, ROT_MAX_PAIRS>(a, r, pos_type, grid, s);
+}
 template <typename T>
-int launch_t(const RotArgs& a, const RotRates& r, int halves, int pos_type, dim3 grid, hipStream_t s) {
-    return halves ? launch_p<T, true>(a, r, pos_type, grid, s) : launch_p<T, false>(a, r, pos_type, grid, s);
+int launch_t(const RotArgs& a, const RotAllRates& r, int halves, int pos_type, dim3 grid, hipStream_t s) {
+    return halves ? launch_r<T, true>(a, r, pos_type, grid, s) : launch_r<T, false>(a, r, pos_type, grid, s);
 }
 
 }  // namespace
@@ -234,7 +244,7 @@ extern "C" int v1t_rotary(const v1t_rotary_operand* ops, int n_ops, int dtype, i
     if (pairs < 1 || 2 * pairs > D) return V1T_ERR_ARG;
     if (pairs > ROT_MAX_PAIRS) return V1T_ERR_UNSUPPORTED;
     RotArgs g{};
-    RotRates r{};
+    RotAllRates r{};
     for (int a = 0, j = 0; a < n_axes; ++a)
         for (int i = 0; i < sections[a]; ++i, ++j) {
             const double part = shared ? (double)j / (double)pairs : (double)i / (double)sections[a];

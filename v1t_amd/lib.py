@@ -215,18 +215,16 @@ def require_cuda(x: torch.Tensor, what: str) -> None:
         raise RuntimeError(f"v1t_amd {what}: tensor is on {x.device}; the HIP path needs a GPU tensor (no CPU fallback).")
 
 
-def leaf_in_capture(x: torch.Tensor, what: str) -> None:
-    """Called by an operator's differentiable forward for each tensor it saves a gradient path to. The node that receives a leaf's gradient belongs to
+def leaves_in_capture(out: torch.Tensor, what: str) -> None:
+    """Called by an operator with its differentiable result. The node that receives a leaf's gradient belongs to
     the stream of the first pass that used the leaf, for as long as any graph of that pass lives; a backward pass captured meanwhile on another
     stream would wait on that stream inside the capture, which ends the process when the capture ends. So an eager pass marks the node with its
     stream, and a captured pass that finds another stream's mark is refused."""
-    if not (x.is_leaf and x.requires_grad):
-        return
-    here = stream_of(x.get_device())
-    made_on = torch.autograd.graph.get_gradient_edge(x).node.metadata.setdefault("v1t_stream", here)
-    if made_on != here and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"v1t_amd {what}: a graph of an earlier pass over the same leaf tensor is still alive on another stream; its backward cannot be "
-                           "captured beside it. Drop that pass's outputs (del) before the capture.")
+    here = stream_of(out.get_device())
+    for node, _ in out.grad_fn.next_functions:
+        if hasattr(node, "variable") and node.metadata.setdefault("v1t_stream", here) != here and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"v1t_amd {what}: a graph of an earlier pass over the same leaf tensor is still alive on another stream; its backward cannot be "
+                               "captured beside it. Drop that pass's outputs (del) before the capture.")
 
 
 def grad_sink(p):

@@ -91,11 +91,11 @@ def _sections(sections: t.Tuple[int, ...]):
 
 
 def _like(x: torch.Tensor) -> torch.Tensor:
-    """x's shape with room for a multiple of 8 features a head: what lies behind the last whole 8 is moved as one store, too. Not a view of the wider tensor but
-    one over its storage: autograd lets a view that a function returns not be changed in place."""
+    """x's shape with room for a multiple of 8 features a head: what lies behind the last whole 8 is moved as one store, too. `.data`: a
+    tensor of its own over the wider one's storage; autograd lets a view that a function returns not be changed in place."""
     shape, d = x.shape, x.shape[-1]
     y = torch.empty((*shape[:-1], (d + 7) // 8 * 8), dtype=x.dtype, device=x.device)
-    return y if d % 8 == 0 else torch.empty(0, dtype=x.dtype, device=x.device).set_(y.untyped_storage(), 0, shape, y.stride())
+    return y if d % 8 == 0 else y.narrow(-1, 0, d).data
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -107,9 +107,6 @@ class _RotaryFn(torch.autograd.Function):
     def forward(ctx, turn: _Turn, positions: torch.Tensor, q: torch.Tensor, k: t.Optional[torch.Tensor]):
         ctx.set_materialize_grads(False)
         ctx.turn = turn
-        for x in (q, k):
-            if x is not None:
-                L.leaf_in_capture(x, "rotary")
         ctx.save_for_backward(positions)
         xs = [_rows(x) for x in (q, k) if x is not None]
         ys = [_like(x) for x in xs]
@@ -120,7 +117,8 @@ class _RotaryFn(torch.autograd.Function):
     def backward(ctx, *grads):
         """A rotation is orthogonal: the gradient turns back. Differentiable itself (a second derivative turns forward again)."""
         (positions,) = ctx.saved_tensors
-        back = ctx.turn._replace(inverse=1 - ctx.turn.inverse)
+        sections, base, shared, halves, inverse = ctx.turn
+        back = _Turn(sections, base, shared, halves, 1 - inverse)
         out: t.List[t.Optional[torch.Tensor]] = [None, None]
         which = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[2 + i]]
         if not torch.is_grad_enabled():
@@ -131,10 +129,18 @@ class _RotaryFn(torch.autograd.Function):
             for i, y in zip(which, ys):
                 out[i] = y
         elif len(which) == 2:
-            out = list(_RotaryFn.apply(back, positions, *grads))
+            out = list(_apply(back, positions, *grads))
         elif which:
-            out[which[0]] = _RotaryFn.apply(back, positions, grads[which[0]], None)
+            out[which[0]] = _apply(back, positions, grads[which[0]], None)
         return (None, None, *out)
+
+
+def _apply(turn: _Turn, positions: torch.Tensor, q: torch.Tensor, k: t.Optional[torch.Tensor]):
+    out = _RotaryFn.apply(turn, positions, q, k)
+    first = out if k is None else out[0]
+    if first.requires_grad:
+        L.leaves_in_capture(first, "rotary")
+    return out
 
 
 def rotary(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int], k: t.Optional[torch.Tensor] = None, base: float = 10000.0,
@@ -153,7 +159,7 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int
     L.require_cuda(q, "rotary")
     turn = _Turn(sections, float(base), int(bool(shared)), _LAYOUTS[layout], int(bool(inverse)))
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _RotaryFn.apply(turn, positions, q, k)
+        return _apply(turn, positions, q, k)
     xs = [_rows(x) for x in (q, k) if x is not None]
     ys = [_like(x) for x in xs]
     _launch(turn, positions, list(zip(xs, ys)))
