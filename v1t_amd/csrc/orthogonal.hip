@@ -17,6 +17,11 @@
 // matrices - are 2^floor(x0 - lg_k) larger, if that is more than one (ns_extra). A and S, small against a, need no more.
 //
 // All matrices of a call ("units") go through each product in one launch: the shared core's matrices are small, and launches are what they cost.
+//
+// Bound: the matrix cores of large matrices, at the rate that power leaves them - a product of 4096 x 4096 in 355 us, 1.16 PFLOP/s of fp16 operations (three a
+// product), pipes busy 64 % of the time at 1.63 GHz; torch's fp16 product reaches 1.33 PFLOP/s - and launch after launch of small ones: 8 us for each of the
+// default core's 15 products, whose operations take 1. Whole calls, five steps: 4096 x 4096 bf16 3.86 ms, 8192 x 1024 fp32 478 us, twelve 777 x 1301 fp16 889 us,
+// the default core's 24 matrices 141 us, one block of width 2048 (a momentum step over 4 matrices, 200 MB of weights) 4.32 ms, one 155 x 64 33 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -371,8 +376,8 @@ DEVFN int ns_deal(int local, int first, int count) {
 }
 typedef f16_t f16x4 __attribute__((ext_vector_type(4)));
 
-// Stages of the ring: two where two or more workgroups share a CU and cover each other's waits; four for the 64 tile of symmetric products, whose launches have few of
-// them; three for the 192 tile, alone on its CU
+// Stages of the ring: two where two or more workgroups share a CU and cover each other's waits (the default core's products back on X: 8.7 us, with four 10.8); four for the 64
+// tile of symmetric products, whose launches have few of them (1024 x 1024: 14.3 us, with two 20.2); three for the 192 tile, alone on its CU
 template <int TW, bool SYM>
 struct NsTile {
     static constexpr int B = 64 * TW, PL = 2 * B * NS_BK, SIDE = 32 * TW;  // PL: elements of an operand's stage, hi and lo
@@ -756,7 +761,7 @@ __global__ __launch_bounds__(64) void ns_join_kernel(NsTable tab, char* ws, NsSt
 
 // ---- small matrices -----------------------------------------------------------------------
 // A matrix whose planes fit a CU's LDS goes through all its steps in one workgroup: what the products above cost there is their launches (155 x 64:
-// 18 launches, 75 us; this 19). X, A and S lie in LDS as two planes each, rows 16 B longer than their numbers, so that neighbouring rows start in other
+// 18 launches, 105 us; this 33: 15 products one behind the other, each a few dependent MFMAs and a barrier). X, A and S lie in LDS as two planes each, rows 16 B longer than their numbers, so that neighbouring rows start in other
 // banks. The waves share the 32 x 32 tiles of A, S and X; a single tile of A
 // is computed in quarters of K by four of them.
 constexpr int NS_LDS = 150 * 1024, NS_PAD = 8, NS_SCRATCH = 4 * 32 * 32 * 4;
@@ -1009,10 +1014,11 @@ std::pair<int, int> ns_parts(long long elements) {
     return {(int)part, (int)((elements + part - 1) / part)};
 }
 
-// Tile and split of a product with t64 / t128 tiles of each size whose K steps sum to k64 / k128, at the least estimated time. A CU holds two workgroups of
-// either tile. Measured, us per K step: the larger tile 1.6 with two on a CU and 0.9 alone, the smaller 0.85 and 0.25 (so the larger does twice
-// the work in a time, where there is enough of it), their epilogues 5 and 1.5; the launch that joins pieces 6, and their sums at 3 TB/s. Only the tiles of the last, part-filled round
-// are split, in pieces of at least 4 steps.
+// Tile (64, 128 or 192) and split of a product with t[.] tiles of each size whose K steps sum to k[.], at the least estimated time. A CU holds two workgroups of
+// the smaller tiles, one of the largest. Measured, us per K step and round: 64 0.25 alone on its CU and 0.85 by two, 128 0.9 and 1.6, 192 1.6 (so 128 does twice the work
+// of 64 in a time, where there is enough of it; 192 does 1.13 times that of 128 where it fills the chip once, 2.25 times where 128 would leave one a CU), epilogues 1.5, 5
+// and 9; the launch that joins pieces 6, and their sums at 3 TB/s. Only the tiles of the last, part-filled round are split, in pieces of at least 4 steps:
+// 8192 x 1024's Gram matrix, 36 tiles of 128 in seven pieces each, takes 36 us and 12 to join them; as 136 whole tiles of 64 it took 107.
 NsPlan ns_plan(const long long (&t)[3], const long long (&k)[3], bool may_split) {
     constexpr int CUS = 256;
     constexpr double FULL[3] = {0.85, 1.6, 1.6}, ALONE[3] = {0.25, 0.9, 1.6}, TAIL[3] = {1.5, 5.0, 9.0};
@@ -1068,7 +1074,8 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
     l.gram = ns_plan(gt, gk, true);
     l.poly = ns_plan(gt, pk, true);
     l.full = ns_plan(ft, fk, false);
-    // two steps: gram, poly, full each twice, or gram, five m x m products, full; 3 us a launch
+    // two steps: gram, poly, full each twice, or gram, five m x m products, full; 3 us a launch. 8192 x 1024: 561 us in pairs, 686 step by step; 4096 x 4096's products are
+    // all of one size, and it stays step by step
     l.pairs = l.gram.us + 5 * l.poly.us + l.full.us + 21.0 < 0.9 * (2 * (l.gram.us + l.poly.us + l.full.us) + 18.0);
     l.table = 0;
     l.heads = ns_align((long long)n * (long long)sizeof(NsUnit));

@@ -3,10 +3,12 @@
 //     y0 = x0 cos - x1 sin,  y1 = x0 sin + x1 cos        (backward: the same with the angle negated - a rotation's transpose is its inverse)
 // Features behind the 2 * pairs rotated ones pass through. One pass: every element is read once and written once.
 //
-// Bound: HBM (2 B of flops per byte). A thread owns a "slot" of 4 pairs of one token - 16 B of 16-bit features - and with it 4 angles, whose cosines and
+// Bound: HBM (less than one operation a byte). A thread owns a "slot" of 4 pairs of one token - 16 B of 16-bit features - and with it 4 angles, whose cosines and
 // sines stay in its registers while it walks over the heads of q and of k, and over the sequences of its batch chunk where these share their positions:
 // the angle, a 64-bit product (below), costs as much as several slots' traffic, and the walk costs two address additions a slot. Four heads' loads
-// stand together.
+// stand together. Measured: q and k of 112 x 1654 tokens, 4 + 4 heads x 155 bf16 out of a padded projection into rows with room for 160 (919 MB) 192 us,
+// 4.8 TB/s, where a copy of as much takes 176 us (an angle per slot: 348 us; without room, the last features one by one: 40 % more); one sequence of 39 672 tokens,
+// 16 + 4 heads x 128 bf16 (406 MB) 84 us, 4.8 TB/s; one token of 8 streams 5 us of which nothing is traffic.
 //
 // Numerics: the angle is held as a number of turns in 64 bits, p * (rate / 2 pi), and reduced to [-1/2, 1/2] before it is rounded to 32: a
 // 32-bit product is off by 0.03 rad at position 10^6. Products and sums of the rotation are fp32, rounded once to the tensor's type.
