@@ -523,6 +523,39 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
     } else if constexpr (KIND == NS_LAST) {
         constexpr int N = 16;
         const bool trans = u.trans();
+        const int row0 = trans ? jw : iw, col0 = trans ? iw : jw;
+        if (row0 + SIDE <= u.rows && col0 + SIDE <= u.cols) {  // all of it: runs of 4
+            typedef T t4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+            typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+            constexpr int R = 4;
+            for (int k0 = 4 * lane; k0 < SIDE * SIDE; k0 += 256 * R) {
+                long long x[R];
+                f32x4 o[R];
+                f4 wt[R];
+#pragma unroll
+                for (int q = 0; q < R; ++q) {
+                    const int a = (k0 + 256 * q) / SIDE, b = (k0 + 256 * q) % SIDE;
+                    x[q] = (long long)(row0 + a) * u.cols + col0 + b;
+                    if (!u.out) wt[q] = *(const f4*)(u.w + x[q]);
+                    if (trans) o[q] = f32x4{at(b, a), at(b + 1, a), at(b + 2, a), at(b + 3, a)};
+                    else o[q] = *(const f32x4*)(img + chunk(a, b / 4));
+                }
+#pragma unroll
+                for (int q = 0; q < R; ++q) {
+                    t4 r;
+                    f4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float y = o[q][e] * inv;
+                        r[e] = (T)y;
+                        if (!u.out) v[e] = u.decay * wt[q][e] - u.lr * y;
+                    }
+                    if (u.out) *(t4*)((T*)u.out + x[q]) = r;
+                    else *(f4*)(u.w + x[q]) = v;
+                }
+            }
+            return;
+        }
         for (int k0 = lane; k0 < SIDE * SIDE; k0 += 64 * N) {  // a batch's loads of the weights stand together
             long long x[N];
             float o[N], wt[N];
@@ -530,7 +563,7 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const int a = (k0 + 64 * e) / SIDE, b = (k0 + 64 * e) % SIDE;  // b runs along the result's rows
-                const int row = (trans ? jw : iw) + a, col = (trans ? iw : jw) + b;
+                const int row = row0 + a, col = col0 + b;
                 on[e] = row < u.rows && col < u.cols;
                 x[e] = (long long)row * u.cols + col;
                 o[e] = (trans ? at(b, a) : at(a, b)) * inv;
