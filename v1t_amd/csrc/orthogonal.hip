@@ -612,21 +612,22 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(NsTable t
     // A 1-KB piece fills 64 16-B chunks of a stage in order; which 16 B of the tile's row a chunk holds is swizzled, so that the fragment reads below spread over all
     // 64 banks. Rows [.][32 hi, 32 lo]: eight chunks a row, chunk c at c ^ (row / 2 % 8). Q as [k][j]: the row's 64-B granules (32 hi or lo) g at g ^ (k % 4). A lane's
     // byte offset from the tile's first row is loop-invariant; pieces 1 .. 3 of a group of four go by the instruction's offset, which moves the LDS and the global
-    // address alike: the lane offset carries 1024 (p % 4) less, the base 3072 less.
+    // address alike: the lane offset carries BIAS - 1024 (p % 4), the base BIAS less.
+    constexpr int BIAS = TileDma<32, 32>::BIAS;
     unsigned po[PIECES], qo[PIECES];
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-        const int c = 64 * (wave * PIECES + p) + lane, row = c / 8, at = 3072 - 1024 * (p & 3) + 16 * ((c & 7) ^ (row >> 1 & 7));
+        const int c = 64 * (wave * PIECES + p) + lane, row = c / 8, at = BIAS - 1024 * (p & 3) + 16 * ((c & 7) ^ (row >> 1 & 7));
         po[p] = (unsigned)min(row, u.mp - 1 - w.i0) * (unsigned)(4 * ldp) + at;
         if constexpr (TR) {
             const int k = c / (B / 4), g = (c % (B / 4) / 4) ^ (k & 3);  // B / 4 chunks a row; granules past the matrix' columns re-read its last block
-            qo[p] = (unsigned)k * (unsigned)(4 * ldq) + 64 * min(g, (u.np - w.j0) / 16 - 2 + (g & 1)) + 16 * (c & 3) + 3072 - 1024 * (p & 3);
+            qo[p] = (unsigned)k * (unsigned)(4 * ldq) + 64 * min(g, (u.np - w.j0) / 16 - 2 + (g & 1)) + 16 * (c & 3) + BIAS - 1024 * (p & 3);
         } else {
             qo[p] = (unsigned)min(row, u.mp - 1 - w.j0) * (unsigned)(4 * ldq) + at;
         }
     }
-    const char* pb = (const char*)(P + (size_t)w.i0 * (2 * ldp)) - 3072;
-    const char* qb = (const char*)(TR ? Q + 2 * w.j0 : Q + (size_t)w.j0 * (2 * ldq)) - 3072;
+    const char* pb = (const char*)(P + (size_t)w.i0 * (2 * ldp)) - BIAS;
+    const char* qb = (const char*)(TR ? Q + 2 * w.j0 : Q + (size_t)w.j0 * (2 * ldq)) - BIAS;
     const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)lds);
     auto uniform = [](const char* p) {
         const unsigned long long b = (unsigned long long)(uintptr_t)p;
