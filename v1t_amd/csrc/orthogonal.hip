@@ -593,8 +593,14 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(NsTable t
     constexpr int W = ns_launch(KIND);
     const int b = blockIdx.x, over = b - st.whole;
     const bool piece = SYM && over >= 0;  // workgroup-uniform
+    // the pieces K range by K range, an XCD's workgroups one behind the other: they read the same part of the rows
+    int number = b, range = 0;
+    if (piece) {
+        const int pieces = (int)gridDim.x - st.whole, rest = pieces / st.split, at = ns_deal(over, st.whole, pieces);
+        range = at / rest;
+        number = st.whole + at - range * rest;
+    }
     ns_head head;
-    int number = piece ? st.whole + over / st.split : b;
     int unit = ns_find<W>(tab, number, head);
     if (!piece) {
         number = head[1] + ns_deal(b - head[1], head[1], SYM ? min(head[2], st.whole - head[1]) : head[2]);
@@ -603,7 +609,7 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(NsTable t
     const NsUnit& u = tab.units[unit];
     const NsWhere w = ns_where<TW, KIND>(u, ws, st, number - head[0]);
     const int steps = (KIND == NS_GRAM ? u.np : u.mp) / NS_BK, each = piece ? (steps + st.split - 1) / st.split : steps;
-    const int t0 = piece ? over % st.split * each : 0, nk = max(0, min(each, steps - t0));  // this workgroup's K steps
+    const int t0 = range * each, nk = max(0, min(each, steps - t0));  // this workgroup's K steps
     const f16_t* X = (const f16_t*)(ws + ns_x(u, st.from));
     const f16_t* P = KIND == NS_GRAM ? X : (const f16_t*)(ws + ns_square_at(u, st.p));
     const f16_t* Q = KIND == NS_SQUARE ? (const f16_t*)(ws + ns_square_at(u, st.q)) : X;
@@ -748,7 +754,7 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(NsTable t
         }
     }
     if (piece) {  // its sums in the accumulators' order; ns_join_kernel adds the pieces up
-        float* to = st.slab + ((size_t)over * 4 + wave) * (TW * TW * 1024) + 4 * lane;
+        float* to = st.slab + ((size_t)((number - st.whole) * st.split + range) * 4 + wave) * (TW * TW * 1024) + 4 * lane;
 #pragma unroll
         for (int i = 0; i < TW; ++i)
 #pragma unroll
