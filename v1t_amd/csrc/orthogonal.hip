@@ -767,36 +767,31 @@ __global__ __launch_bounds__(256, TW == 3 ? 1 : 2) void ns_gemm_kernel(NsTable t
     ns_epilogue<TW, KIND, T>(u, w, st, acc, (float*)lds + wave * (32 * TW) * (32 * TW), wi, wj, lane);
 }
 
-// The pieces of the split tiles, added up in their order, and the epilogue: one wave per quarter of a tile
+// The pieces of the split tiles, added up in their order, and the epilogue: one wave per 32 x 32 of a tile (one per quarter of a 128 tile took 12 us for 36 tiles of 7 pieces)
 template <int TW, int KIND>
 __global__ __launch_bounds__(64) void ns_join_kernel(NsTable tab, char* ws, NsStep st) {
-    constexpr int W = ns_launch(KIND);
-    __shared__ __attribute__((aligned(16))) float lds[32 * TW * 32 * TW];
-    const int lane = threadIdx.x, wave = blockIdx.x & 3, tile = blockIdx.x >> 2;
+    constexpr int W = ns_launch(KIND), BLOCKS = 4 * TW * TW;
+    __shared__ __attribute__((aligned(16))) float lds[32 * 32];
+    const int lane = threadIdx.x, tile = blockIdx.x / BLOCKS, block = blockIdx.x % BLOCKS, wave = block / (TW * TW), ij = block % (TW * TW);
     ns_head head;
     const NsUnit& u = tab.units[ns_find<W>(tab, st.whole + tile, head)];
-    const NsWhere w = ns_where<TW, KIND>(u, ws, st, st.whole + tile - head[0]);
-    f32x16 acc[TW][TW];
+    NsWhere w = ns_where<TW, KIND>(u, ws, st, st.whole + tile - head[0]);
+    w.i0 += 32 * (TW * (wave >> 1) + ij / TW);
+    w.j0 += 32 * (TW * (wave & 1) + ij % TW);
+    f32x16 acc[1][1];
 #pragma unroll
-    for (int i = 0; i < TW; ++i)
+    for (int e = 0; e < 16; ++e) acc[0][0][e] = 0.f;
+    const float* from = st.slab + ((size_t)tile * st.split * 4 + wave) * (TW * TW * 1024) + ij * 1024 + 4 * lane;
+#pragma unroll 4
+    for (int p = 0; p < st.split; ++p, from += 4 * TW * TW * 1024) {
 #pragma unroll
-        for (int j = 0; j < TW; ++j)
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 v = *(const f32x4*)(from + q * 256);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    for (int p = 0; p < st.split; ++p) {
-        const float* from = st.slab + (((size_t)tile * st.split + p) * 4 + wave) * (TW * TW * 1024) + 4 * lane;
-#pragma unroll
-        for (int i = 0; i < TW; ++i)
-#pragma unroll
-            for (int j = 0; j < TW; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const f32x4 v = *(const f32x4*)(from + ((i * TW + j) * 4 + q) * 256);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += v[e];
-                }
+            for (int e = 0; e < 4; ++e) acc[0][0][4 * q + e] += v[e];
+        }
     }
-    ns_epilogue<TW, KIND, float>(u, w, st, acc, lds, wave >> 1, wave & 1, lane);
+    ns_epilogue<1, KIND, float>(u, w, st, acc, lds, 0, 0, lane);
 }
 
 // ---- small matrices -----------------------------------------------------------------------
@@ -1228,8 +1223,8 @@ int ns_gemm(const NsLayout& l, const NsTable& table, char* ws, NsStep st, hipStr
     else hipLaunchKernelGGL((ns_gemm_kernel<1, KIND, T>), dim3(p.grid()), dim3(256), 0, s, table, ws, st);
     if constexpr (KIND == NS_GRAM || KIND == NS_SQUARE)
         if (p.joined()) {
-            if (p.tw == 3) hipLaunchKernelGGL((ns_join_kernel<3, KIND>), dim3(4 * p.joined()), dim3(64), 0, s, table, ws, st);
-            else if (p.tw == 2) hipLaunchKernelGGL((ns_join_kernel<2, KIND>), dim3(4 * p.joined()), dim3(64), 0, s, table, ws, st);
+            if (p.tw == 3) hipLaunchKernelGGL((ns_join_kernel<3, KIND>), dim3(36 * p.joined()), dim3(64), 0, s, table, ws, st);
+            else if (p.tw == 2) hipLaunchKernelGGL((ns_join_kernel<2, KIND>), dim3(16 * p.joined()), dim3(64), 0, s, table, ws, st);
             else hipLaunchKernelGGL((ns_join_kernel<1, KIND>), dim3(4 * p.joined()), dim3(64), 0, s, table, ws, st);
         }
     return hipGetLastError() == hipSuccess ? V1T_OK : V1T_ERR_LAUNCH;
