@@ -84,9 +84,10 @@ def test_large_tiles():
     close(v1t_amd.orthogonalize(u), u)
 
 
-@pytest.mark.parametrize("count,rows,cols", [(4, 1300, 1300), (1, 1500, 1500), (2, 1000, 1900), (1, 100, 20000), (1, 4001, 4100)])
+@pytest.mark.parametrize("count,rows,cols", [(1, 100, 20000), (1, 1600, 1660), (1, 1800, 1900), (4, 1300, 1300), (2, 1000, 1900), (1, 2300, 2360), (5, 1800, 1860), (1, 4001, 4100)])
 def test_tiles_and_pieces(count, rows, cols):
-    """Symmetric products in tiles of 192 split over K, of 128 split, of 128 and 64 side by side, of 64 in 16 pieces, of 192 whole; the same bits every time."""
+    """Symmetric products in tiles of 64 in 16 pieces, of 64 with pieces beside whole ones, of 128 in pieces, of 128 with pieces beside, of two kinds, of 192 in pieces,
+    of 192 with pieces behind whole ones, of 192 whole; the same bits every time."""
     us = [update(rows, cols, i) for i in range(count)]
     os = v1t_amd.orthogonalize(us)
     for u, o in zip(us, os):

@@ -1050,30 +1050,37 @@ std::pair<int, int> ns_parts(long long elements) {
 }
 
 // Tile (64, 128 or 192) and split of a product with t[.] tiles of each size whose K steps sum to k[.], at the least estimated time. A CU holds two workgroups of
-// the smaller tiles, one of the largest. Measured, us per K step and round: 64 0.25 alone on its CU and 0.85 by two, 128 0.9 and 1.6, 192 1.6 (so 128 does twice the work
-// of 64 in a time, where there is enough of it; 192 does 1.13 times that of 128 where it fills the chip once, 2.25 times where 128 would leave one a CU), epilogues 1.5, 5
-// and 9; the launch that joins pieces 6, and their sums at 3 TB/s. Only the tiles of the last, part-filled round are split, in pieces of at least 4 steps:
-// 8192 x 1024's Gram matrix, 36 tiles of 128 in seven pieces each, takes 36 us and 12 to join them; as 136 whole tiles of 64 it took 107.
+// the smaller tiles, one of the largest. Measured, us per K step and round: 64 0.25 alone on its CU, 0.55 where a few CUs hold two and 0.85 where all do (power); 128 0.9,
+// 1.25 and 1.6; 192 1.6 (so 128 does twice the work of 64 in a time, where there is enough of it; 192 does 1.13 times that of 128 where it fills the chip once,
+// 2.25 times where 128 would leave one a CU); epilogues 1.5, 5 and 9; the launch that joins pieces 4, and their sums at 5 TB/s. Only tiles of the last, part-filled round
+// are split, in pieces of at least 4 steps: all of them, or those beyond one a CU, whose pieces then run beside the whole ones (two of 2000 x 2000, 272
+// tiles of 128: 1195 us a call, 1292 unsplit; twelve 777 x 1301, 336 tiles: 928 and 915, and the estimate leaves them whole).
+// 8192 x 1024's Gram matrix, 36 tiles of 128 in seven pieces each, takes 35 us and 7 to join them; as 136 whole tiles of 64 it took 107.
 NsPlan ns_plan(const long long (&t)[3], const long long (&k)[3], bool may_split) {
     constexpr int CUS = 256;
-    constexpr double FULL[3] = {0.85, 1.6, 1.6}, ALONE[3] = {0.25, 0.9, 1.6}, TAIL[3] = {1.5, 5.0, 9.0};
+    constexpr double FULL[3] = {0.85, 1.6, 1.6}, SOME[3] = {0.55, 1.25, 1.6}, ALONE[3] = {0.25, 0.9, 1.6}, TAIL[3] = {1.5, 5.0, 9.0};
     NsPlan best;
     double least = 1e30;
     for (int tw = 1; tw <= 3; ++tw) {
         const int slots = tw == 3 ? CUS : 2 * CUS;
         const long long tiles = t[tw - 1];
         const double steps = (double)k[tw - 1] / (double)tiles;
-        auto round = [&](double k, long long w) { return w == 0 ? 0.0 : TAIL[tw - 1] + k * (w <= CUS ? ALONE : FULL)[tw - 1]; };
-        for (int split = 1; split <= (may_split ? 16 : 1); ++split) {
-            const long long whole = split == 1 ? tiles : tiles / slots * slots, rest = tiles - whole, pieces = rest * split;
-            if (split > 1 && (rest == 0 || pieces > slots || steps < 4 * split)) continue;
-            double us = (double)(whole / slots) * round(steps, slots) + round(steps, whole % slots);
-            if (split > 1) us += round(steps / split, pieces) + 6.0 + (double)pieces * tw * tw * 16384.0 * 2.0 / 3e6;
-            if (us < least) {
-                least = us;
-                best.us = us; best.tw = tw; best.tiles = (int)tiles; best.whole = (int)whole; best.split = split;
+        auto step = [&](long long w) { return w <= CUS ? ALONE[tw - 1] : SOME[tw - 1] + (FULL[tw - 1] - SOME[tw - 1]) * (double)(w - CUS) / CUS; };
+        auto round = [&](double k, long long w) { return w == 0 ? 0.0 : TAIL[tw - 1] + k * step(w); };
+        for (int split = 1; split <= (may_split ? 16 : 1); ++split)
+            for (int beside = 0; beside < (split > 1 && tw < 3 ? 2 : 1); ++beside) {  // pieces alone behind whole rounds, or beside one whole tile a CU
+                const long long whole = split == 1 ? tiles : beside ? tiles / CUS * CUS : tiles / slots * slots, rest = tiles - whole, pieces = rest * split;
+                if (beside && whole % slots != CUS) continue;
+                if (split > 1 && (rest == 0 || pieces > (beside ? CUS : slots) || steps < 4 * split)) continue;
+                double us = (double)(whole / slots) * round(steps, slots) + round(steps, beside ? 0 : whole % slots);
+                if (beside) us += 4.0 + round(steps / split, CUS + pieces) + (steps - steps / split) * step(CUS);
+                else if (split > 1) us += round(steps / split, pieces);
+                if (split > 1) us += 4.0 + (double)pieces * tw * tw * 16384.0 * 2.0 / 5e6;
+                if (us < least) {
+                    least = us;
+                    best.us = us; best.tw = tw; best.tiles = (int)tiles; best.whole = (int)whole; best.split = split;
+                }
             }
-        }
     }
     return best;
 }
