@@ -441,6 +441,33 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
     const int r = lane & 31, h = lane >> 5, extra = KIND == NS_SQUARE ? 0 : ns_extra(u.x0, st.lg);
     const float grown = KIND == NS_APPLY ? ldexpf(1.f, ns_extra(u.x0, st.lg_next) - extra) : KIND == NS_GRAM ? ldexpf(1.f, -2 * extra) : 1.f;
     const float alpha = st.alpha * grown, beta = st.beta * grown, inv = KIND == NS_LAST ? ldexpf(st.inv, -extra) : 0.f;
+    const int iw = w.i0 + SIDE * wi, jw = w.j0 + SIDE * wj;
+    const bool mirror = SYM && w.bi != w.bj;  // the lower triangle
+    // what is added to the product, loaded before the image is written: one after the other, each would wait behind the stores of the one before (8192 x 1024 455 against
+    // 446 us). The 192 tile's registers are full: there the batches are single (4096 x 4096's A A 236 us, in nines 255)
+    constexpr int LOOPS = SIDE * SIDE / 512, N = TW == 3 ? 1 : LOOPS;
+    f16x8 dh[N], dl[N], eh[N], el[N];
+    auto load = [&](int k0) {
+        if constexpr (KIND != NS_GRAM) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const int k = k0 + 64 * n + lane, i = iw + k / (SIDE / 8), j = jw + 8 * (k % (SIDE / 8));
+                dh[n] = dl[n] = eh[n] = el[n] = f16x8{};
+                if (i >= u.mp || j >= w.cols) continue;
+                if (beta != 0.f) {
+                    const f16_t* d = w.D + ns_at(i, j, w.ldd);
+                    dh[n] = *(const f16x8*)d;
+                    dl[n] = *(const f16x8*)(d + NS_LO);
+                }
+                if (KIND == NS_SQUARE && st.beta2 != 0.f) {
+                    const f16_t* d = w.D2 + ns_at(i, j, w.ldd);
+                    eh[n] = *(const f16x8*)d;
+                    el[n] = *(const f16x8*)(d + NS_LO);
+                }
+            }
+        }
+    };
+    if constexpr (N > 1) load(0);
 #pragma unroll
     for (int ti = 0; ti < TW; ++ti)
 #pragma unroll
@@ -452,53 +479,52 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
                     f32x4{alpha * a[4 * q], alpha * a[4 * q + 1], alpha * a[4 * q + 2], alpha * a[4 * q + 3]};
             }
     __builtin_amdgcn_wave_barrier();
-    const int iw = w.i0 + SIDE * wi, jw = w.j0 + SIDE * wj;
-    const bool mirror = SYM && w.bi != w.bj;  // the lower triangle
-    for (int k = lane; k < SIDE * SIDE / 8; k += 64) {
-        const int il = k / (SIDE / 8), jl = 8 * (k % (SIDE / 8)), i = iw + il, j = jw + jl;
-        if (i >= u.mp || j >= w.cols) continue;  // both are multiples of 32: groups of 8 are whole
-        f32x4 v0 = *(const f32x4*)(img + chunk(il, jl / 4)), v1 = *(const f32x4*)(img + chunk(il, jl / 4 + 1));
-        if constexpr (KIND != NS_GRAM) {
-            const f16_t* d = w.D + ns_at(i, j, w.ldd);
-            const f16x8 dh = *(const f16x8*)d, dl = *(const f16x8*)(d + NS_LO);
+#pragma unroll 1
+    for (int l = 0; l < LOOPS; l += N) {
+        if constexpr (N == 1) load(64 * l);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v0[e] += beta * ((float)dh[e] + (float)dl[e]);
-                v1[e] += beta * ((float)dh[4 + e] + (float)dl[4 + e]);
-            }
-        }
-        if constexpr (KIND == NS_SQUARE) {
-            if (st.beta2 != 0.f) {
-                const f16_t* d = w.D2 + ns_at(i, j, w.ldd);
-                const f16x8 dh = *(const f16x8*)d, dl = *(const f16x8*)(d + NS_LO);
+        for (int n = 0; n < N; ++n) {
+            const int k = 64 * (l + n) + lane, il = k / (SIDE / 8), jl = 8 * (k % (SIDE / 8)), i = iw + il, j = jw + jl;
+            if (i >= u.mp || j >= w.cols) continue;  // both are multiples of 32: groups of 8 are whole
+            f32x4 v0 = *(const f32x4*)(img + chunk(il, jl / 4)), v1 = *(const f32x4*)(img + chunk(il, jl / 4 + 1));
+            if constexpr (KIND != NS_GRAM) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    v0[e] += st.beta2 * ((float)dh[e] + (float)dl[e]);
-                    v1[e] += st.beta2 * ((float)dh[4 + e] + (float)dl[4 + e]);
+                    v0[e] += beta * ((float)dh[n][e] + (float)dl[n][e]);
+                    v1[e] += beta * ((float)dh[n][4 + e] + (float)dl[n][4 + e]);
                 }
             }
+            if constexpr (KIND == NS_SQUARE) {
+                if (st.beta2 != 0.f) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (i == j + e && i < u.m()) v0[e] += st.diagonal;
-                if (i == j + 4 + e && i < u.m()) v1[e] += st.diagonal;
-            }
-        }
-        if constexpr (KIND != NS_LAST) {
-            f16x8 ch, cl;
+                    for (int e = 0; e < 4; ++e) {
+                        v0[e] += st.beta2 * ((float)eh[n][e] + (float)el[n][e]);
+                        v1[e] += st.beta2 * ((float)eh[n][4 + e] + (float)el[n][4 + e]);
+                    }
+                }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                f16_t a, b;
-                ns_split(e < 4 ? v0[e] : v1[e - 4], a, b);
-                ch[e] = a;
-                cl[e] = b;
+                for (int e = 0; e < 4; ++e) {
+                    if (i == j + e && i < u.m()) v0[e] += st.diagonal;
+                    if (i == j + 4 + e && i < u.m()) v1[e] += st.diagonal;
+                }
             }
-            f16_t* to = w.C + ns_at(i, j, w.cols);
-            *(f16x8*)to = ch;
-            *(f16x8*)(to + NS_LO) = cl;
-        }
-        if (KIND == NS_LAST || (KIND == NS_SQUARE && mirror)) {
-            *(f32x4*)(img + chunk(il, jl / 4)) = v0;
-            *(f32x4*)(img + chunk(il, jl / 4 + 1)) = v1;
+            if constexpr (KIND != NS_LAST) {
+                f16x8 ch, cl;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    f16_t a, b;
+                    ns_split(e < 4 ? v0[e] : v1[e - 4], a, b);
+                    ch[e] = a;
+                    cl[e] = b;
+                }
+                f16_t* to = w.C + ns_at(i, j, w.cols);
+                *(f16x8*)to = ch;
+                *(f16x8*)(to + NS_LO) = cl;
+            }
+            if (KIND == NS_LAST || (KIND == NS_SQUARE && mirror)) {
+                *(f32x4*)(img + chunk(il, jl / 4)) = v0;
+                *(f32x4*)(img + chunk(il, jl / 4 + 1)) = v1;
+            }
         }
     }
     __builtin_amdgcn_wave_barrier();
