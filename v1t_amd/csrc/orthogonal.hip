@@ -20,8 +20,8 @@
 //
 // Bound: the matrix cores of large matrices, at the rate that power leaves them - a product of 4096 x 4096 in 355 us, 1.16 PFLOP/s of fp16 operations (three a
 // product), pipes busy 64 % of the time at 1.63 GHz; torch's fp16 product reaches 1.33 PFLOP/s - and launch after launch of small ones: 8 us for each of the
-// default core's 15 products, whose operations take 1. Whole calls, five steps: 4096 x 4096 bf16 3.86 ms, 8192 x 1024 fp32 478 us, twelve 777 x 1301 fp16 889 us,
-// the default core's 24 matrices 141 us, one block of width 2048 (a momentum step over 4 matrices, 200 MB of weights) 4.32 ms, one 155 x 64 33 us.
+// default core's 15 products, whose operations take 1. Whole calls, five steps: 4096 x 4096 bf16 3.9 ms, 8192 x 1024 fp32 446 us, twelve 777 x 1301 fp16 870 us,
+// the default core's 24 matrices 141 us, one block of width 2048 (a momentum step over 4 matrices, 200 MB of weights) 4.2 ms, one 155 x 64 33 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -1142,7 +1142,7 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
     l.gram = ns_plan(gt, gk, true);
     l.poly = ns_plan(gt, pk, true);
     l.full = ns_plan(ft, fk, false);
-    // two steps: gram, poly, full each twice, or gram, five m x m products, full; 3 us a launch. 8192 x 1024: 561 us in pairs, 686 step by step; 4096 x 4096's products are
+    // two steps: gram, poly, full each twice, or gram, five m x m products, full; 3 us a launch. 8192 x 1024: 561 us in pairs, 686 step by step (in an earlier form of the products); 4096 x 4096's products are
     // all of one size, and it stays step by step
     l.pairs = l.gram.us + 5 * l.poly.us + l.full.us + 21.0 < 0.9 * (2 * (l.gram.us + l.poly.us + l.full.us) + 18.0);
     l.table = 0;
