@@ -22,14 +22,16 @@ MAX_SIZE = 1 << 31  # the C entry's sizes have 32 bits
 
 class _Turn(t.NamedTuple):
     sections: t.Tuple[int, ...]
+    pairs: int
     base: float
     shared: int
     halves: int
     inverse: int
+    array: t.Any  # sections, for the C entry
 
 
-def _check(q: torch.Tensor, k: t.Optional[torch.Tensor], positions: torch.Tensor, sections, base: float, layout: str) -> t.Tuple[int, ...]:
-    sections = tuple(int(s) for s in sections)
+@functools.lru_cache(maxsize=64)  # checks and conversions of a call's plain arguments cost as much as its launch
+def _turn(sections: t.Tuple[int, ...], base: float, layout: str, shared: bool, inverse: bool) -> _Turn:
     if not 1 <= len(sections) <= 4 or min(sections) < 0 or sum(sections) < 1:
         raise ValueError(f"rotary: sections are 1 to 4 non-negative numbers of pairs, got {sections}")
     if sum(sections) > MAX_PAIRS:
@@ -38,6 +40,14 @@ def _check(q: torch.Tensor, k: t.Optional[torch.Tensor], positions: torch.Tensor
         raise ValueError(f"rotary: layout is 'pairs' or 'halves', got {layout!r}")
     if not 0.0 < float(base) < float("inf"):
         raise ValueError(f"rotary: base must be positive and finite, got {base}")
+    return _Turn(sections, sum(sections), float(base), int(bool(shared)), _LAYOUTS[layout], int(bool(inverse)), (C.c_int * len(sections))(*sections))
+
+
+def _back(turn: _Turn) -> _Turn:
+    return _turn(turn.sections, turn.base, "halves" if turn.halves else "pairs", turn.shared, 1 - turn.inverse)
+
+
+def _check(q: torch.Tensor, k: t.Optional[torch.Tensor], positions: torch.Tensor, turn: _Turn) -> None:
     for x in (q, k):
         if x is None:
             continue
@@ -45,8 +55,8 @@ def _check(q: torch.Tensor, k: t.Optional[torch.Tensor], positions: torch.Tensor
             raise ValueError(f"rotary: q and k are (tokens, heads, features) or (batch, tokens, heads, features), got {tuple(x.shape)}")
         if x.dtype not in _DTYPES or x.dtype != q.dtype:
             raise TypeError(f"rotary: q and k share one of {list(_DTYPES)}, got {[y.dtype for y in (q, k) if y is not None]}")
-        if 2 * sum(sections) > x.shape[-1]:
-            raise ValueError(f"rotary: {sum(sections)} pairs need {2 * sum(sections)} features a head, got {x.shape[-1]}")
+        if 2 * turn.pairs > x.shape[-1]:
+            raise ValueError(f"rotary: {turn.pairs} pairs need {2 * turn.pairs} features a head, got {x.shape[-1]}")
         if x.device != q.device or x.shape[:-2] != q.shape[:-2] or x.shape[-1] != q.shape[-1]:
             raise ValueError(f"rotary: q and k share device, batch, tokens and features, got {tuple(q.shape)} on {q.device} and {tuple(x.shape)} on {x.device}")
         if x.shape[-2] < 1:
@@ -57,10 +67,9 @@ def _check(q: torch.Tensor, k: t.Optional[torch.Tensor], positions: torch.Tensor
         raise TypeError(f"rotary: positions are one of {list(_POSITION_TYPES)}, got {positions.dtype}")
     if positions.requires_grad:
         raise ValueError("rotary: no gradient with respect to positions")
-    ok = (q.shape[-3], len(sections))
+    ok = (q.shape[-3], len(turn.sections))
     if positions.device != q.device or tuple(positions.shape) not in ((ok, (q.shape[0],) + ok) if q.dim() == 4 else (ok,)):
         raise ValueError(f"rotary: positions are (tokens, axes) = {ok} - or (batch, tokens, axes) - on {q.device}, got {tuple(positions.shape)} on {positions.device}")
-    return sections
 
 
 def _launch(turn: _Turn, positions: torch.Tensor, pairs_of: t.Sequence[t.Tuple[torch.Tensor, torch.Tensor]]) -> None:
@@ -79,23 +88,18 @@ def _launch(turn: _Turn, positions: torch.Tensor, pairs_of: t.Sequence[t.Tuple[t
             shape, sx, sy = (1, *shape), (0, *sx), (0, *sy)
         ops.append(L.RotaryOperand(x.data_ptr(), y.data_ptr(), *sx[:3], *sy[:3], shape[2], 0 if x is y else (shape[3] + 7) // 8 * 8))
     sp = positions.stride()
-    n, sections = len(turn.sections), _sections(turn.sections)
-    L.check(L.load().v1t_rotary((L.RotaryOperand * len(ops))(*ops), len(ops), _DTYPES[x0.dtype], shape[0], shape[1], shape[3], sections, n, turn.base, turn.shared,
+    L.check(L.load().v1t_rotary((L.RotaryOperand * len(ops))(*ops), len(ops), _DTYPES[x0.dtype], shape[0], shape[1], shape[3], turn.array, len(turn.sections), turn.base, turn.shared,
                                 turn.halves, turn.inverse, positions.data_ptr(), _POSITION_TYPES[positions.dtype], sp[0] if len(sp) == 3 else 0, sp[-2], sp[-1],
                                 L.stream_of(device)), "rotary")
-
-
-@functools.lru_cache(maxsize=64)
-def _sections(sections: t.Tuple[int, ...]):
-    return (C.c_int * len(sections))(*sections)
 
 
 def _like(x: torch.Tensor) -> torch.Tensor:
     """x's shape with room for a multiple of 8 features a head: what lies behind the last whole 8 is moved as one store, too. `.data`: a
     tensor of its own over the wider one's storage; autograd lets a view that a function returns not be changed in place."""
     shape, d = x.shape, x.shape[-1]
-    y = torch.empty((*shape[:-1], (d + 7) // 8 * 8), dtype=x.dtype, device=x.device)
-    return y if d % 8 == 0 else y.narrow(-1, 0, d).data
+    if d % 8 == 0:
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
+    return torch.empty((*shape[:-1], (d + 7) // 8 * 8), dtype=x.dtype, device=x.device).narrow(-1, 0, d).data
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -117,8 +121,7 @@ class _RotaryFn(torch.autograd.Function):
     def backward(ctx, *grads):
         """A rotation is orthogonal: the gradient turns back. Differentiable itself (a second derivative turns forward again)."""
         (positions,) = ctx.saved_tensors
-        sections, base, shared, halves, inverse = ctx.turn
-        back = _Turn(sections, base, shared, halves, 1 - inverse)
+        back = _back(ctx.turn)
         out: t.List[t.Optional[torch.Tensor]] = [None, None]
         which = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[2 + i]]
         if not torch.is_grad_enabled():
@@ -155,9 +158,9 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int
     P pairs of all axes share one ladder, pair j turns by position * base^(-j / P). layout: pair j is features (2j, 2j + 1), "pairs", or (j, P + j),
     "halves". Features behind the 2P turned ones are copied.
     Angles are reduced in 64 bits (exact positions up to 2^53); products are fp32, rounded once to the tensor's type."""
-    sections = _check(q, k, positions, sections, base, layout)
+    turn = _turn(tuple(map(int, sections)), base, layout, shared, inverse)
+    _check(q, k, positions, turn)
     L.require_cuda(q, "rotary")
-    turn = _Turn(sections, float(base), int(bool(shared)), _LAYOUTS[layout], int(bool(inverse)))
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _apply(turn, positions, q, k)
     xs = [_rows(x) for x in (q, k) if x is not None]
@@ -187,7 +190,8 @@ def rotary_(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[in
             layout: str = "pairs", shared: bool = False, inverse: bool = False):
     """`rotary` in place, outside autograd (a new token's q and k, a projection's buffer): the same values, features behind the turned ones untouched.
     Positions lie in memory of their own."""
-    sections = _check(q, k, positions, sections, base, layout)
+    turn = _turn(tuple(map(int, sections)), base, layout, shared, inverse)
+    _check(q, k, positions, turn)
     xs = [x for x in (q, k) if x is not None]
     for x in xs:
         if torch.is_grad_enabled() and x.requires_grad:
@@ -200,7 +204,7 @@ def rotary_(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[in
     if k is not None and not _apart(q, k):
         raise ValueError("rotary_: q and k share elements")
     L.require_cuda(q, "rotary_")
-    _launch(_Turn(sections, float(base), int(bool(shared)), _LAYOUTS[layout], int(bool(inverse))), positions, [(x, x) for x in xs])
+    _launch(turn, positions, [(x, x) for x in xs])
     for x in xs:
         if not x.is_inference():
             torch.autograd.graph.increment_version(x)
