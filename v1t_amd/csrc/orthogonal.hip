@@ -430,6 +430,14 @@ DEVFN NsWhere ns_where(const NsUnit& u, char* ws, const NsStep& st, int t) {  //
     return w;
 }
 
+// Between a lane's writes to its wave's LDS and another lane's reads of them. The hardware keeps a wave's LDS operations in order; the fences, which cost no instruction, keep
+// the compiler to it: the barrier alone orders no memory, and to one lane the other's address need not alias its own
+DEVFN void ns_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Accumulators -> alpha acc + beta D -> planes (both triangles of a symmetric product), or the result. Each wave turns its part over in its own LDS, so that
 // planes are read and written 16 B a lane along their rows - also the mirrored tile's - and the result along its own rows, whichever way the matrix lies.
 // LDS image [SIDE][SIDE] fp32, 16-B chunks of a row swizzled by the row: writes by lanes of one column and reads along rows both spread over the banks.
@@ -478,7 +486,7 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
                 *(f32x4*)(img + chunk(32 * ti + r, 8 * tj + 2 * q + h)) =
                     f32x4{alpha * a[4 * q], alpha * a[4 * q + 1], alpha * a[4 * q + 2], alpha * a[4 * q + 3]};
             }
-    __builtin_amdgcn_wave_barrier();
+    ns_wave_sync();
 #pragma unroll 1
     for (int l = 0; l < LOOPS; l += N) {
         if constexpr (N == 1) load(64 * l);
@@ -527,7 +535,7 @@ DEVFN void ns_epilogue(const NsUnit& u, const NsWhere& w, const NsStep& st, f32x
             }
         }
     }
-    __builtin_amdgcn_wave_barrier();
+    ns_wave_sync();
     auto at = [&](int il, int jl) { return img[chunk(il, jl / 4) + (jl & 3)]; };
     if constexpr (SYM) {
         if (!mirror) return;
