@@ -11,6 +11,7 @@ import os
 import typing as t
 
 import torch
+from torch.autograd import forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", os.environ.get("V1T_LIB", "libv1t_amd.so"))  # V1T_LIB (dev): an experiment build next to it
@@ -213,6 +214,13 @@ def stream_of(device: int) -> int:
 def require_cuda(x: torch.Tensor, what: str) -> None:
     if not x.is_cuda:
         raise RuntimeError(f"v1t_amd {what}: tensor is on {x.device}; the HIP path needs a GPU tensor (no CPU fallback).")
+
+
+def refuse_tangents(what: str, tensors) -> None:
+    """Called by operators whose kernels read and write raw pointers: a dual tensor's tangent (torch.autograd.forward_ad) would be lost without a word, which reads as a derivative of
+    zero. Outside every dual level - where no tensor has one - it is a single comparison."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise NotImplementedError(f"v1t_amd {what}: forward-mode differentiation is not supported (a tensor carries a tangent)")
 
 
 def leaves_in_capture(out: torch.Tensor, what: str) -> None:

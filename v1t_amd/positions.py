@@ -121,6 +121,7 @@ class _RotaryFn(torch.autograd.Function):
     def backward(ctx, *grads):
         """A rotation is orthogonal: the gradient turns back. Differentiable itself (a second derivative turns forward again)."""
         (positions,) = ctx.saved_tensors
+        L.refuse_tangents("rotary", grads)
         back = _back(ctx.turn)
         out: t.List[t.Optional[torch.Tensor]] = [None, None]
         which = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[2 + i]]
@@ -148,8 +149,9 @@ def _apply(turn: _Turn, positions: torch.Tensor, q: torch.Tensor, k: t.Optional[
 
 def rotary(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int], k: t.Optional[torch.Tensor] = None, base: float = 10000.0,
            layout: str = "pairs", shared: bool = False, inverse: bool = False):
-    """q (and k) turned by their tokens' positions: new tensors; differentiable in q and k. Where 8 does not divide the number of features, the
-    result has rows with room for the next multiple: it is not contiguous (`reshape`, not `view`, joins its heads).
+    """q (and k) turned by their tokens' positions: new tensors; differentiable in q and k, any number of times, in reverse mode (forward mode is refused).
+    Where 8 does not divide the number of features, the result has rows with room for the next multiple: it is not contiguous (`reshape`, not `view`, joins
+    its heads).
 
     q: (batch, tokens, heads, features) or (tokens, heads, features), bf16 / fp16 / fp32, any strides; k: the same with its own number of heads.
     positions: (tokens, axes) for all sequences, or (batch, tokens, axes); int32, int64 or fp32, negative ones too. A token at 0 on every axis is
@@ -160,6 +162,7 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int
     Angles are reduced in 64 bits (exact positions up to 2^53); products are fp32, rounded once to the tensor's type."""
     turn = _turn(tuple(map(int, sections)), base, layout, shared, inverse)
     _check(q, k, positions, turn)
+    L.refuse_tangents("rotary", (q, k, positions))
     L.require_cuda(q, "rotary")
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _apply(turn, positions, q, k)
@@ -203,6 +206,7 @@ def rotary_(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[in
             raise ValueError(f"rotary_: elements of an expanded or overlapping view cannot be turned in place, got shape {tuple(x.shape)}, strides {x.stride()}")
     if k is not None and not _apart(q, k):
         raise ValueError("rotary_: q and k share elements")
+    L.refuse_tangents("rotary_", (q, k, positions))
     L.require_cuda(q, "rotary_")
     _launch(turn, positions, [(x, x) for x in xs])
     for x in xs:
