@@ -38,13 +38,13 @@ def _turn(sections: t.Tuple[int, ...], base: float, layout: str, shared: bool, i
         raise ValueError(f"rotary: {sum(sections)} pairs a head, at most {MAX_PAIRS} are supported")
     if layout not in _LAYOUTS:
         raise ValueError(f"rotary: layout is 'pairs' or 'halves', got {layout!r}")
-    if not 0.0 < float(base) < float("inf"):
+    if not 0.0 < base < float("inf"):
         raise ValueError(f"rotary: base must be positive and finite, got {base}")
-    return _Turn(sections, sum(sections), float(base), int(bool(shared)), _LAYOUTS[layout], int(bool(inverse)), (C.c_int * len(sections))(*sections))
+    return _Turn(sections, sum(sections), base, int(shared), _LAYOUTS[layout], int(inverse), (C.c_int * len(sections))(*sections))
 
 
 def _back(turn: _Turn) -> _Turn:
-    return _turn(turn.sections, turn.base, "halves" if turn.halves else "pairs", turn.shared, 1 - turn.inverse)
+    return _turn(turn.sections, turn.base, "halves" if turn.halves else "pairs", bool(turn.shared), not turn.inverse)
 
 
 def _check(q: torch.Tensor, k: t.Optional[torch.Tensor], positions: torch.Tensor, turn: _Turn) -> None:
@@ -160,7 +160,7 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int
     P pairs of all axes share one ladder, pair j turns by position * base^(-j / P). layout: pair j is features (2j, 2j + 1), "pairs", or (j, P + j),
     "halves". Features behind the 2P turned ones are copied.
     Angles are reduced in 64 bits (exact positions up to 2^53); products are fp32, rounded once to the tensor's type."""
-    turn = _turn(tuple(map(int, sections)), base, layout, shared, inverse)
+    turn = _turn(tuple(map(int, sections)), float(base), str(layout), bool(shared), bool(inverse))  # plain values: the cache keeps none that can change
     _check(q, k, positions, turn)
     L.refuse_tangents("rotary", (q, k, positions))
     L.require_cuda(q, "rotary")
@@ -193,7 +193,7 @@ def rotary_(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[in
             layout: str = "pairs", shared: bool = False, inverse: bool = False):
     """`rotary` in place, outside autograd (a new token's q and k, a projection's buffer): the same values, features behind the turned ones untouched.
     Positions lie in memory of their own."""
-    turn = _turn(tuple(map(int, sections)), base, layout, shared, inverse)
+    turn = _turn(tuple(map(int, sections)), float(base), str(layout), bool(shared), bool(inverse))  # plain values: the cache keeps none that can change
     _check(q, k, positions, turn)
     xs = [x for x in (q, k) if x is not None]
     for x in xs:
