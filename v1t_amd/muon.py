@@ -92,7 +92,7 @@ def orthogonalize(updates, *, steps: int = 5, coefficients=COEFFICIENTS, eps: fl
     else:
         outs = [torch.empty(u.shape, dtype=u.dtype, device=u.device) for u in us]
         out = outs[0] if one else outs
-    _orthogonalize([(u, o) for u, o in zip(us, outs) if u.numel()], int(steps), co, float(eps))
+    _orthogonalize([(u.resolve_neg(), o) for u, o in zip(us, outs) if u.numel()], int(steps), co, float(eps))
     return out
 
 
@@ -139,6 +139,8 @@ def muon_step(params: t.Sequence[torch.Tensor], grads: t.Sequence[torch.Tensor],
             raise TypeError(f"muon_step: fp32 tensors are needed, got {[x.dtype for x in (p, g, m)]}")
         if not (g.shape == shape == m.shape and p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and p.get_device() == g.get_device() == m.get_device() == device):
             raise ValueError(f"muon_step: parameter, gradient and momentum are contiguous tensors of one shape on one device, got {[(tuple(x.shape), str(x.device)) for x in (p, g, m)]}")
+        if p.is_neg() or g.is_neg() or m.is_neg():
+            raise ValueError("muon_step: views that negate their memory (the imaginary part of a conjugate) cannot be updated in place; resolve_neg() copies them")
         size = p.numel()
         if size == 0:
             continue

@@ -103,6 +103,7 @@ def _like(x: torch.Tensor) -> torch.Tensor:
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
+    x = x.resolve_neg()  # the imaginary part of a conjugate view holds its numbers with the other sign
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
@@ -164,6 +165,7 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int
     _check(q, k, positions, turn)
     L.refuse_tangents("rotary", (q, k, positions))
     L.require_cuda(q, "rotary")
+    positions = positions.resolve_neg()
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _apply(turn, positions, q, k)
     xs = [_rows(x) for x in (q, k) if x is not None]
@@ -199,6 +201,8 @@ def rotary_(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[in
     for x in xs:
         if torch.is_grad_enabled() and x.requires_grad:
             raise RuntimeError("rotary_: a tensor that requires grad cannot be turned in place; use rotary")
+        if x.is_neg():
+            raise ValueError("rotary_: a view that negates its memory (the imaginary part of a conjugate) cannot be turned in place; resolve_neg() copies it")
         if x.stride(-1) != 1 and x.shape[-1] > 1:
             raise ValueError(f"rotary_: unit stride in the last dimension is needed, got strides {x.stride()}")
         dims = sorted((s, n) for s, n in zip(x.stride(), x.shape) if n > 1)
@@ -208,7 +212,7 @@ def rotary_(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[in
         raise ValueError("rotary_: q and k share elements")
     L.refuse_tangents("rotary_", (q, k, positions))
     L.require_cuda(q, "rotary_")
-    _launch(turn, positions, [(x, x) for x in xs])
+    _launch(turn, positions.resolve_neg(), [(x, x) for x in xs])
     for x in xs:
         if not x.is_inference():
             torch.autograd.graph.increment_version(x)
