@@ -116,6 +116,7 @@ class _RotaryFn(torch.autograd.Function):
         xs = [_rows(x) for x in (q, k) if x is not None]
         ys = [_like(x) for x in xs]
         _launch(turn, positions, list(zip(xs, ys)))
+        ctx.mark_non_differentiable(*(y for i, y in enumerate(ys) if not ctx.needs_input_grad[2 + i]))
         return ys[0] if k is None else tuple(ys)
 
     @staticmethod
@@ -142,9 +143,10 @@ class _RotaryFn(torch.autograd.Function):
 
 def _apply(turn: _Turn, positions: torch.Tensor, q: torch.Tensor, k: t.Optional[torch.Tensor]):
     out = _RotaryFn.apply(turn, positions, q, k)
-    first = out if k is None else out[0]
-    if first.requires_grad:
-        L.leaves_in_capture(first, "rotary")
+    for y in (out,) if k is None else out:
+        if y.requires_grad:  # both results' node is one
+            L.leaves_in_capture(y, "rotary")
+            break
     return out
 
 
