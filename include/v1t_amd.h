@@ -166,15 +166,15 @@ int v1t_gaussian2d_backward(const float* z, long long zsb, long long zsc, int B,
                             int N, const float* grid, const float* feat, int FS, const float* gout,
                             float* dz, long long dzsb, long long dzsc, float* dgrid, float* dfeat,
                             float* dbias, void* stream);
-/* Same with `ws` = v1t_gaussian2d_backward_ws_bytes() bytes of scratch: the taps are counting-sorted by cell (per image)
- * into the scratch and dz is summed per run of equal cells, one atomic row per run (~20 MB) instead of 4*C*N*B
- * float atomics (317 MB at N = 8000, B = 16). The form the training path uses. */
+/* Same with `ws` = v1t_gaussian2d_backward_ws_bytes() bytes of scratch: the taps are sorted by cell and neuron (per image) into the scratch
+ * and dz is summed per run of equal cells, in a fixed order (the same bits in every pass), instead of by 4*C*N*B float atomics (317 MB at
+ * N = 8000, B = 16). The form the training path uses. */
 long long v1t_gaussian2d_backward_ws_bytes(int B, int H, int W, int N);
 int v1t_gaussian2d_backward_ws(const float* z, long long zsb, long long zsc, int B, int C, int H, int W,
                                int N, const float* grid, const float* feat, int FS, const float* gout,
                                float* dz, long long dzsb, long long dzsc, float* dgrid, float* dfeat,
                                float* dbias, void* ws, long long ws_bytes, void* stream);
-/* The three kernels of the form above one by one, `parts` = bit mask: 1 sort the taps (needs grid only - the training step runs
+/* The stages of the form above one by one, `parts` = bit mask: 1 sort the taps (needs grid only - the training step runs
  * it while the core is still in its forward), 2 parameter gradients (dgrid, dfeat, dbias), 4 gather dz from the sorted taps
  * (needs part 1's scratch and gout; z / dz addressing as above). 7 == v1t_gaussian2d_backward_ws. */
 int v1t_gaussian2d_backward_parts(const float* z, long long zsb, long long zsc, int B, int C, int H, int W,

@@ -47,7 +47,7 @@ MODEL = {
     "gemm_nt_kernel<5, 5, 4, 32, true, false, 0>": ("patch projection + bias + pos + cls + dropout", "hbm", R * 128 * 2 + x32, 2 * R * 64 * D, "U fp16; x0"),
     "patch_bwd_pos_cast_kernel": ("d pos / d cls + bf16 gradient", "hbm", x32 + p160, 0, "d x0; bf16 copy"),
     "drop_cast_kernel<5>": ("dropout backward + cast of the core output gradient", "hbm", x32 + p160, 0, "gout; dy"),
-    "readout_sort_multi_kernel": ("counting sort of the taps", "hbm", MICE * 16 * N_NEUR * 4 * 12, 0, "taps"),
+    "readout_sort_multi_kernel": ("sort of the taps by cell", "hbm", MICE * 16 * N_NEUR * 4 * 12, 0, "taps"),
     "pack_kernel": ("bf16 / fp16 weight shadow refresh", "hbm", core_floats * 4 + core_floats * 2 * 3, 0, "fp32 arena; 16-bit planes + transposes"),
 }
 ks = d["kernels"]

@@ -9,6 +9,8 @@
 // channel sum is one wave reduction. HBM-bound; algorithmic bytes in DESIGN.md.
 #include "readout.h"
 
+#include <algorithm>
+
 namespace {
 
 struct Taps {
@@ -134,116 +136,256 @@ DEVFN void readout_bwd_body(const ReadoutArgs& a, int bx) {
 template <int NE>
 __global__ __launch_bounds__(256) void readout_bwd_kernel(ReadoutArgs a) { readout_bwd_body<NE>(a, blockIdx.x); }
 
-// dz without a flood of global float atomics (4 x C x N x B adds = 317 MB at N = 8000, B = 16: ~250 us at the chip-wide
-// 1.3 TB/s atomic rate; LDS float atomics are slower still, ~1 lane per clock per CU): invert the sampling.
-//   sort  : workgroup (slice s of the neurons, image b) counting-sorts its taps by cell in LDS (histogram, scan,
-//           scatter: integer LDS atomics only) into its region of the scratch: (cell, tap id, bilinear weight),
-//           taps outside the map and the padding of the region carry the sentinel cell `cells` and sort last
-//   gather: one wave per 64 consecutive sorted taps sums G[b][n] * w * F[n][:] (coalesced feature rows) while the
-//           cell stays the same and adds the finished row to dz with ONE atomic row (620 B) per (chunk, cell) run:
-//           ~20 MB of atomics for any distribution of the neurons over the map - including the freshly initialised
-//           model, whose 8000 neurons all sit on a handful of cells, which per-cell lists could not balance.
-constexpr int DZ_SLICES = 4;       // neuron slices per image (parallelism of the sort pass)
-constexpr int DZ_MAX_CELLS = 4096; // LDS histogram capacity; larger maps use the atomic form
+// dz without float atomics (4 x C x N x B adds = 317 MB at N = 8000, B = 16: ~250 us at the chip-wide 1.3 TB/s atomic rate; LDS float
+// atomics are slower still, ~1 lane per clock per CU - and the order of any of them changes the sums): invert the sampling. Everything is
+// in a fixed order, so dz is the same bit for bit in every pass: the core's backward rounds it to bf16 next, where another last bit of a sum
+// becomes another bf16 value, and that a row of every weight gradient behind it.
+//   sort  : workgroup (slice s of the neurons, image b) sorts keys (cell, tap) by cell in LDS, in the order of the taps
+//   merge : the image's slices into one list by cell, within a cell by neuron: (cell, tap id, bilinear weight); taps outside the map and the
+//           list's padding carry the sentinel cell `cells` and come last
+//   gather: a wave per 64 consecutive taps sums G[b][n] * w * F[n][:] (coalesced feature rows) while the cell stays the same. A run of equal
+//           cells is all of its cell: added to dz. One that is cut between the waves of a workgroup is put together in LDS, one that is cut
+//           between workgroups leaves a part in the scratch
+//   join  : adds the parts of a run in order. Balanced for any distribution of the neurons over the map - including the freshly initialised
+//           model, whose 8000 neurons all sit on a handful of cells
+// 16 images, 8000 neurons: sort 17, merge 12, gather 31 and join 5 us where the neurons lie all over the map; 17, 9, 27 and 5 us where all lie in one cell (in an earlier form,
+// whose runs met in atomics in any order, 18 us and 44, 18 and 33). The training step sorts and merges beside the core's forward.
+constexpr int DZ_SLICES = 4;       // neuron slices per image at least (parallelism of the sort)
+constexpr int DZ_SLICE = 2048;     // neurons per slice at most: 8192 keys in LDS
+constexpr int DZ_MAX_CELLS = 4096; // LDS table capacity; larger maps use the atomic form
+constexpr int DZ_TAP_BITS = 13;    // key = cell << 13 | tap of the slice
+constexpr int DZ_GROUP = 256;      // taps per workgroup of the gather, 64 a wave
+constexpr int DZ_PART = 256;       // floats of a part (C <= 256)
+static_assert((4 * DZ_SLICE) >> DZ_TAP_BITS <= 1 && (unsigned long long)(DZ_MAX_CELLS + 1) << DZ_TAP_BITS < 0xffffffffu, "keys");
+constexpr int DZ_DIGIT_BITS = 7, DZ_DIGITS = 1 << DZ_DIGIT_BITS;  // two passes over a cell's bits
+static_assert(DZ_MAX_CELLS < DZ_DIGITS * DZ_DIGITS && DZ_DIGITS * 16 % 1024 == 0, "digits");
 struct DzSort {
-    unsigned* cell;  // [B * DZ_SLICES][R]
-    unsigned* id;    // tap id = 4 * (b * N + n) + k
+    unsigned* keys;   // [B][slices][4 * ns] sorted
+    int* first;       // [B][slices][cells + 1] where a slice's cells begin
+    unsigned* cell;   // [B][R]
+    unsigned* id;     // tap id = 4 * (b * N + n) + k
     float* wt;
-    int ns, R;       // neurons per slice, region stride (multiple of 64)
+    float* part;      // [B * R / DZ_GROUP][2][DZ_PART]: a group's part of the run that began before it, of the run that goes on behind it
+    int slices, ns, R;  // neurons per slice, taps per image (multiple of DZ_GROUP)
 };
 
-DEVFN void readout_sort_body(const ReadoutArgs& a, const DzSort& ix, int s, int b, int* hist, int* wsum) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int cells = a.H * a.W;
-    const int n0 = s * ix.ns, n1 = min(a.N, n0 + ix.ns);
-    for (int i = tid; i <= cells; i += 1024) hist[i] = 0;
-    __syncthreads();
-    for (int n = n0 + tid; n < n1; n += 1024) {
-        const size_t i = (size_t)b * a.N + n;
-        const Taps t = make_taps(a.grid[2 * i], a.grid[2 * i + 1], a.W, a.H);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) atomicAdd(&hist[t.in[q] ? t.cell[q] : cells], 1);
-    }
-    __syncthreads();
-    // exclusive scan of hist[0..cells]: each thread owns a contiguous run of PER entries
-    const int PER = (cells + 1 + 1023) / 1024;
-    int run[(DZ_MAX_CELLS + 1 + 1023) / 1024], tot = 0;
-#pragma unroll
-    for (int e = 0; e < (DZ_MAX_CELLS + 1 + 1023) / 1024; ++e) {
-        const int idx = tid * PER + e;
-        run[e] = (e < PER && idx <= cells) ? hist[idx] : 0;
-        tot += run[e];
-    }
-    int inc = tot;  // inclusive scan over the wave
+// One pass of a radix sort in LDS: n keys (a multiple of 1024) by 7 bits, equal ones in the order they came in. A wave owns n / 16 keys in a row, 64 at a time: the lanes of a
+// digit find each other by ballots, their places in the wave's share are the digit's count so far and their number among themselves.
+struct DzSortLds {
+    unsigned key[2][4 * DZ_SLICE];
+    int count[16][DZ_DIGITS + 1];  // [wave][digit]
+    int sum[16];
+};
+DEVFN void dz_wave_sync() {  // between one lane's write to LDS and another's read, within a wave
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+// sum of v over the threads before this one of 1024; sum: LDS of 16
+DEVFN int dz_exclusive_scan(int v, int* sum) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int inc = v;  // inclusive over the wave
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int v = __shfl_up(inc, o);
-        if (lane >= o) inc += v;
+        const int x = __shfl_up(inc, o);
+        if (lane >= o) inc += x;
     }
-    if (lane == 63) wsum[wave] = inc;
+    if (lane == 63) sum[wave] = inc;
     __syncthreads();
-    int base = inc - tot;
-    for (int w = 0; w < wave; ++w) base += wsum[w];
+    int base = inc - v;
+    for (int w = 0; w < wave; ++w) base += sum[w];
+    return base;
+}
+
+DEVFN void dz_radix_pass(DzSortLds& L, int src, int n, int shift) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, own = n / 16;
+    constexpr int GROUPS = 4 * DZ_SLICE / 1024;
+    unsigned k[GROUPS];
+    int at[GROUPS];
+    for (int i = tid; i < 16 * (DZ_DIGITS + 1); i += 1024) (&L.count[0][0])[i] = 0;
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < (DZ_MAX_CELLS + 1 + 1023) / 1024; ++e) {
-        const int idx = tid * PER + e;
-        if (e < PER && idx <= cells) {
-            hist[idx] = base;
+    for (int g = 0; g < GROUPS; ++g) {
+        if (64 * g >= own) break;
+        k[g] = L.key[src][wave * own + 64 * g + lane];
+        const unsigned d = k[g] >> shift & (DZ_DIGITS - 1);
+        unsigned long long same = ~0ull;
+#pragma unroll
+        for (int bit = 0; bit < DZ_DIGIT_BITS; ++bit) {
+            const bool on = d >> bit & 1;
+            const unsigned long long b = __ballot(on);
+            same &= on ? b : ~b;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1)), before = L.count[wave][d];
+        at[g] = before + rank;
+        dz_wave_sync();
+        if (rank == 0) L.count[wave][d] = before + __popcll(same);
+        dz_wave_sync();
+    }
+    __syncthreads();
+    // counts -> first places, digit by digit and wave by wave
+    int v[DZ_DIGITS * 16 / 1024], tot = 0;
+#pragma unroll
+    for (int e = 0; e < DZ_DIGITS * 16 / 1024; ++e) {
+        const int i = tid * (DZ_DIGITS * 16 / 1024) + e;
+        v[e] = L.count[i & 15][i >> 4];
+        tot += v[e];
+    }
+    int base = dz_exclusive_scan(tot, L.sum);
+#pragma unroll
+    for (int e = 0; e < DZ_DIGITS * 16 / 1024; ++e) {
+        const int i = tid * (DZ_DIGITS * 16 / 1024) + e;
+        L.count[i & 15][i >> 4] = base;
+        base += v[e];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        if (64 * g >= own) break;
+        L.key[src ^ 1][L.count[wave][k[g] >> shift & (DZ_DIGITS - 1)] + at[g]] = k[g];
+    }
+    __syncthreads();
+}
+
+DEVFN void readout_sort_body(const ReadoutArgs& a, const DzSort& ix, int s, int b, DzSortLds& L) {
+    const int tid = threadIdx.x;
+    const int cells = a.H * a.W;
+    const int n0 = min(a.N, s * ix.ns), cnt = min(a.N - n0, ix.ns), taps = 4 * cnt, n = (taps + 1023) / 1024 * 1024;
+    for (int i = tid; i < n / 4; i += 1024) {
+        u32x4 v = {~0u, ~0u, ~0u, ~0u};
+        if (i < cnt) {
+            const size_t g = 2 * ((size_t)b * a.N + n0 + i);
+            const Taps t = make_taps(a.grid[g], a.grid[g + 1], a.W, a.H);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = (unsigned)(t.in[q] ? t.cell[q] : cells) << DZ_TAP_BITS | (unsigned)(4 * i + q);
+        }
+        *(u32x4*)&L.key[0][4 * i] = v;
+    }
+    __syncthreads();
+    dz_radix_pass(L, 0, n, DZ_TAP_BITS);
+    dz_radix_pass(L, 1, n, DZ_TAP_BITS + DZ_DIGIT_BITS);
+    const unsigned* key = L.key[0];
+    const size_t reg = (size_t)b * ix.slices + s;
+    for (int p = tid; p < taps; p += 1024) ix.keys[reg * (4 * ix.ns) + p] = key[p];
+    for (int c = tid; c <= cells; c += 1024) {  // the first key at or above the cell's least
+        int lo = 0, hi = taps;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (key[mid] < (unsigned)c << DZ_TAP_BITS) lo = mid + 1;
+            else hi = mid;
+        }
+        ix.first[reg * (cells + 1) + c] = lo;
+    }
+}
+__global__ __launch_bounds__(1024) void readout_sort_kernel(ReadoutArgs a, DzSort ix) {
+    __shared__ __attribute__((aligned(16))) DzSortLds L;
+    readout_sort_body(a, ix, blockIdx.x, blockIdx.y, L);
+}
+
+DEVFN void readout_merge_body(const ReadoutArgs& a, const DzSort& ix, int s, int b, int* to, int* wsum) {
+    const int tid = threadIdx.x;
+    const int cells = a.H * a.W;
+    auto taps_of = [&](int x) { return 4 * max(0, min(a.N - x * ix.ns, ix.ns)); };
+    // to[c]: what a tap of cell c adds to its place in the slice for its place in the image. Each thread owns a contiguous run of PER cells
+    constexpr int MOST = (DZ_MAX_CELLS + 1 + 1023) / 1024;
+    const int PER = (cells + 1 + 1023) / 1024;
+    int run[MOST], mine[MOST], tot = 0;  // the image's taps of a cell; where this slice's begin behind them, less their place in the slice
+#pragma unroll
+    for (int e = 0; e < MOST; ++e) {
+        const int c = tid * PER + e;
+        run[e] = mine[e] = 0;
+        if (e >= PER || c > cells) continue;
+        for (int x = 0; x < ix.slices; ++x) {
+            const int* first = ix.first + ((size_t)b * ix.slices + x) * (cells + 1);
+            const int at = first[c], next = c < cells ? first[c + 1] : taps_of(x);
+            if (x == s) mine[e] = run[e] - at;
+            run[e] += next - at;
+        }
+        tot += run[e];
+    }
+    int base = dz_exclusive_scan(tot, wsum);
+#pragma unroll
+    for (int e = 0; e < MOST; ++e) {
+        const int c = tid * PER + e;
+        if (e < PER && c <= cells) {
+            to[c] = base + mine[e];
             base += run[e];
         }
     }
     __syncthreads();
-    const size_t reg = ((size_t)b * DZ_SLICES + s) * ix.R;
-    for (int n = n0 + tid; n < n1; n += 1024) {
-        const size_t i = (size_t)b * a.N + n;
-        const Taps t = make_taps(a.grid[2 * i], a.grid[2 * i + 1], a.W, a.H);
+    const unsigned* keys = ix.keys + ((size_t)b * ix.slices + s) * (4 * ix.ns);
+    const size_t reg = (size_t)b * ix.R, i0 = (size_t)b * a.N + (size_t)s * ix.ns;
+    constexpr int MINE = 4 * DZ_SLICE / 1024;  // a thread's taps, all loads in flight together
+    const int taps = taps_of(s);
+    unsigned k[MINE];
+    float gx[MINE], gy[MINE];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int c = t.in[q] ? t.cell[q] : cells;
-            const int slot = atomicAdd(&hist[c], 1);
-            ix.cell[reg + slot] = (unsigned)c;
-            ix.id[reg + slot] = 4u * (unsigned)i + q;
-            ix.wt[reg + slot] = t.w[q];
-        }
+    for (int e = 0; e < MINE; ++e) k[e] = tid + 1024 * e < taps ? keys[tid + 1024 * e] : 0u;
+#pragma unroll
+    for (int e = 0; e < MINE; ++e) {
+        const size_t i = i0 + ((k[e] & ((1u << DZ_TAP_BITS) - 1)) >> 2);
+        const bool on = tid + 1024 * e < taps;
+        gx[e] = on ? a.grid[2 * i] : 0.f;
+        gy[e] = on ? a.grid[2 * i + 1] : 0.f;
     }
-    for (int p = 4 * (n1 - n0) + tid; p < ix.R; p += 1024) ix.cell[reg + p] = (unsigned)cells;  // padding
+#pragma unroll
+    for (int e = 0; e < MINE; ++e) {
+        const int p = tid + 1024 * e;
+        if (p >= taps) break;
+        const unsigned c = k[e] >> DZ_TAP_BITS, tap = k[e] & ((1u << DZ_TAP_BITS) - 1);
+        const Taps t = make_taps(gx[e], gy[e], a.W, a.H);
+        const size_t at = reg + to[c] + p;
+        ix.cell[at] = c;
+        ix.id[at] = 4u * (unsigned)i0 + tap;
+        ix.wt[at] = (tap & 2 ? (tap & 1 ? t.w[3] : t.w[2]) : (tap & 1 ? t.w[1] : t.w[0]));
+    }
+    if (s == 0)
+        for (int p = 4 * a.N + tid; p < ix.R; p += 1024) ix.cell[reg + p] = (unsigned)cells;  // padding
 }
-__global__ __launch_bounds__(1024) void readout_sort_kernel(ReadoutArgs a, DzSort ix) {
-    __shared__ int hist[DZ_MAX_CELLS + 1];
+__global__ __launch_bounds__(1024) void readout_merge_kernel(ReadoutArgs a, DzSort ix) {
+    __shared__ int to[DZ_MAX_CELLS + 1];
     __shared__ int wsum[16];
-    readout_sort_body(a, ix, blockIdx.x, blockIdx.y, hist, wsum);
+    readout_merge_body(a, ix, blockIdx.x, blockIdx.y, to, wsum);
 }
 
 template <int NE>
 DEVFN void readout_dz_gather_body(const ReadoutArgs& a, const DzSort& ix, int bx) {
-    const int lane = threadIdx.x & 63;
-    const size_t chunk = (size_t)bx * 4 + (threadIdx.x >> 6);
-    const size_t total = (size_t)a.B * DZ_SLICES * ix.R;
-    if (chunk * 64 >= total) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const unsigned groups = ix.R / DZ_GROUP, b = (unsigned)bx / groups, gi = (unsigned)bx % groups;
     const unsigned cells = a.H * a.W;
-    const unsigned rowb = (unsigned)(chunk * 64 / ((size_t)DZ_SLICES * ix.R)) * cells;  // image of this chunk's region
-    const unsigned rows = rowb + cells;
-    // lane j holds tap j of the chunk; key = global row (image * cells + cell), >= rows for sentinels
-    const size_t me = chunk * 64 + lane;
-    const unsigned key = rowb + ix.cell[me];
-    const unsigned id = key < rows ? ix.id[me] : 0u;
-    const float gw = key < rows ? ix.wt[me] * a.gout[id >> 2] : 0.f;
+    __shared__ float s_cut[4][2][64 * NE];  // a wave's part of the run that began before its taps, and of the one that goes on behind them
+    // lane j holds the wave's tap j
+    const unsigned* cl = ix.cell + (size_t)bx * DZ_GROUP;
+    const size_t me = (size_t)bx * DZ_GROUP + 64 * wave + lane;
+    const unsigned key = ix.cell[me];
+    auto cell_at = [&](int t) { return t < 0 && gi == 0 || t >= DZ_GROUP && gi + 1 == groups ? cells : cl[t]; };  // tap t of the group, the neighbouring groups' too
+    const unsigned before = cell_at(64 * wave - 1), behind = cell_at(64 * wave + 64);
+    const unsigned id = key < cells ? ix.id[me] : 0u;
+    const float gw = key < cells ? ix.wt[me] * a.gout[id >> 2] : 0.f;
     const unsigned nn = (id >> 2) % (unsigned)a.N;
     float acc[NE];
 #pragma unroll
     for (int j = 0; j < NE; ++j) acc[j] = 0.f;
     unsigned cur = __builtin_amdgcn_readfirstlane(key);
-    auto flush = [&](unsigned row) {
-        float* dzr = a.dz + (size_t)(row / cells) * a.dzsb + (size_t)(row % cells) * a.dzsc;
+    bool head = cur == before;  // the current run began before this wave's taps
+    auto add = [&](unsigned row) {  // the only addend of its pass: an atomic because nothing waits for it (a load to add to holds up the features')
+        float* dzr = a.dz + (size_t)b * a.dzsb + (size_t)row * a.dzsc;
 #pragma unroll
-        for (int j = 0; j < NE; ++j) {
-            const int c = lane + 64 * j;
-            if (c < a.C) atomicAdd(&dzr[c], acc[j]);
-            acc[j] = 0.f;
-        }
+        for (int j = 0; j < NE; ++j)
+            if (lane + 64 * j < a.C) atomicAdd(&dzr[lane + 64 * j], acc[j]);
     };
-    constexpr int RIF = 8;  // feature rows in flight (4 -> 8 rows: 189 -> 178 us per step, round 4)
+    auto flush = [&](unsigned row, bool cut) {  // cut: it goes on in the next wave's
+        if (head || cut) {
+#pragma unroll
+            for (int j = 0; j < NE; ++j) s_cut[wave][head ? 0 : 1][lane + 64 * j] = acc[j];
+        } else {
+            add(row);
+        }
+#pragma unroll
+        for (int j = 0; j < NE; ++j) acc[j] = 0.f;
+        head = false;
+    };
+    constexpr int RIF = 8;  // feature rows in flight (4 -> 8 rows: 189 -> 178 us per step)
     for (int t0 = 0; t0 < 64; t0 += RIF) {
         unsigned kq[RIF], nq[RIF], gq[RIF];
         float f[RIF][NE];
@@ -253,7 +395,7 @@ DEVFN void readout_dz_gather_body(const ReadoutArgs& a, const DzSort& ix, int bx
             nq[u] = __builtin_amdgcn_readlane(nn, t0 + u);
             gq[u] = __builtin_amdgcn_readlane(__float_as_uint(gw), t0 + u);
         }
-        if (kq[0] >= rows) break;  // sentinels and padding sort to the end of the region
+        if (kq[0] >= cells) break;  // sentinels and padding sort to the end of the image
 #pragma unroll
         for (int u = 0; u < RIF; ++u)
 #pragma unroll
@@ -263,9 +405,9 @@ DEVFN void readout_dz_gather_body(const ReadoutArgs& a, const DzSort& ix, int bx
             }
 #pragma unroll
         for (int u = 0; u < RIF; ++u) {
-            if (kq[u] >= rows) break;
+            if (kq[u] >= cells) break;
             if (kq[u] != cur) {
-                flush(cur);
+                flush(cur, false);
                 cur = kq[u];
             }
             const float g = __uint_as_float(gq[u]);
@@ -273,12 +415,81 @@ DEVFN void readout_dz_gather_body(const ReadoutArgs& a, const DzSort& ix, int bx
             for (int j = 0; j < NE; ++j) acc[j] += g * f[u][j];
         }
     }
-    if (cur < rows) flush(cur);
+    const unsigned first = __builtin_amdgcn_readfirstlane(key), last = __builtin_amdgcn_readlane(key, 63);
+    if (cur < cells) flush(cur, last == cur && behind == cur);
+    __syncthreads();
+    // the cut runs, each by the wave that it begins in - one that began before the group by its first - in order
+    const bool early = wave == 0 && first < cells && first == before;            // began before the group
+    const bool starts = last < cells && last == behind && !(first == last && first == before);  // begins here and goes on
+    auto whole_run = [&](unsigned row, int slot, bool began) {
+        int w = wave;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) acc[j] = s_cut[w][slot][lane + 64 * j];
+        // wave w's part is followed by wave w + 1's while w's taps end and w + 1's begin with the run
+        bool on = cell_at(64 * w + 63) == row && cell_at(64 * w + 64) == row;
+        while (on && w < 3) {
+            ++w;
+#pragma unroll
+            for (int j = 0; j < NE; ++j) acc[j] += s_cut[w][0][lane + 64 * j];
+            on = cell_at(64 * w + 63) == row && cell_at(64 * w + 64) == row;
+        }
+        if (!began && !on) return add(row);
+        float* to = ix.part + ((size_t)bx * 2 + (began ? 0 : 1)) * DZ_PART;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) to[lane + 64 * j] = acc[j];
+    };
+    if (early) whole_run(first, 0, true);
+    if (starts) whole_run(last, 1, false);
 }
 template <int NE>
 __global__ __launch_bounds__(256) void readout_dz_gather_kernel(ReadoutArgs a, DzSort ix) { readout_dz_gather_body<NE>(a, ix, blockIdx.x); }
 
-// ---- the same four kernels over SEVERAL units (mice) in one launch each: a training step runs the tails of all local mice as one launch
+template <int NE>
+DEVFN void readout_dz_join_body(const ReadoutArgs& a, const DzSort& ix, int bx) {
+    const int lane = threadIdx.x & 63;
+    const unsigned groups = ix.R / DZ_GROUP, group = __builtin_amdgcn_readfirstlane(bx * 4 + (int)(threadIdx.x >> 6));
+    if (group >= (unsigned)a.B * groups) return;
+    const unsigned cells = a.H * a.W, b = group / groups, gi = group % groups;
+    const unsigned* cl = ix.cell + (size_t)group * DZ_GROUP;
+    if (gi + 1 >= groups) return;
+    const unsigned cur = cl[DZ_GROUP - 1], next = cl[DZ_GROUP], first = cl[0], before = gi > 0 ? cl[-1] : cells;
+    if (cur >= cells || next != cur) return;         // no run is cut here
+    if (first == cur && before == cur) return;       // it began in an earlier group
+    // it goes on through groups gi + 1 .. gi + more: the cells are in order, so group x is the last one when group x + 1 begins with another
+    unsigned more = 1;
+    for (;; more += 64) {
+        const unsigned x = gi + more + 1 + lane;
+        const unsigned long long on = __ballot(x < groups && cl[(size_t)(x - gi) * DZ_GROUP] == cur);
+        if (~on) {
+            more += __builtin_ctzll(~on);
+            break;
+        }
+    }
+    const float* part = ix.part + (size_t)group * 2 * DZ_PART + lane;  // whole rows, so that nothing stands between the loads: what lies behind the channels is not used
+    float acc[NE];
+#pragma unroll
+    for (int j = 0; j < NE; ++j) acc[j] = part[DZ_PART + 64 * j];
+    constexpr unsigned IF = 8;  // parts in flight
+    for (unsigned m = 1; m <= more; m += IF) {
+        float v[IF][NE];
+#pragma unroll
+        for (unsigned u = 0; u < IF; ++u)
+#pragma unroll
+            for (int j = 0; j < NE; ++j) v[u][j] = part[(size_t)min(m + u, more) * 2 * DZ_PART + 64 * j];
+#pragma unroll
+        for (unsigned u = 0; u < IF; ++u)
+#pragma unroll
+            for (int j = 0; j < NE; ++j) acc[j] += m + u <= more ? v[u][j] : 0.f;
+    }
+    float* dzr = a.dz + (size_t)b * a.dzsb + (size_t)cur * a.dzsc;
+#pragma unroll
+    for (int j = 0; j < NE; ++j)
+        if (lane + 64 * j < a.C) atomicAdd(&dzr[lane + 64 * j], acc[j]);  // as in the gather: calls that add to one dz at once lose nothing
+}
+template <int NE>
+__global__ __launch_bounds__(256) void readout_dz_join_kernel(ReadoutArgs a, DzSort ix) { readout_dz_join_body<NE>(a, ix, blockIdx.x); }
+
+// ---- the same kernels over SEVERAL units (mice) in one launch each: a training step runs the tails of all local mice as one launch
 // per stage instead of one chain of small launches per mouse (v1t_tails_*). The unit table travels by value in the kernel arguments;
 // a workgroup finds its unit from the prefix sums of the units' workgroup counts (wave-uniform scalar loads).
 struct ReadoutMulti {
@@ -306,11 +517,17 @@ __global__ __launch_bounds__(256) void readout_bwd_multi_kernel(ReadoutMulti m) 
     readout_bwd_body<NE>(m.a[u], bx);
 }
 __global__ __launch_bounds__(1024) void readout_sort_multi_kernel(ReadoutMulti m) {
-    __shared__ int hist[DZ_MAX_CELLS + 1];
+    __shared__ __attribute__((aligned(16))) DzSortLds L;
+    int bx;
+    const int u = multi_unit(m.start, m.n, blockIdx.x, bx);
+    readout_sort_body(m.a[u], m.ix[u], bx % m.ix[u].slices, bx / m.ix[u].slices, L);
+}
+__global__ __launch_bounds__(1024) void readout_merge_multi_kernel(ReadoutMulti m) {
+    __shared__ int to[DZ_MAX_CELLS + 1];
     __shared__ int wsum[16];
     int bx;
     const int u = multi_unit(m.start, m.n, blockIdx.x, bx);
-    readout_sort_body(m.a[u], m.ix[u], bx % DZ_SLICES, bx / DZ_SLICES, hist, wsum);
+    readout_merge_body(m.a[u], m.ix[u], bx % m.ix[u].slices, bx / m.ix[u].slices, to, wsum);
 }
 template <int NE>
 __global__ __launch_bounds__(256) void readout_dz_gather_multi_kernel(ReadoutMulti m) {
@@ -318,14 +535,31 @@ __global__ __launch_bounds__(256) void readout_dz_gather_multi_kernel(ReadoutMul
     const int u = multi_unit(m.start, m.n, blockIdx.x, bx);
     readout_dz_gather_body<NE>(m.a[u], m.ix[u], bx);
 }
+template <int NE>
+__global__ __launch_bounds__(256) void readout_dz_join_multi_kernel(ReadoutMulti m) {
+    int bx;
+    const int u = multi_unit(m.start, m.n, blockIdx.x, bx);
+    readout_dz_join_body<NE>(m.a[u], m.ix[u], bx);
+}
 
-DzSort sort_plan(void* ws, int B, int N) {
+DzSort sort_plan(void* ws, int B, int H, int W, int N, size_t* bytes = nullptr) {
     DzSort d;
-    d.ns = (N + DZ_SLICES - 1) / DZ_SLICES;
-    d.R = (4 * d.ns + 63) / 64 * 64;
-    const size_t arr = (size_t)B * DZ_SLICES * d.R * 4;
+    d.slices = std::max(DZ_SLICES, (N + DZ_SLICE - 1) / DZ_SLICE);
+    d.ns = (N + d.slices - 1) / d.slices;
+    d.R = round_up(4 * N, DZ_GROUP);
     char* p = (char*)ws;
-    d.cell = (unsigned*)p; d.id = (unsigned*)(p + arr); d.wt = (float*)(p + 2 * arr);
+    auto take = [&](size_t words) {
+        char* at = p;
+        p += (words * 4 + 255) / 256 * 256;
+        return at;
+    };
+    d.part = (float*)take((size_t)B * (d.R / DZ_GROUP) * 2 * DZ_PART);
+    d.cell = (unsigned*)take((size_t)B * d.R);
+    d.id = (unsigned*)take((size_t)B * d.R);
+    d.wt = (float*)take((size_t)B * d.R);
+    d.keys = (unsigned*)take((size_t)B * d.slices * 4 * d.ns);
+    d.first = (int*)take((size_t)B * d.slices * ((size_t)H * W + 1));
+    if (bytes) *bytes = (size_t)(p - (char*)ws);
     return d;
 }
 
@@ -335,19 +569,23 @@ int launch_t(const ReadoutArgs& a, bool bwd, void* ws, size_t ws_bytes, hipStrea
     if (!bwd) {
         hipLaunchKernelGGL(readout_fwd_kernel<NE>, grid, dim3(256), 0, s, a);
     } else if (ws && a.H * a.W <= DZ_MAX_CELLS && ws_bytes >= readout_bwd_ws_bytes(a.B, a.H, a.W, a.N) && (a.dz || parts != READOUT_BWD_ALL)) {
-        // the three kernels of the sorted form, individually selectable (the training step sorts the taps while the core is still
+        // the kernels of the sorted form, individually selectable (the training step sorts the taps while the core is still
         // in its forward - the sort needs the sample positions only - and gathers dz before the parameter gradients, so that the
         // core's backward can start as early as possible)
-        const DzSort ix = sort_plan(ws, a.B, a.N);
-        if (parts & READOUT_BWD_SORT) hipLaunchKernelGGL(readout_sort_kernel, dim3(DZ_SLICES, a.B), dim3(1024), 0, s, a, ix);
+        const DzSort ix = sort_plan(ws, a.B, a.H, a.W, a.N);
+        if (parts & READOUT_BWD_SORT) {
+            hipLaunchKernelGGL(readout_sort_kernel, dim3(ix.slices, a.B), dim3(1024), 0, s, a, ix);
+            hipLaunchKernelGGL(readout_merge_kernel, dim3(ix.slices, a.B), dim3(1024), 0, s, a, ix);
+        }
         if (parts & READOUT_BWD_PARAMS) {
             ReadoutArgs a2 = a;
             a2.dz = nullptr;
             hipLaunchKernelGGL(readout_bwd_kernel<NE>, grid, dim3(256), 0, s, a2);
         }
         if ((parts & READOUT_BWD_DZ) && a.dz) {
-            const size_t chunks = (size_t)a.B * DZ_SLICES * ix.R / 64;
-            hipLaunchKernelGGL(readout_dz_gather_kernel<NE>, dim3((unsigned)((chunks + 3) / 4)), dim3(256), 0, s, a, ix);
+            const unsigned groups = (unsigned)a.B * (ix.R / DZ_GROUP);
+            hipLaunchKernelGGL(readout_dz_gather_kernel<NE>, dim3(groups), dim3(256), 0, s, a, ix);
+            hipLaunchKernelGGL(readout_dz_join_kernel<NE>, dim3((groups + 3) / 4), dim3(256), 0, s, a, ix);
         }
     } else if (parts != READOUT_BWD_ALL) {
         return V1T_ERR_WORKSPACE;  // the split form exists with the sorted workspace only
@@ -369,21 +607,30 @@ int dispatch(const ReadoutArgs& a, bool bwd, void* ws, size_t ws_bytes, hipStrea
 
 template <int NE>
 int launch_multi_t(ReadoutMulti& m, int stage, hipStream_t s) {
-    int tot = 0;
-    for (int u = 0; u < m.n; ++u) {
-        const ReadoutArgs& a = m.a[u];
-        m.start[u] = tot;
-        if (stage == TAILS_SORT) tot += DZ_SLICES * a.B;
-        else if (stage == TAILS_DZ) tot += (int)(((size_t)a.B * DZ_SLICES * m.ix[u].R / 64 + 3) / 4);
-        else tot += (a.N + 3) / 4;
-    }
-    m.start[m.n] = tot;
+    auto deal = [&](auto blocks) {
+        int tot = 0;
+        for (int u = 0; u < m.n; ++u) {
+            m.start[u] = tot;
+            tot += blocks(m.a[u], m.ix[u]);
+        }
+        return m.start[m.n] = tot;
+    };
+    int tot = deal([&](const ReadoutArgs& a, const DzSort& ix) {
+        return stage == TAILS_SORT ? ix.slices * a.B : stage == TAILS_DZ ? a.B * (ix.R / DZ_GROUP) : (a.N + 3) / 4;
+    });
     if (tot == 0) return V1T_OK;
     switch (stage) {
         case TAILS_FWD: hipLaunchKernelGGL(readout_fwd_multi_kernel<NE>, dim3(tot), dim3(256), 0, s, m); break;
         case TAILS_PARAMS: hipLaunchKernelGGL(readout_bwd_multi_kernel<NE>, dim3(tot), dim3(256), 0, s, m); break;
-        case TAILS_SORT: hipLaunchKernelGGL(readout_sort_multi_kernel, dim3(tot), dim3(1024), 0, s, m); break;
-        case TAILS_DZ: hipLaunchKernelGGL(readout_dz_gather_multi_kernel<NE>, dim3(tot), dim3(256), 0, s, m); break;
+        case TAILS_SORT:
+            hipLaunchKernelGGL(readout_sort_multi_kernel, dim3(tot), dim3(1024), 0, s, m);
+            hipLaunchKernelGGL(readout_merge_multi_kernel, dim3(tot), dim3(1024), 0, s, m);
+            break;
+        case TAILS_DZ:
+            hipLaunchKernelGGL(readout_dz_gather_multi_kernel<NE>, dim3(tot), dim3(256), 0, s, m);
+            tot = deal([](const ReadoutArgs& a, const DzSort& ix) { return (a.B * (ix.R / DZ_GROUP) + 3) / 4; });
+            hipLaunchKernelGGL(readout_dz_join_multi_kernel<NE>, dim3(tot), dim3(256), 0, s, m);
+            break;
         default: return V1T_ERR_ARG;
     }
     return hipGetLastError() == hipSuccess ? V1T_OK : V1T_ERR_LAUNCH;
@@ -402,7 +649,7 @@ int launch_readout_multi(const ReadoutArgs* a, void* const* ws, const size_t* ws
         if (stage == TAILS_PARAMS) m.a[u].dz = nullptr;
         if (stage == TAILS_SORT || stage == TAILS_DZ) {
             if (!ws[u] || a[u].H * a[u].W > DZ_MAX_CELLS || ws_bytes[u] < readout_bwd_ws_bytes(a[u].B, a[u].H, a[u].W, a[u].N)) return V1T_ERR_WORKSPACE;
-            m.ix[u] = sort_plan(ws[u], a[u].B, a[u].N);
+            m.ix[u] = sort_plan(ws[u], a[u].B, a[u].H, a[u].W, a[u].N);
         }
     }
     switch ((a[0].C + 63) / 64) {
@@ -414,9 +661,9 @@ int launch_readout_multi(const ReadoutArgs* a, void* const* ws, const size_t* ws
 }
 
 size_t readout_bwd_ws_bytes(int B, int H, int W, int N) {
-    (void)H; (void)W;
-    const DzSort d = sort_plan(nullptr, B, N);
-    return 3 * (size_t)B * DZ_SLICES * d.R * 4 + 256;
+    size_t bytes = 0;
+    (void)sort_plan(nullptr, B, H, W, N, &bytes);
+    return bytes;
 }
 int launch_readout_fwd(const ReadoutArgs& a, hipStream_t s) { return dispatch(a, false, nullptr, 0, s); }
 int launch_readout_bwd(const ReadoutArgs& a, void* ws, size_t ws_bytes, hipStream_t s) { return dispatch(a, true, ws, ws_bytes, s); }
