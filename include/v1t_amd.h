@@ -454,10 +454,13 @@ int v1t_rotary(const v1t_rotary_operand* operands, int n_operands, int dtype, in
 
 /* Orthogonalised updates (no reference counterpart: train.py:216-223 steps every parameter with AdamW). For each of n matrices U (rows x cols), on its
  * own: X = U / (|U|_F + eps) with the shorter side first; `steps` times (<= 32) A = X X^T, X <- a X + (b A + c A A) X with the step's
- * (a, b, c) = coefficients[3k .. 3k + 2] (host memory); the result in U's shape. fp32 arithmetic throughout whatever the dtype (0 = bf16, 1 = fp16, 2 = fp32 of
- * `in` and `out`), rounded once. Coefficients that let a plane of the iteration grow to 128 or more (their bound over all singular values in
+ * (a, b, c) = coefficients[3k .. 3k + 2] (host memory); the result in U's shape, rounded once to its dtype (0 = bf16, 1 = fp16, 2 = fp32 of `in` and `out`).
+ * Sums are fp32, their operands - X, A, S and what they are joined to - two fp16 numbers each at one exponent for the whole matrix, without the product of the two
+ * lower ones: 22 bits of a number near the matrix's scale, where fp32 has 24, and fewer of smaller ones. The error is that of fp32 arithmetic relative to the matrix
+ * (2e-6 of its norm under the usual coefficients), not to each number: of a row 1e-5 below the others some 15 bits are right, 1e-7 below 9. Which other matrices a call
+ * holds decides how the products are cut and the steps joined, and so a matrix's last bits; the same call gives the same bits. Coefficients that let a plane of the iteration grow to 128 or more (their bound over all singular values in
  * [0, 1]) are refused. `in` has element strides of any sign, `out` is row-major without gaps and overlaps no `in` of the call but its own, where that is
- * laid out alike. m = min(rows, cols) <= 32768, rows * cols <= 2^31. Deterministic. The workspace is 16-byte aligned. */
+ * laid out alike. m = min(rows, cols) <= 32768, rows * cols <= 2^31. The workspace is 16-byte aligned. */
 typedef struct v1t_matrix {
     const void* in;
     void* out;

@@ -102,6 +102,18 @@ def test_no_bit_less_than_the_planes_hold(rows, cols):
     assert got <= bound, (got, bound)
 
 
+@pytest.mark.parametrize("scale", [1e-3, 1e-5, 1e-7])
+@pytest.mark.parametrize("rows,cols", [(64, 155), (155, 620), (488, 155)])
+def test_rows_far_below_the_others(rows, cols, scale):
+    """The planes have one exponent per matrix: such a row keeps fewer of its bits, as `held` has it, and costs the others none."""
+    u = gradient(rows, cols, 3)
+    u[5] *= scale
+    want, bound = allowed(u)
+    got, model, plain = (x.double() - want for x in (v1t_amd.orthogonalize(u), held(u), formula(u, torch.float32)))
+    assert float(got.norm() / want.norm()) <= bound
+    assert float(got[5].norm()) <= 2 * float(model[5].norm() + plain[5].norm())
+
+
 def test_the_momentum_step_to_the_same_bits():
     """With a momentum of a half, m and U are one rounding each, fused or not: U is known to the bit. The parameter: the rate's rounding, its product's and the sum's."""
     gen = torch.Generator(device=DEV).manual_seed(9)

@@ -8,7 +8,8 @@
 // The first pair applies a a' X + (...) X, which keeps small singular values exact; later ones, whose Q is near 1, all of Q: a a' = 12 would cancel.
 //
 // Precision: fp32, on fp16 matrix instructions. A number v of X, A or S (spectral norm known to the host to stay below 2^15 / 2^e for the given
-// coefficients) is kept as two fp16 planes of v 2^e: hi = fp16(v 2^e) and lo = fp16(v 2^e - hi), 22 bits of it, and a product of two such numbers is
+// coefficients) is kept as two fp16 planes of v 2^e: hi = fp16(v 2^e) and lo = fp16(v 2^e - hi) - 22 bits of a number near the matrix's scale; where lo is subnormal, 2^-25
+// of v 2^e, so that rows 1e-5 below the others keep some 15 bits of theirs, 1e-7 below 9 - and a product of two such numbers is
 // hi hi + hi lo + lo hi, accumulated in fp32: three MFMAs where fp16 has one, at a sixteenth of the time of an fp32 one. The term that is left out
 // and the two roundings are 2^-22 of a product each, of random sign: the error of fp32 operands (the steps amplify what is lost on the small
 // singular values up to a^5 = 480 times: one fp16 plane leaves 2e-3 of the result's norm, two leave what fp32 does, 2e-6).
@@ -1090,6 +1091,8 @@ std::pair<int, int> ns_parts(long long elements) {
 // are split, in pieces of at least 4 steps: all of them, or those beyond one a CU, whose pieces then run beside the whole ones (two of 2000 x 2000, 272
 // tiles of 128: 1195 us a call, 1292 unsplit; twelve 777 x 1301, 336 tiles: 928 and 915, and the estimate leaves them whole).
 // 8192 x 1024's Gram matrix, 36 tiles of 128 in seven pieces each, takes 35 us and 7 to join them; as 136 whole tiles of 64 it took 107.
+// Where it is off: launches of less than a round. A product of two 1024 x 1024 is estimated 9.5 us and takes 14 (every XCD's L2 takes the operands in anew), the default core's
+// A A 2.8 and 6.2, its Gram matrices 6.2 and 9.6; a product of 4096 x 4096 with X 420 and 360. What is compared - tiles and splits of one product - is off alike.
 NsPlan ns_plan(const long long (&t)[3], const long long (&k)[3], bool may_split) {
     constexpr int CUS = 256;
     constexpr double FULL[3] = {0.85, 1.6, 1.6}, SOME[3] = {0.55, 1.25, 1.6}, ALONE[3] = {0.25, 0.9, 1.6}, TAIL[3] = {1.5, 5.0, 9.0};
@@ -1150,8 +1153,8 @@ int ns_layout(int n, Shape shape, Put put, NsLayout& l) {
     l.gram = ns_plan(gt, gk, true);
     l.poly = ns_plan(gt, pk, true);
     l.full = ns_plan(ft, fk, false);
-    // two steps: gram, poly, full each twice, or gram, five m x m products, full; 3 us a launch. 8192 x 1024: 561 us in pairs, 686 step by step (in an earlier form of the products); 4096 x 4096's products are
-    // all of one size, and it stays step by step
+    // two steps: gram, poly, full each twice, or gram, five m x m products, full; 3 us a launch. 8192 x 1024, four steps: 350 us in pairs, 420 one by one; 4096 x 4096's products are
+    // all of one size, and it stays step by step. One plan serves all matrices of a call
     l.pairs = l.gram.us + 5 * l.poly.us + l.full.us + 21.0 < 0.9 * (2 * (l.gram.us + l.poly.us + l.full.us) + 18.0);
     l.table = 0;
     l.heads = ns_align((long long)n * (long long)sizeof(NsUnit));

@@ -11,7 +11,8 @@
 // 16 + 4 heads x 128 bf16 (406 MB) 84 us, 4.8 TB/s; one token of 8 streams 5 us of which nothing is traffic.
 //
 // Numerics: the angle is held as a number of turns in 64 bits, p * (rate / 2 pi), and reduced to [-1/2, 1/2] before it is rounded to 32: a
-// 32-bit product is off by 0.03 rad at position 10^6. Products and sums of the rotation are fp32, rounded once to the tensor's type.
+// 32-bit product is off by 0.03 rad at position 10^6. Cosine and sine are taken of the rounded angle: fp32 results err by 4.3e-8 of their norm, with those of
+// 64 bits by 3.7e-8. Products and sums of the rotation are fp32, rounded once to the tensor's type.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -27,7 +28,7 @@ constexpr int ROT_THREADS = 256;
 
 template <int P>
 struct RotRates {  // kernel argument: a captured graph keeps it, no device memory behind it. P: 64 where they suffice - a launch copies all of it; 2.3 KB cost a
-                   // small training pass of two launches 8 of 160 us
+                   // small training pass of two launches 8 of 160 us. The default core's 2 x 38 pairs take the large one
     double turns[P];
     unsigned char axis[P];
 };

@@ -62,8 +62,12 @@ def orthogonalize(updates, *, steps: int = 5, coefficients=COEFFICIENTS, eps: fl
     """Each update's Newton-Schulz iterate: X = U / (|U|_F + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T (of the shorter side).
 
     updates: a matrix, a stack (count, rows, cols), or a list of matrices of any shapes; bf16 / fp16 / fp32, any strides, one device. Returns new contiguous
-    tensors, laid out alike. coefficients: (a, b, c) or one triple per step. Arithmetic is fp32 whatever the type; the result is rounded once. A matrix of
-    zeros stays zero; NaN or infinity spoils its own matrix only. Not differentiable."""
+    tensors, laid out alike. coefficients: (a, b, c) or one triple per step. A matrix of zeros stays zero; NaN or infinity spoils its own matrix only. Not
+    differentiable.
+
+    Sums are fp32 whatever the type, operands are held to 22 bits at one exponent per matrix, the result is rounded once: the error is that of fp32 arithmetic
+    relative to the matrix (2e-6 of its norm), not to each number - a row 1e-5 below the others keeps some 15 bits, 1e-7 below 9. The same call gives the
+    same bits; beside other matrices, whose sizes decide how the products are cut, a matrix's last bits may be others."""
     one = isinstance(updates, torch.Tensor)
     if one and updates.dim() not in (2, 3):
         raise ValueError(f"orthogonalize: a matrix, a stack of matrices or a list of matrices, got shape {tuple(updates.shape)}")

@@ -162,7 +162,9 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int
     sections: pairs of features that each axis turns, in order; pair i of an axis with s pairs turns by position * base^(-i / s), or - `shared` - the
     P pairs of all axes share one ladder, pair j turns by position * base^(-j / P). layout: pair j is features (2j, 2j + 1), "pairs", or (j, P + j),
     "halves". Features behind the 2P turned ones are copied.
-    Angles are reduced in 64 bits (exact positions up to 2^53); products are fp32, rounded once to the tensor's type."""
+    Positions are read exactly up to 2^53. An angle is a number of turns in 64 bits, the product of the position and the rate: it is off by some 2^-52
+    of itself - at the highest rate 4e-11 of a turn at position 10^6, 0.04 at 10^15 - and loses its whole turns there. What is left of it, its cosine and its
+    sine are fp32, as are the products, which are rounded once to the tensor's type."""
     turn = _turn(tuple(map(int, sections)), float(base), str(layout), bool(shared), bool(inverse))  # plain values: the cache keeps none that can change
     _check(q, k, positions, turn)
     L.refuse_tangents("rotary", (q, k, positions))
