@@ -216,10 +216,15 @@ def require_cuda(x: torch.Tensor, what: str) -> None:
         raise RuntimeError(f"v1t_amd {what}: tensor is on {x.device}; the HIP path needs a GPU tensor (no CPU fallback).")
 
 
+def dual_level() -> bool:
+    """Whether tensors may carry a tangent (torch.autograd.forward_ad)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
 def refuse_tangents(what: str, tensors) -> None:
-    """Called by operators whose kernels read and write raw pointers: a dual tensor's tangent (torch.autograd.forward_ad) would be lost without a word, which reads as a derivative of
-    zero. Outside every dual level - where no tensor has one - it is a single comparison."""
-    if getattr(forward_ad, "_current_level", 0) >= 0 and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+    """Called within a dual level by operators whose kernels read and write raw pointers: a dual tensor's tangent would be lost without a word, which reads as a
+    derivative of zero."""
+    if any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors):
         raise NotImplementedError(f"v1t_amd {what}: forward-mode differentiation is not supported (a tensor carries a tangent)")
 
 

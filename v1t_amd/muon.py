@@ -86,7 +86,8 @@ def orthogonalize(updates, *, steps: int = 5, coefficients=COEFFICIENTS, eps: fl
             raise ValueError("orthogonalize: updates on several devices")
         if torch.is_grad_enabled() and u.requires_grad:
             raise RuntimeError("orthogonalize: not differentiable; call it under torch.no_grad() or on detached tensors")
-    L.refuse_tangents("orthogonalize", us)
+    if L.dual_level():
+        L.refuse_tangents("orthogonalize", us)
     if not us:
         return updates.clone() if one else []
     L.require_cuda(us[0], "orthogonalize")
@@ -160,7 +161,8 @@ def muon_step(params: t.Sequence[torch.Tensor], grads: t.Sequence[torch.Tensor],
         if x < end:
             raise ValueError("muon_step: tensors of the call share memory")
         end = y
-    L.refuse_tangents("muon_step", params + grads + moments)
+    if L.dual_level():
+        L.refuse_tangents("muon_step", params + grads + moments)
     if not rs:
         return
     L.require_cuda(params[0], "muon_step")

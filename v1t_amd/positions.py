@@ -103,7 +103,8 @@ def _like(x: torch.Tensor) -> torch.Tensor:
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
-    x = x.resolve_neg()  # the imaginary part of a conjugate view holds its numbers with the other sign
+    if x.is_neg():  # the imaginary part of a conjugate view holds its numbers with the other sign
+        x = x.resolve_neg()
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
@@ -116,14 +117,16 @@ class _RotaryFn(torch.autograd.Function):
         xs = [_rows(x) for x in (q, k) if x is not None]
         ys = [_like(x) for x in xs]
         _launch(turn, positions, list(zip(xs, ys)))
-        ctx.mark_non_differentiable(*(y for i, y in enumerate(ys) if not ctx.needs_input_grad[2 + i]))
+        if k is not None and q.requires_grad != k.requires_grad:
+            ctx.mark_non_differentiable(ys[q.requires_grad])
         return ys[0] if k is None else tuple(ys)
 
     @staticmethod
     def backward(ctx, *grads):
         """A rotation is orthogonal: the gradient turns back. Differentiable itself (a second derivative turns forward again)."""
         (positions,) = ctx.saved_tensors
-        L.refuse_tangents("rotary", grads)
+        if L.dual_level():
+            L.refuse_tangents("rotary", grads)
         back = _back(ctx.turn)
         out: t.List[t.Optional[torch.Tensor]] = [None, None]
         which = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[2 + i]]
@@ -167,9 +170,11 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int
     sine are fp32, as are the products, which are rounded once to the tensor's type."""
     turn = _turn(tuple(map(int, sections)), float(base), str(layout), bool(shared), bool(inverse))  # plain values: the cache keeps none that can change
     _check(q, k, positions, turn)
-    L.refuse_tangents("rotary", (q, k, positions))
+    if L.dual_level():
+        L.refuse_tangents("rotary", (q, k, positions))
     L.require_cuda(q, "rotary")
-    positions = positions.resolve_neg()
+    if positions.is_neg():
+        positions = positions.resolve_neg()
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _apply(turn, positions, q, k)
     xs = [_rows(x) for x in (q, k) if x is not None]
@@ -214,7 +219,8 @@ def rotary_(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[in
             raise ValueError(f"rotary_: elements of an expanded or overlapping view cannot be turned in place, got shape {tuple(x.shape)}, strides {x.stride()}")
     if k is not None and not _apart(q, k):
         raise ValueError("rotary_: q and k share elements")
-    L.refuse_tangents("rotary_", (q, k, positions))
+    if L.dual_level():
+        L.refuse_tangents("rotary_", (q, k, positions))
     L.require_cuda(q, "rotary_")
     _launch(turn, positions.resolve_neg(), [(x, x) for x in xs])
     for x in xs:
