@@ -184,7 +184,8 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int
 
 
 def _apart(q: torch.Tensor, k: torch.Tensor) -> bool:
-    """Whether no element of q is one of k: whole ranges apart, or - views of one packed projection - apart within every token's row."""
+    """Whether no element of q is one of k: whole ranges apart, or - views of one packed projection - q's and k's heads beside each other in every token's
+    row, or head by head in turn. (Neither overlaps itself.)"""
     if q.numel() == 0 or k.numel() == 0 or q.untyped_storage().data_ptr() != k.untyped_storage().data_ptr():
         return True
 
@@ -195,9 +196,25 @@ def _apart(q: torch.Tensor, k: torch.Tensor) -> bool:
     (lo, x), (hi, y) = ((a, q), (b, k)) if a <= b else ((b, k), (a, q))
     if lo + extent(x, 0) <= hi:
         return True
-    outer = [(n, s) for n, s in zip(x.shape[:-2], x.stride()[:-2]) if n > 1]
-    same = outer == [(n, s) for n, s in zip(y.shape[:-2], y.stride()[:-2]) if n > 1]
-    return same and lo + extent(x, -2) <= hi and hi - lo + extent(y, -2) <= min((s for _, s in outer), default=1 << 62)
+    # the blocks of the inner dimensions lie at multiples of the same outer strides, which count like digits; what is left of the distance sets y's behind x's
+    for inner in (-2, -1):
+        outer = []
+        for n, m, s, t in zip(x.shape[:inner], y.shape[:inner], x.stride(), y.stride()):
+            if n > 1 and m > 1 and s != t:
+                break
+            if max(n, m) > 1:
+                outer.append((s if n > 1 else t, n, m))
+        else:
+            left, above = hi - lo, 1 << 62
+            for s, n, m in sorted(outer, reverse=True):
+                ahead, left = divmod(left, s)
+                if max(n, m + ahead) * s > above:
+                    break
+                above = s
+            else:
+                if extent(x, inner) <= left and left + extent(y, inner) <= above:
+                    return True
+    return False
 
 
 def rotary_(q: torch.Tensor, positions: torch.Tensor, *, sections: t.Sequence[int], k: t.Optional[torch.Tensor] = None, base: float = 10000.0,
