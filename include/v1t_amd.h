@@ -168,7 +168,7 @@ int v1t_gaussian2d_backward(const float* z, long long zsb, long long zsc, int B,
                             float* dbias, void* stream);
 /* Same with `ws` = v1t_gaussian2d_backward_ws_bytes() bytes of scratch: the taps are sorted by cell and neuron (per image) into the scratch
  * and dz is summed per run of equal cells, in a fixed order (the same bits in every pass), instead of by 4*C*N*B float atomics (317 MB at
- * N = 8000, B = 16). The form the training path uses. */
+ * N = 8000, B = 16). The form the training path uses. Maps of more than 4096 cells, and calls without a scratch, take the atomics. */
 long long v1t_gaussian2d_backward_ws_bytes(int B, int H, int W, int N);
 int v1t_gaussian2d_backward_ws(const float* z, long long zsb, long long zsc, int B, int C, int H, int W,
                                int N, const float* grid, const float* feat, int FS, const float* gout,
